@@ -7,6 +7,7 @@ layouts, conv2d unfold kernels) through the C ABI declared in include/dfdx_b200.
 from . import _lib
 from ._lib import (AMP_F16, F16, F32, F64, PATH_AUTO, PATH_SIMT, PATH_TENSOR, B200Error, Conv2DOp)
 from .cuda import Cuda, ShapeMismatch, conv2d_out_dim
+from .heads import KvCache, Rotary
 
-__all__ = ["Cuda", "ShapeMismatch", "conv2d_out_dim", "Conv2DOp", "B200Error", "F32", "F64", "F16", "AMP_F16",
+__all__ = ["Cuda", "KvCache", "Rotary", "ShapeMismatch", "conv2d_out_dim", "Conv2DOp", "B200Error", "F32", "F64", "F16", "AMP_F16",
            "PATH_AUTO", "PATH_SIMT", "PATH_TENSOR", "_lib"]

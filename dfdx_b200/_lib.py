@@ -16,7 +16,7 @@ PATH_AUTO, PATH_SIMT, PATH_TENSOR = 0, 1, 2
 # b200_status
 OK = 0
 ERR_SHAPE, ERR_STRIDE, ERR_DTYPE, ERR_NULL, ERR_WORKSPACE = -1, -2, -3, -4, -5
-ERR_CUDA, ERR_DEVICE_TIMEOUT, ERR_UNSUPPORTED, ERR_NOT_CONTIGUOUS, ERR_LIMIT = -6, -7, -8, -9, -10
+ERR_CUDA, ERR_DEVICE_TIMEOUT, ERR_UNSUPPORTED, ERR_NOT_CONTIGUOUS, ERR_LIMIT, ERR_INDEX = -6, -7, -8, -9, -10, -11
 
 
 # b200_activation
@@ -39,6 +39,24 @@ class Conv1DOp(C.Structure):
     """Bit-identical to dfdx's `Conv1DOp` (dfdx-core/src/tensor_ops/conv1d/mod.rs:12-23)."""
     _fields_ = [(n, C.c_size_t) for n in (
         "kernel", "stride", "padding", "dilation", "groups", "batch", "chan_in", "chan_out", "l_in", "l_out")]
+
+
+class HeadOp(C.Structure):
+    """`b200_head_op`: norm and rotation of query / key heads."""
+    _fields_ = [("frequencies", C.c_void_p), ("axis_pairs", C.c_size_t * 3), ("interleaved", C.c_int), ("normalize", C.c_int),
+                ("epsilon", C.c_double), ("q_gain", C.c_void_p), ("k_gain", C.c_void_p)]
+
+
+class KvCacheView(C.Structure):
+    """`b200_kv_cache`: the paged 8-bit key/value cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_size_t), ("heads", C.c_size_t), ("page_size", C.c_size_t), ("d", C.c_size_t)]
+
+
+class KvBatch(C.Structure):
+    """`b200_kv_batch`: a ragged batch of new tokens."""
+    _fields_ = [("seqs", C.c_size_t), ("tokens", C.c_size_t), ("max_new", C.c_size_t), ("cu_tokens", C.c_void_p),
+                ("seq_lens", C.c_void_p), ("page_table", C.c_void_p), ("page_table_stride", C.c_size_t), ("max_pages", C.c_size_t)]
 
 
 _sz, _vp, _i, _d = C.c_size_t, C.c_void_p, C.c_int, C.c_double
@@ -93,6 +111,17 @@ SIGNATURES = {
     "b200_attention_backward_workspace_bytes": (_sz, [_sz, _sz, _sz]),
     "b200_attention_backward": (_i, [_i, _sz, _sz, _sz, _sz, _sz, _vp, _szp, _vp, _szp, _vp, _szp, _d, _vp, _szp, _vp,
                                      _vp, _szp, _vp, _szp, _vp, _szp, _vp, _szp, _i, _vp, _sz, _vp]),
+    "b200_qk_norm_rotary_forward": (_i, [_i, C.POINTER(HeadOp), _sz, _sz, _sz, _sz, _sz, _vp, _szp, _vp, _szp, _vp, _vp, _szp,
+                                         _vp, _szp, _vp]),
+    "b200_qk_norm_rotary_backward_workspace_bytes": (_sz, [_sz]),
+    "b200_qk_norm_rotary_backward": (_i, [_i, C.POINTER(HeadOp), _sz, _sz, _sz, _sz, _sz, _vp, _szp, _vp, _szp, _vp, _vp, _szp,
+                                          _vp, _szp, _vp, _szp, _vp, _szp, _vp, _vp, _i, _vp, _sz, _vp]),
+    "b200_kv_cache_append": (_i, [_i, C.POINTER(KvCacheView), C.POINTER(KvBatch), C.POINTER(HeadOp), _sz, _vp, _szp, _vp, _szp,
+                                  _vp, _szp, _vp, _vp, _szp, _vp]),
+    "b200_kv_cache_read": (_i, [_i, C.POINTER(KvCacheView), _sz, _vp, _vp, _vp, _vp]),
+    "b200_kv_cache_attention_workspace_bytes": (_sz, [C.POINTER(KvCacheView), C.POINTER(KvBatch), _sz, _i, _sz]),
+    "b200_kv_cache_attention": (_i, [_i, C.POINTER(KvCacheView), C.POINTER(KvBatch), _sz, _vp, _szp, _d, _i, _sz, _vp, _szp, _vp,
+                                     _vp, _sz, _vp]),
     "b200_conv2d_workspace_bytes": (_sz, [_i, C.POINTER(Conv2DOp), _i]),
     "b200_conv2d_forward": (_i, [_i, C.POINTER(Conv2DOp), _vp, _szp, _vp, _vp, _vp, _sz, _vp]),
     "b200_conv2d_backward": (_i, [_i, C.POINTER(Conv2DOp), _vp, _vp, _vp, _szp, _vp, _vp, _vp, _sz, _vp, _vp]),

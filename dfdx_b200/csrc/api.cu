@@ -154,6 +154,7 @@ const char* b200_strerror(int status) {
     case B200_ERR_UNSUPPORTED: return "unsupported on the requested path";
     case B200_ERR_NOT_CONTIGUOUS: return "image & filter inputs to conv2d must be contiguous";
     case B200_ERR_LIMIT: return "request exceeds a fixed capacity";
+    case B200_ERR_INDEX: return "an index read on the device was out of range; what it named was skipped";
     default: return "unknown status";
   }
 }
@@ -578,6 +579,144 @@ int b200_attention_backward(int dtype, size_t batch, size_t heads, size_t s1, si
   return attention_backward(dtype, (int64_t)batch, (int64_t)heads, (int64_t)s1, (int64_t)s2, (int64_t)d, q, a[0], k, a[1], v,
                             a[2], alpha, out, a[3], lse, grad_out, a[4], grad_q, a[5], grad_k, a[6], grad_v, a[7],
                             accumulate, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+// ---- queries and keys before attention -------------------------------------------------------------
+// The pointer and the strides of one (batch, token, head, element) view of an operand that is needed.
+static int check_heads_view(const void* p, const size_t s[4], size_t batch, size_t tokens, size_t heads, bool written) {
+  if (!p || !s) return B200_ERR_NULL;
+  if (s[3] != 1) return B200_ERR_UNSUPPORTED;
+  const size_t n[3] = {batch, tokens, heads};
+  for (int i = 0; i < 3; ++i) {
+    if (written && n[i] > 1 && s[i] == 0) return B200_ERR_STRIDE;
+    if (s[i] > ((size_t)1 << 40)) return B200_ERR_LIMIT;
+  }
+  return B200_OK;
+}
+
+static int qk_norm_rotary_call(int dtype, const b200_head_op* op, size_t batch, size_t tokens, size_t q_heads, size_t k_heads,
+                               size_t d, const void* const in[4], const size_t* const in_s[4], const int32_t* positions,
+                               void* const out[2], const size_t* const out_s[2], bool backward, float* q_gain_grad,
+                               float* k_gain_grad, int accumulate, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(dtype)) return B200_ERR_DTYPE;
+  if (dtype == B200_F64) return B200_ERR_UNSUPPORTED;
+  if (!op) return B200_ERR_NULL;
+  if (d == 0 || d % 2 || d > 256) return B200_ERR_UNSUPPORTED;
+  if (batch > 0x7fffffff || tokens > 0x7fffffff || batch * tokens > 0x3fffffff || q_heads > 0xffff || k_heads > 0xffff) return B200_ERR_LIMIT;
+  if (!op->normalize && (q_gain_grad || k_gain_grad)) return B200_ERR_UNSUPPORTED;
+  // an empty batch has gradients too: sums over nothing
+  const size_t heads[2] = {q_heads, k_heads};
+  int64_t is[4][3] = {}, os[2][3] = {};
+  int rc;
+  const bool empty = batch * tokens == 0;
+  for (int i = 0; i < (backward ? 4 : 2); ++i) {
+    if (empty || heads[i & 1] == 0) continue;
+    if ((rc = check_heads_view(in[i], in_s[i], batch, tokens, heads[i & 1], false))) return rc;
+    for (int a = 0; a < 3; ++a) is[i][a] = (int64_t)in_s[i][a];
+  }
+  for (int i = 0; i < 2; ++i) {
+    if (empty || heads[i] == 0) continue;
+    if ((rc = check_heads_view(out[i], out_s[i], batch, tokens, heads[i], true))) return rc;
+    for (int a = 0; a < 3; ++a) os[i][a] = (int64_t)out_s[i][a];
+  }
+  if (q_gain_grad || k_gain_grad) {
+    if (!workspace || ((uintptr_t)workspace & 15)) return B200_ERR_NULL;
+    if (workspace_bytes < qk_norm_rotary_backward_workspace_bytes((int64_t)d)) return B200_ERR_WORKSPACE;
+  }
+  return qk_norm_rotary(dtype, op, (int64_t)batch, (int64_t)tokens, (int64_t)q_heads, (int64_t)k_heads, (int64_t)d, in, is, positions,
+                        out, os, backward, q_gain_grad, k_gain_grad, accumulate, workspace, (cudaStream_t)stream);
+}
+
+int b200_qk_norm_rotary_forward(int dtype, const b200_head_op* op, size_t batch, size_t tokens, size_t q_heads, size_t k_heads,
+                                size_t d, const void* q, const size_t qs[4], const void* k, const size_t ks[4],
+                                const int32_t* positions, void* q_out, const size_t qos[4], void* k_out, const size_t kos[4],
+                                void* stream) {
+  const void* const in[4] = {q, k, nullptr, nullptr};
+  const size_t* const in_s[4] = {qs, ks, nullptr, nullptr};
+  void* const out[2] = {q_out, k_out};
+  const size_t* const out_s[2] = {qos, kos};
+  return qk_norm_rotary_call(dtype, op, batch, tokens, q_heads, k_heads, d, in, in_s, positions, out, out_s, false, nullptr, nullptr,
+                             0, nullptr, 0, stream);
+}
+
+size_t b200_qk_norm_rotary_backward_workspace_bytes(size_t d) {
+  return d > 256 ? 0 : qk_norm_rotary_backward_workspace_bytes((int64_t)d);
+}
+
+int b200_qk_norm_rotary_backward(int dtype, const b200_head_op* op, size_t batch, size_t tokens, size_t q_heads, size_t k_heads,
+                                 size_t d, const void* q, const size_t qs[4], const void* k, const size_t ks[4],
+                                 const int32_t* positions, const void* q_grad_out, const size_t gqs[4], const void* k_grad_out,
+                                 const size_t gks[4], void* grad_q, const size_t gqos[4], void* grad_k, const size_t gkos[4],
+                                 float* q_gain_grad, float* k_gain_grad, int accumulate, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  const void* const in[4] = {q, k, q_grad_out, k_grad_out};
+  const size_t* const in_s[4] = {qs, ks, gqs, gks};
+  void* const out[2] = {grad_q, grad_k};
+  const size_t* const out_s[2] = {gqos, gkos};
+  return qk_norm_rotary_call(dtype, op, batch, tokens, q_heads, k_heads, d, in, in_s, positions, out, out_s, true, q_gain_grad,
+                             k_gain_grad, accumulate, workspace, workspace_bytes, stream);
+}
+
+// ---- paged 8-bit key/value cache -------------------------------------------------------------------
+static int check_token_view(const size_t s[3], int64_t to[2], size_t tokens, size_t heads, bool written) {
+  if (!s) return B200_ERR_NULL;
+  if (s[2] != 1) return B200_ERR_UNSUPPORTED;
+  const size_t n[2] = {tokens, heads};
+  for (int i = 0; i < 2; ++i) {
+    if (written && n[i] > 1 && s[i] == 0) return B200_ERR_STRIDE;
+    if (s[i] > ((size_t)1 << 40)) return B200_ERR_LIMIT;
+    to[i] = (int64_t)s[i];
+  }
+  return B200_OK;
+}
+
+int b200_kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* batch, const b200_head_op* op, size_t q_heads,
+                         const void* q, const size_t qs[3], const void* k, const size_t ks[3], const void* v, const size_t vs[3],
+                         const int32_t* positions, void* q_out, const size_t qos[3], void* stream) {
+  if (!valid_dtype(dtype)) return B200_ERR_DTYPE;
+  if (dtype == B200_F64) return B200_ERR_UNSUPPORTED;
+  if (!cache || !batch) return B200_ERR_NULL;
+  int64_t a[4][2] = {};
+  int rc;
+  if ((rc = check_token_view(ks, a[1], batch->tokens, cache->heads, false))) return rc;
+  if ((rc = check_token_view(vs, a[2], batch->tokens, cache->heads, false))) return rc;
+  if (q) {
+    if (q_heads == 0 || q_heads > 0xffff) return B200_ERR_SHAPE;
+    if (!q_out) return B200_ERR_NULL;
+    if ((rc = check_token_view(qs, a[0], batch->tokens, q_heads, false))) return rc;
+    if ((rc = check_token_view(qos, a[3], batch->tokens, q_heads, true))) return rc;
+  }
+  return kv_cache_append(dtype, cache, batch, op, (int64_t)q_heads, q, a[0], k, a[1], v, a[2], positions, q_out, a[3], (cudaStream_t)stream);
+}
+
+int b200_kv_cache_read(int dtype, const b200_kv_cache* cache, size_t n, const int32_t* pages, void* k_out, void* v_out, void* stream) {
+  if (!valid_dtype(dtype)) return B200_ERR_DTYPE;
+  if (dtype == B200_F64) return B200_ERR_UNSUPPORTED;
+  if (n && (!pages || !k_out || !v_out)) return B200_ERR_NULL;
+  if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return B200_ERR_UNSUPPORTED;
+  if (n > 0x3fffffff) return B200_ERR_LIMIT;
+  return kv_cache_read(dtype, cache, (int64_t)n, pages, k_out, v_out, (cudaStream_t)stream);
+}
+
+size_t b200_kv_cache_attention_workspace_bytes(const b200_kv_cache* cache, const b200_kv_batch* batch, size_t q_heads, int causal,
+                                               size_t window) {
+  if (!cache || !batch || q_heads > 0xffff || window > 0x3fffffff) return 0;
+  return kv_cache_attention_workspace_bytes(cache, batch, (int64_t)q_heads, (int64_t)window, causal);
+}
+
+int b200_kv_cache_attention(int dtype, const b200_kv_cache* cache, const b200_kv_batch* batch, size_t q_heads, const void* q,
+                            const size_t qs[3], double alpha, int causal, size_t window, void* out, const size_t os[3], float* lse,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(dtype)) return B200_ERR_DTYPE;
+  if (!cache || !batch) return B200_ERR_NULL;
+  if (q_heads == 0 || q_heads > 0xffff) return B200_ERR_SHAPE;
+  if (window > 0x3fffffff) return B200_ERR_LIMIT;
+  int64_t a[2][2];
+  int rc;
+  if ((rc = check_token_view(qs, a[0], batch->tokens, q_heads, false))) return rc;
+  if ((rc = check_token_view(os, a[1], batch->tokens, q_heads, true))) return rc;
+  return kv_cache_attention(dtype, cache, batch, (int64_t)q_heads, q, a[0], alpha, causal, (int64_t)window, out, a[1], lse, workspace,
+                            workspace_bytes, (cudaStream_t)stream);
 }
 
 int b200_matmat_batch4_forward(int dtype, size_t batch, size_t seq, size_t m, size_t k, size_t n,

@@ -107,6 +107,22 @@ int softmax_backward(int dtype, int64_t rows, int64_t cols, const void* y, int64
                      double alpha, void* gx, int64_t gx_ld, int accumulate, cudaStream_t stream);
 int column_sum(int dtype, int64_t rows, int64_t cols, const void* g, int64_t ld, float* out, cudaStream_t stream);
 
+// Norm and rotation of query / key heads (rotary.cu), the paged 8-bit cache (kv_cache.cu) and the attention over it
+// (kv_attention.cu); strides in elements without the unit last one.
+size_t qk_norm_rotary_backward_workspace_bytes(int64_t d);
+int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t d,
+                   const void* const in[4], const int64_t in_strides[4][3], const int32_t* positions, void* const out[2],
+                   const int64_t out_strides[2][3], bool backward, float* q_gain_grad, float* k_gain_grad, int accumulate,
+                   void* workspace, cudaStream_t stream);
+int kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* batch, const b200_head_op* op, int64_t q_heads,
+                    const void* q, const int64_t qs[2], const void* k, const int64_t ks[2], const void* v, const int64_t vs[2],
+                    const int32_t* positions, void* q_out, const int64_t qos[2], cudaStream_t stream);
+int kv_cache_read(int dtype, const b200_kv_cache* cache, int64_t n, const int32_t* pages, void* k_out, void* v_out, cudaStream_t stream);
+size_t kv_cache_attention_workspace_bytes(const b200_kv_cache* cache, const b200_kv_batch* batch, int64_t q_heads, int64_t window, int causal);
+int kv_cache_attention(int dtype, const b200_kv_cache* cache, const b200_kv_batch* batch, int64_t q_heads, const void* q,
+                       const int64_t qs[2], double alpha, int causal, int64_t window, void* out, const int64_t os[2], float* lse,
+                       void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
 // Lowers one problem to a kernel family according to b200_set_path and eligibility.
 int run_gemm(const GemmProblem& p, cudaStream_t stream);
 int current_path();                          // b200_path in force

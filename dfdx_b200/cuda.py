@@ -16,12 +16,9 @@ import torch
 
 from . import _lib
 from ._lib import Conv1DOp, Conv2DOp, check, strides as _st
+from .heads import HeadOps, ShapeMismatch
 
 _DTYPES = {torch.float32: _lib.F32, torch.float64: _lib.F64, torch.float16: _lib.F16}
-
-
-class ShapeMismatch(AssertionError):
-    """Raised where the reference panics with `assertion left == right failed` before any launch."""
 
 
 def _assert_eq(left, right):
@@ -37,7 +34,7 @@ def conv2d_out_dim(dim: int, kernel: int, stride: int, padding: int, dilation: i
     return (dim + 2 * padding - span) // stride + 1
 
 
-class Cuda:
+class Cuda(HeadOps):
     """One device ordinal, like `Cuda::try_build(ordinal, seed)` (tensor/cuda/device.rs:72-91)."""
 
     def __init__(self, ordinal: int = 0, amp: bool = False, par_stream: bool = False):

@@ -48,7 +48,9 @@ typedef enum {
   B200_ERR_DEVICE_TIMEOUT = -7, /* a bounded device-side wait expired (reported by b200_device_status) */
   B200_ERR_UNSUPPORTED = -8,
   B200_ERR_NOT_CONTIGUOUS = -9, /* conv2d: "Image & filter inputs to conv2d must be contiguous" (conv2d/mod.rs:287-289) */
-  B200_ERR_LIMIT = -10          /* request exceeds a documented fixed capacity */
+  B200_ERR_LIMIT = -10,         /* request exceeds a documented fixed capacity */
+  B200_ERR_INDEX = -11          /* a page, length or token index that a kernel read on the device was out of range; the
+                                   work it named was skipped (reported by b200_device_status) */
 } b200_status;
 
 /* Mirrors `Conv2DOp` bit for bit: 12 x usize, #[repr(C)]
@@ -105,7 +107,8 @@ const char* b200_strerror(int status);
 /* Text of the last CUDA error seen by this thread inside the library ("" if none). */
 const char* b200_last_cuda_error(void);
 /* Reads (and clears) the device-side status word of the current device after synchronising
- * `stream`: 0, or B200_ERR_DEVICE_TIMEOUT if any kernel gave up on a bounded wait. */
+ * `stream`: 0, B200_ERR_DEVICE_TIMEOUT if any kernel gave up on a bounded wait, or B200_ERR_INDEX if one met an index
+ * outside its buffers; the latest of several. */
 int b200_device_status(void* stream);
 /* Process-wide override of kernel-family selection (testing / profiling). */
 int b200_set_path(int path);
@@ -423,6 +426,112 @@ int b200_softmax_forward(int dtype, size_t rows, size_t cols, const void* x, siz
 int b200_softmax_backward(int dtype, size_t rows, size_t cols, const void* y, size_t y_ld,
                           const void* grad_out, size_t grad_out_ld, double alpha,
                           void* grad_x, size_t grad_x_ld, int accumulate, void* stream);
+
+/* ---- queries and keys before attention (API additions) ---------------------------------------------- */
+
+/* What happens to every query and key head between the projections and the attention (MultiHeadAttention,
+ * dfdx/src/nn/layers/multi_head_attention.rs:118-136, has nothing there):
+ *     h = x / sqrt(mean(x^2) + epsilon) * gain                                            if normalize != 0
+ *     (y_a, y_b) = (h_a cos t - h_b sin t, h_b cos t + h_a sin t),  t = position[axis(i)] * frequencies[i]
+ * for each of the sum(axis_pairs) rotated pairs i.  Pair i's elements are (i, i + pairs), or (2 i, 2 i + 1) when
+ * interleaved != 0; the elements behind the rotated ones pass through.  The first axis_pairs[0] pairs turn with position
+ * axis 0, the next axis_pairs[1] with axis 1, the others with axis 2 (e.g. time, height, width); a text model uses one axis.
+ *   frequencies : device pointer, radians per position of each pair in f64 (NULL without rotated pairs).  The angle is
+ *                 reduced in f64, so any 32-bit position is as exact as position 0.
+ *   q_gain, k_gain : d elements of the call's dtype each, or NULL for 1; only with normalize. */
+typedef struct {
+  const double* frequencies;
+  size_t axis_pairs[3];
+  int interleaved;
+  int normalize;
+  double epsilon;
+  const void* q_gain;
+  const void* k_gain;
+} b200_head_op;
+
+/* The transform above on all query and key heads in one pass.  q: (batch, tokens, q_heads, d) view, k: (batch, tokens,
+ * k_heads, d) view, likewise the outputs, which may be the inputs themselves; strides [batch, token, head, element], the
+ * last one 1, output strides non-zero over extents > 1 (B200_ERR_STRIDE).  positions: int32, axes x batch x tokens
+ * contiguous, `axes` being the last axis with rotated pairs; NULL: the index in the sequence, on every axis.
+ * f32 and f16 (f32 arithmetic, one rounding); even d <= 256, otherwise B200_ERR_UNSUPPORTED.  q_heads or k_heads may be 0. */
+int b200_qk_norm_rotary_forward(int dtype, const b200_head_op* op, size_t batch, size_t tokens, size_t q_heads, size_t k_heads,
+                                size_t d, const void* q, const size_t q_strides[4], const void* k, const size_t k_strides[4],
+                                const int32_t* positions, void* q_out, const size_t q_out_strides[4], void* k_out,
+                                const size_t k_out_strides[4], void* stream);
+
+/* Its backward: grad_q and grad_k are written (each may be the upstream gradient itself); q_gain_grad and k_gain_grad (f32, d elements,
+ * either may be NULL) are written, or added to when accumulate != 0.  The gains' sums over all rows have a fixed order:
+ * the same bits in every run.  A broadcast (stride 0) q or k gets the gradient of every element of the view.
+ * workspace: b200_qk_norm_rotary_backward_workspace_bytes(d) bytes, 16-byte aligned; not needed without gain gradients. */
+size_t b200_qk_norm_rotary_backward_workspace_bytes(size_t d);
+int b200_qk_norm_rotary_backward(int dtype, const b200_head_op* op, size_t batch, size_t tokens, size_t q_heads, size_t k_heads,
+                                 size_t d, const void* q, const size_t q_strides[4], const void* k, const size_t k_strides[4],
+                                 const int32_t* positions, const void* q_grad_out, const size_t q_grad_out_strides[4],
+                                 const void* k_grad_out, const size_t k_grad_out_strides[4], void* grad_q,
+                                 const size_t grad_q_strides[4], void* grad_k, const size_t grad_k_strides[4],
+                                 float* q_gain_grad, float* k_gain_grad, int accumulate, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* ---- paged 8-bit key/value cache (API additions) ------------------------------------------------------ */
+
+/* Keys and values of earlier tokens in pages of page_size slots.  k, v: e4m3 codes, (pages, heads, page_size, d)
+ * contiguous, 16-byte aligned; k_scale, v_scale: f32 (pages, heads), a power of two >= 2^-60 for each block of one page's
+ * slots and one head: value = code * scale.  page_size 16, 32, 64 or 128; d 32, 64, 96 or 128, otherwise
+ * B200_ERR_UNSUPPORTED.  A cache needs no initialisation: nothing is read from slots that no append has written.
+ * Infinities are held as +-448 * scale, NaN as NaN. */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  size_t pages, heads, page_size, d;
+} b200_kv_cache;
+
+/* A ragged batch of new tokens, several sequences' one after another.  Sequence s has the tokens
+ * [cu_tokens[s], cu_tokens[s + 1]) and, these included, seq_lens[s] slots in use: its j-th of m new tokens has slot
+ * seq_lens[s] - m + j.  Slot i lies in page page_table[s * page_table_stride + i / page_size].  The three arrays are int32
+ * on the device and are read by the kernels: a captured graph replays with what they hold then.  Entries of the page
+ * table behind a sequence's length are never read.  max_new: the most new tokens that a sequence has.  A sequence whose
+ * numbers do not fit (cu_tokens outside [0, tokens] or falling, more than max_new tokens, a length outside
+ * [0, max_pages * page_size]), and a page outside the cache, are skipped and reported as B200_ERR_INDEX by
+ * b200_device_status.  Tokens of no sequence are left alone, in outputs too. */
+typedef struct {
+  size_t seqs, tokens, max_new;
+  const int32_t* cu_tokens;
+  const int32_t* seq_lens;
+  const int32_t* page_table;
+  size_t page_table_stride, max_pages;
+} b200_kv_batch;
+
+/* Writes the new tokens' keys, transformed by `op` (NULL: as they are), and values into the cache, and their queries,
+ * transformed likewise, to q_out (q NULL: keys and values only), in one launch.  q: (tokens, q_heads, d) view; k, v:
+ * (tokens, cache heads, d) views; strides [token, head, element], the last 1.  positions: int32, axes x tokens, or
+ * NULL: the token's slot on every axis.  Codes are rounded to nearest, ties to even.  A block's scale is the smallest
+ * power of two that brings its largest finite magnitude to at most 448 codes; it starts anew with the block's first
+ * slot and never shrinks after; when it grows, the codes of the block's other slots move to it.  A page that several
+ * sequences share must be full before they append.  f32 and f16. */
+int b200_kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* batch, const b200_head_op* op, size_t q_heads,
+                         const void* q, const size_t q_strides[3], const void* k, const size_t k_strides[3], const void* v,
+                         const size_t v_strides[3], const int32_t* positions, void* q_out, const size_t q_out_strides[3],
+                         void* stream);
+
+/* Values of n pages (int32 ids on the device): k_out, v_out (n, heads, page_size, d) contiguous f16 or f32, 16-byte aligned.
+ * A page outside the cache reads as zeros and is reported as B200_ERR_INDEX. */
+int b200_kv_cache_read(int dtype, const b200_kv_cache* cache, size_t n, const int32_t* pages, void* k_out, void* v_out, void* stream);
+
+/* softmax(alpha * q K^T) V over the cache: token j of a sequence sees the slots up to its own (causal != 0), of these
+ * the last `window` ones if window != 0; or all seq_lens[s] slots (causal == 0, no window).  q, out: (tokens, q_heads,
+ * d) views, strides [token, head, element] with the last 1 and the others multiples of 8, 16-byte aligned; q_heads a
+ * multiple of the cache's heads, query head h reads key head h / (q_heads / heads).  lse: NULL or tokens x q_heads floats,
+ * log(sum exp(alpha * s)).  A token that sees no slot gets zeros and -infinity.  f16 / AMP f16 only; f32 softmax and sums.
+ * workspace: b200_kv_cache_attention_workspace_bytes() bytes, 16-byte aligned: the partial results of long sequences,
+ * whose length the page table's width (max_pages) bounds.  Results do not depend on the other sequences of the batch
+ * but for the order of sums, which follows from the batch's sizes; the same call gives the same bits. */
+size_t b200_kv_cache_attention_workspace_bytes(const b200_kv_cache* cache, const b200_kv_batch* batch, size_t q_heads,
+                                               int causal, size_t window);
+int b200_kv_cache_attention(int dtype, const b200_kv_cache* cache, const b200_kv_batch* batch, size_t q_heads, const void* q,
+                            const size_t q_strides[3], double alpha, int causal, size_t window, void* out,
+                            const size_t out_strides[3], float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- conv2d (unfold + GEMM lowering) ---------------------------------------------------------- */
 
