@@ -3,15 +3,15 @@
 //     o = softmax(alpha * q K^T) V   over the slots that the token may see,   K = ck * sk,  V = cv * sv
 //
 // with ck, cv the e4m3 codes and sk, sv their blocks' scales, powers of two.  The value scale goes into the exponent:
-// with  s' = alpha log2(e) sk (q . ck) + log2(sv),  m' a running maximum of s',  p' = 2^(s' - m' + 15):
+// with  s' = alpha log2(e) sk (q . ck) + log2(sv),  m' a running maximum of s',  p' = 2^(s' - m' + 14):
 //
-//     o = sum p' cv / l,     l = sum p' / sv,     log-sum-exp = ln 2 (m' - 15 + log2 l)
+//     o = sum p' cv / l,     l = sum p' / sv,     log-sum-exp = ln 2 (m' - 14 + log2 l)
 //
-// so the probabilities that meet the codes lie in [0, 2^15] whatever the scales are, and one pass keeps one maximum.
-// The lift by 2^15 uses f16's upper binades too: a probability keeps its 11 bits down to 2^-29 of the largest, which
-// matters where the most probable slot's values are small beside another's.
+// so the probabilities that meet the codes lie in [0, 2^15] whatever the scales are, and one pass keeps one maximum
+// (which may lag behind the largest s' by 1).  The lift by 2^14 uses f16's upper binades too: a probability keeps its 11
+// bits down to 2^-28 of the largest, which matters where the most probable slot's values are small beside another's.
 //
-//   kv_decode_kernel    few rows: bound by reading the codes.  A CTA has one (sequence, key head), up to 16 * MT of its
+//   kv_decode_kernel    few rows: bound by reading the codes.  A CTA has one (sequence, key head), up to 8 * NQ of its
 //                       rows (a row is a new token and one of the query heads that share the key head) and a range of
 //                       slots; each of its four warps walks 16 slots at a time on m16n8k16 f16 matrix instructions.
 //                       Codes go from global memory to registers directly: the order of the products' summation index
@@ -49,7 +49,7 @@ struct AttArgs {
 };
 
 constexpr int WARPS = 4;
-constexpr float LIFT = 15.f;       // log2 of the largest probability as the second product sees it
+constexpr float LIFT = 14.f;       // log2 of the probability at the running maximum, as the second product sees it
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -84,13 +84,14 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
     for (int i = 0; i < N; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
   }
 }
-__device__ __forceinline__ bool has_nan(uint32_t codes) {  // a byte that is 0x7f but for its sign
-  const uint32_t x = (codes & 0x7f7f7f7fu) + 0x01010101u;
-  return (x & 0x80808080u) != 0;
-}
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {    // 0xff where the code is NaN
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {    // 0xff where the code is NaN: 0x7f but for its sign
   const uint32_t x = (((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
   return x * 0xffu;
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {         // an 8 x 8 matrix of f16, two a lane
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // The slots that row r of a sequence sees: [lo, hi).
@@ -103,100 +104,128 @@ __device__ __forceinline__ View view_of(const AttArgs& g, const Seq& q, int r) {
   return v;
 }
 
-template <int D, int MT>
-__global__ void __launch_bounds__(WARPS * 32) kv_decode_kernel(const AttArgs g) {
-  constexpr int KS = D / 16;                               // k-steps of the scores' product
-  constexpr int NT = D / 8;                                // column tiles of the output
+// What a CTA of either kernel works on: a row tile of R rows of one (sequence, key head), and one of its ranges.
+struct Work {
+  Seq q;
+  int s, head, tile, rows;
+  int lo_tile, hi_tile;            // slots that some row sees
+  int lo_all, hi_all;              // slots that every row sees
+  int ranges, begin, end;          // ranges in use; this one's tiles of 16 slots
+};
+template <int R>
+__device__ __forceinline__ bool work_of(const AttArgs& g, unsigned unit, int x, Work& w) {
+  w.tile = (int)(unit % (unsigned)g.tiles); unit /= (unsigned)g.tiles;
+  w.head = (int)(unit % (unsigned)g.cache.heads);
+  w.s = (int)(unit / (unsigned)g.cache.heads);
+  if (w.s >= g.batch.seqs) return false;
+  w.q = load_seq(g.batch, g.cache, w.s);
+  if (!w.q.ok) {
+    if (threadIdx.x == 0) flag_index(g.status);
+    return false;
+  }
+  w.rows = min(w.q.m * g.group - w.tile * R, R);
+  if (w.rows <= 0) return false;
+  const View first = view_of(g, w.q, w.tile * R), last = view_of(g, w.q, w.tile * R + w.rows - 1);
+  w.lo_tile = first.lo; w.hi_tile = last.hi;
+  w.lo_all = last.lo; w.hi_all = first.hi;
+  const int first_range = w.lo_tile / g.range;
+  w.ranges = w.hi_tile > w.lo_tile ? (w.hi_tile - 1) / g.range - first_range + 1 : 1;
+  if (x >= w.ranges) return false;
+  w.begin = max(w.lo_tile, (first_range + x) * g.range) >> 4;
+  w.end = w.hi_tile > w.lo_tile ? (int)min((long long)w.hi_tile, (first_range + x + 1ll) * g.range) + 15 >> 4 : w.begin;
+  return true;
+}
+
+// NaN values in slots that only some rows of a tile see were taken out of the product; this puts them where they belong.
+// Rare enough to read the codes again: eight output elements of one row, over the tiles at the edges of the rows' views.
+__device__ __noinline__ void nan_fixup(const AttArgs& g, const Work& w, int row, int j, float (&v)[8]) {
+  const View view = view_of(g, w.q, row);
+  const int* table = g.batch.table + (long long)w.s * g.batch.table_stride;
+  for (int t = w.begin; t < w.end; ++t) {
+    if (t * 16 >= w.lo_all && t * 16 + 16 <= w.hi_all) continue;
+    const int id = table[(t << 4) >> g.cache.page_log2];
+    if (id < 0 || id >= g.cache.pages) continue;
+    for (int slot = max(t * 16, view.lo); slot < min(t * 16 + 16, view.hi); ++slot) {
+      const uint8_t* p = g.cache.v + (((long long)id * g.cache.heads + w.head) * g.cache.page + (slot & (g.cache.page - 1))) * g.cache.d + j;
+      for (int e = 0; e < 8; ++e)
+        if ((p[e] & 0x7f) == 0x7f) v[e] = NAN;
+    }
+  }
+}
+
+// NQ: eights of rows.  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T: the matrix instruction's 16-row
+// side then holds slots and head elements, which there are always enough of, and its 8-column side the few rows.
+template <int D, int NQ>
+__global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 4 : NQ == 2 ? 3 : 2) kv_decode_kernel(const __grid_constant__ AttArgs g) {
+  constexpr int KS = D / 16;                               // k-steps of S^T; also 16-element tiles of O^T
   constexpr int KW = D / 16;                               // words of a key row that a lane holds (D / 4 codes)
   constexpr int VW = D / 32;                               // words of a value row that a lane holds (D / 8 codes)
-  constexpr int R = 16 * MT;
-  __shared__ __align__(16) float sh_o[WARPS][16][D + 4];
-  __shared__ float sh_m[WARPS][16], sh_l[WARPS][16];
+  constexpr int R = 8 * NQ;
+  constexpr bool Q_REGS = NQ == 1;
+  __shared__ __align__(16) float sh_o[WARPS][8][D + 4];
+  __shared__ float sh_m[WARPS][8], sh_l[WARPS][8];
+  __shared__ __align__(16) uint2 sh_q[Q_REGS ? 1 : NQ * KS * 32];
+  __shared__ int sh_nan;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, c = lane & 3;
-  unsigned rest = blockIdx.x;
-  const int x = (int)(rest % (unsigned)g.splits); rest /= (unsigned)g.splits;
-  const int tile = (int)(rest % (unsigned)g.tiles); rest /= (unsigned)g.tiles;
-  const int head = (int)(rest % (unsigned)g.cache.heads), s = (int)(rest / (unsigned)g.cache.heads);
-  const Seq q = load_seq(g.batch, g.cache, s);
-  if (!q.ok) {
-    if (threadIdx.x == 0) flag_index(g.status);
-    return;
-  }
-  const int rows = min(q.m * g.group - tile * R, R);       // of this tile
-  if (rows <= 0) return;
-  const int lo_tile = view_of(g, q, tile * R).lo, hi_tile = view_of(g, q, tile * R + rows - 1).hi;
-  const int first_range = lo_tile / g.range;
-  const int ranges = hi_tile > lo_tile ? (hi_tile - 1) / g.range - first_range + 1 : 1;
-  if (x >= ranges) return;
-  const int begin = max(lo_tile, (first_range + x) * g.range) >> 4;          // in 16-slot tiles
-  const int end = hi_tile > lo_tile ? (min(hi_tile, (first_range + x + 1) * g.range) + 15) >> 4 : begin;
+  asm volatile("griddepcontrol.launch_dependents;");       // the joining kernel may be brought in; it waits for this one
+  Work w;
+  if (!work_of<R>(g, blockIdx.x / (unsigned)g.splits, (int)(blockIdx.x % (unsigned)g.splits), w)) return;
+  if (threadIdx.x == 0) sh_nan = 0;
 
-  // this lane's rows: gr and gr + 8 of every 16
-  uint32_t qf[MT][KS][4];
-  int lo[MT][2], hi[MT][2];
-  int lo_all = 0, hi_all = 0x7fffffff;                     // slots [lo_all, hi_all) are seen by every row of the tile
+  // the queries as the second operand: lane (gr, c) has row gr's elements c D / 4 + 4 ks .. + 3 at step ks, the same order
+  // of summation in which it reads the keys
+  uint2 qf[Q_REGS ? KS : 1];
+  auto query_of = [&](int r) -> const __half* {
+    const int row = w.tile * R + r;
+    return g.q + (long long)(w.q.first + row / g.group) * g.qt + (long long)(w.head * g.group + row % g.group) * g.qh;
+  };
+  if constexpr (Q_REGS) {
+    const __half* src = query_of(min(gr, w.rows - 1)) + c * (D / 4);
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = t * 16 + h * 8 + gr;
-      View v = {0, 0};
-      if (r < rows) {
-        const int row = tile * R + r;
-        v = view_of(g, q, row);
-        const __half* src = g.q + (long long)(q.first + row / g.group) * g.qt + (long long)(head * g.group + row % g.group) * g.qh + c * (D / 4);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const uint2 w = *reinterpret_cast<const uint2*>(src + ks * 4);
-          qf[t][ks][h] = w.x;
-          qf[t][ks][2 + h] = w.y;
-        }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qf[t][ks][h] = qf[t][ks][2 + h] = 0;
-      }
-      lo[t][h] = v.lo; hi[t][h] = v.hi;
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const uint2*>(src + ks * 4);
+  } else {
+    for (int i = threadIdx.x; i < NQ * KS * 32; i += WARPS * 32) {
+      const int l = i & 31, ks = (i >> 5) % KS, nt = (i >> 5) / KS;
+      sh_q[i] = *reinterpret_cast<const uint2*>(query_of(min(nt * 8 + (l >> 2), w.rows - 1)) + (l & 3) * (D / 4) + ks * 4);
     }
-  lo_all = view_of(g, q, tile * R + rows - 1).lo;
-  hi_all = view_of(g, q, tile * R).hi;
+  }
+  __syncthreads();
 
-  float o[MT][NT][4];
-  float m[MT][2], l[MT][2];
+  float o[NQ][KS][4];
+  float m[NQ][2], l[NQ][2];                                // of rows 2 c and 2 c + 1
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
+  for (int t = 0; t < NQ; ++t) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < KS; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[t][j][e] = 0.f;
     m[t][0] = m[t][1] = -INFINITY;
     l[t][0] = l[t][1] = 0.f;
   }
 
-  const int* table = g.batch.table + (long long)s * g.batch.table_stride;
+  const int* table = g.batch.table + (long long)w.s * g.batch.table_stride;
   const int in_page = g.cache.page - 1, shift = g.cache.page_log2;
-  for (int i0 = begin + warp; i0 < end; i0 += WARPS * 32) {
+  for (int i0 = w.begin + warp; i0 < w.end; i0 += WARPS * 32) {
     // the pages and scales of the warp's next 32 tiles, one a lane
     const int mine = i0 + lane * WARPS;
     int id = 0;
     float ks_l = 0.f, vs_l = 1.f;
     bool bad = false;
-    if (mine < end) {
+    if (mine < w.end) {
       id = table[(mine << 4) >> shift];
       bad = id < 0 || id >= g.cache.pages;
-      if (!bad) {
-        ks_l = g.cache.k_scale[(long long)id * g.cache.heads + head];
-        vs_l = g.cache.v_scale[(long long)id * g.cache.heads + head];
-      }
+      if (bad) id = 0;                                     // its slots count for nothing; the caller learns of it
+      ks_l = g.cache.k_scale[(long long)id * g.cache.heads + w.head] * g.scale_log2;
+      vs_l = g.cache.v_scale[(long long)id * g.cache.heads + w.head];
     }
-    if (__any_sync(0xffffffffu, bad)) {                    // its slots count for nothing; the caller learns of it
-      if (lane == 0) flag_index(g.status);
-    }
-    const int n = min(32, (end - i0 + WARPS - 1) / WARPS);
+    const uint32_t bad_tiles = __ballot_sync(0xffffffffu, bad);
+    if (bad_tiles && lane == 0) flag_index(g.status);
+    const int n = min(32, (w.end - i0 + WARPS - 1) / WARPS);
     uint32_t kw[2][KW], vw[4][VW];
     auto base_of = [&](int i) -> long long {               // byte offset of tile i's first row
-      const int page = max(__shfl_sync(0xffffffffu, bad ? -1 : id, i), 0);
-      return (((long long)page * g.cache.heads + head) * g.cache.page + (((i0 + i * WARPS) << 4) & in_page)) * D;
+      const int page = __shfl_sync(0xffffffffu, id, i);
+      return (((long long)page * g.cache.heads + w.head) * g.cache.page + (((i0 + i * WARPS) << 4) & in_page)) * D;
     };
     auto load_k = [&](long long at) {
 #pragma unroll
@@ -211,129 +240,97 @@ __global__ void __launch_bounds__(WARPS * 32) kv_decode_kernel(const AttArgs g) 
     load_v(at);
     for (int i = 0; i < n; ++i) {
       const int slot0 = (i0 + i * WARPS) << 4;
-      const bool tile_bad = __shfl_sync(0xffffffffu, (int)bad, i) != 0;
-      const float sk = __shfl_sync(0xffffffffu, ks_l, i) * g.scale_log2, sv = __shfl_sync(0xffffffffu, vs_l, i);
-      const float lsv = log2f(sv), inv_sv = 1.f / sv;      // sv is a power of two: both exact
-      float sc[MT][2][4];
+      const float sk = __shfl_sync(0xffffffffu, ks_l, i);
+      const uint32_t sv = __float_as_uint(__shfl_sync(0xffffffffu, vs_l, i));
+      const float lsv = (float)((int)(sv >> 23) - 127), inv_sv = __uint_as_float((254u << 23) - sv);   // a power of two
+      float sc[NQ][4];
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < NQ; ++t)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int e = 0; e < 4; ++e) sc[t][e] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[t][h][e] = 0.f;
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint32_t a0 = values2(kw[0][ks]), a1 = values2(kw[1][ks]), a2 = values2(kw[0][ks] >> 16), a3 = values2(kw[1][ks] >> 16);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t b0 = values2(kw[h][ks]), b1 = values2(kw[h][ks] >> 16);
-#pragma unroll
-          for (int t = 0; t < MT; ++t) mma16816(sc[t][h], qf[t][ks][0], qf[t][ks][1], qf[t][ks][2], qf[t][ks][3], b0, b1);
+        for (int t = 0; t < NQ; ++t) {
+          const uint2 b = Q_REGS ? qf[Q_REGS ? ks : 0] : sh_q[(t * KS + ks) * 32 + lane];
+          mma16816(sc[t], a0, a1, a2, a3, b.x, b.y);
         }
+      }
       const long long next = i + 1 < n ? base_of(i + 1) : at;
       if (i + 1 < n) load_k(next);
 
-      const bool edge = tile_bad || slot0 < lo_all || slot0 + 16 > hi_all;
-      uint32_t p[MT][4];
+      // sc: slots gr (0, 1) and gr + 8 (2, 3), rows 2 c (0, 2) and 2 c + 1 (1, 3)
+      const bool tile_bad = (bad_tiles >> i) & 1u;
+      const bool edge = tile_bad || slot0 < w.lo_all || slot0 + 16 > w.hi_all;
+      uint32_t pb[NQ][2];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
+      for (int t = 0; t < NQ; ++t) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[t][h][e] = fmaf(sc[t][h][e], sk, lsv);
+        for (int e = 0; e < 4; ++e) sc[t][e] = fmaf(sc[t][e], sk, lsv);
         if (edge) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int y = 0; y < 2; ++y) {
+            const int r = t * 8 + 2 * c + y;
+            const View v = view_of(g, w.q, w.tile * R + min(r, w.rows - 1));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int slot = slot0 + h * 8 + 2 * c + (e & 1);
-              if (tile_bad || slot < lo[t][e >> 1] || slot >= hi[t][e >> 1]) sc[t][h][e] = -INFINITY;
+            for (int h = 0; h < 2; ++h) {
+              const int slot = slot0 + h * 8 + gr;
+              if (tile_bad || slot < v.lo || slot >= v.hi) sc[t][2 * h + y] = -INFINITY;
             }
+          }
         }
-        float top[2];
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          top[y] = fmaxf(fmaxf(sc[t][0][2 * y], sc[t][0][2 * y + 1]), fmaxf(sc[t][1][2 * y], sc[t][1][2 * y + 1]));
-          top[y] = fmaxf(top[y], __shfl_xor_sync(0xffffffffu, top[y], 1));
-          top[y] = fmaxf(top[y], __shfl_xor_sync(0xffffffffu, top[y], 2));
-        }
-        if (__any_sync(0xffffffffu, top[0] > m[t][0] || top[1] > m[t][1])) {
+        // The maximum moves only when a score passes it by more than 1: most tiles then need neither its reduction over
+        // the slots nor a change of the sums, and probabilities stay below 2 * 2^LIFT.
+        if (__any_sync(0xffffffffu, fmaxf(sc[t][0], sc[t][2]) > m[t][0] + 1.f || fmaxf(sc[t][1], sc[t][3]) > m[t][1] + 1.f)) {
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const float now = fmaxf(m[t][y], top[y]);
+            float top = fmaxf(sc[t][y], sc[t][2 + y]);
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float now = fmaxf(m[t][y], top);
             const float f = now == -INFINITY ? 1.f : ex2(m[t][y] - now);
             m[t][y] = now;
             l[t][y] *= f;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) { o[t][j][2 * y] *= f; o[t][j][2 * y + 1] *= f; }
+            for (int j = 0; j < KS; ++j) { o[t][j][y] *= f; o[t][j][2 + y] *= f; }
           }
         }
+        float p[4];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const float nm = m[t][y] == -INFINITY ? 0.f : LIFT - m[t][y];
-          float sum = 0.f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float p0 = ex2(sc[t][h][2 * y] + nm), p1 = ex2(sc[t][h][2 * y + 1] + nm);
-            sum += p0 + p1;
-            p[t][2 * h + y] = half2_of(p0, p1);
-          }
-          l[t][y] = fmaf(sum, inv_sv, l[t][y]);
+          p[y] = ex2(sc[t][y] + nm);
+          p[2 + y] = ex2(sc[t][2 + y] + nm);
+          l[t][y] = fmaf(p[y] + p[2 + y], inv_sv, l[t][y]);
         }
+        pb[t][0] = transposed(half2_of(p[0], p[1]));
+        pb[t][1] = transposed(half2_of(p[2], p[3]));
       }
       if (edge) {
-        // A NaN among values that some row does not see must not reach it through 0 * NaN: such codes become 0 here, and
-        // a second product of "sees the slot" with "is NaN" finds the outputs that are NaN by right.
-        bool any = false;
+        // A NaN among values that some row does not see must not reach it through 0 * NaN: it is taken out here and put
+        // back at the end where it belongs.
+        uint32_t any = 0;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int w = 0; w < VW; ++w) any |= has_nan(vw[t][w]);
-        if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            uint32_t sees[4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                const int slot = slot0 + h * 8 + 2 * c;
-                const bool s0 = !tile_bad && slot >= lo[t][y] && slot < hi[t][y];
-                const bool s1 = !tile_bad && slot + 1 >= lo[t][y] && slot + 1 < hi[t][y];
-                sees[2 * h + y] = half2_of(s0 ? 1.f : 0.f, s1 ? 1.f : 0.f);
-              }
-#pragma unroll
-            for (int w = 0; w < VW; ++w)
-#pragma unroll
-              for (int b = 0; b < 4; ++b) {
-                uint32_t f[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) f[k] = (nan_bytes(vw[k][w]) >> (8 * b)) & 1u;
-                float hit[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816(hit, sees[0], sees[1], sees[2], sees[3], f[0] * 0x3c00u | f[1] * 0x3c000000u, f[2] * 0x3c00u | f[3] * 0x3c000000u);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (hit[e] != 0.f) o[t][w * 4 + b][e] = NAN;
-              }
+          for (int x = 0; x < VW; ++x) {
+            const uint32_t gone = nan_bytes(vw[t][x]);
+            any |= gone;
+            vw[t][x] &= ~gone;
           }
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vw[t][w] &= ~nan_bytes(vw[t][w]);
-        }
+        if (any) sh_nan = 1;
       }
 #pragma unroll
-      for (int w = 0; w < VW; ++w)
+      for (int x = 0; x < VW; ++x)
 #pragma unroll
-        for (int b = 0; b < 4; b += 2) {
-          // codes of columns 4 w + b and + 1: (slot, slot + 1) pairs side by side
+        for (int b = 0; b < 2; ++b) {
+          // codes 4 x + 2 b and + 1 of the lane's run: (slot, slot + 1) pairs side by side
           const uint32_t sel = b == 0 ? 0x5140u : 0x7362u;
-          const uint32_t x0 = __byte_perm(vw[0][w], vw[1][w], sel), x1 = __byte_perm(vw[2][w], vw[3][w], sel);
-          const uint32_t f0 = values2(x0), f1 = values2(x1), f2 = values2(x0 >> 16), f3 = values2(x1 >> 16);
+          const uint32_t x0 = __byte_perm(vw[0][x], vw[1][x], sel), x1 = __byte_perm(vw[2][x], vw[3][x], sel);
+          const uint32_t a0 = values2(x0), a1 = values2(x0 >> 16), a2 = values2(x1), a3 = values2(x1 >> 16);
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            mma16816(o[t][w * 4 + b], p[t][0], p[t][1], p[t][2], p[t][3], f0, f1);
-            mma16816(o[t][w * 4 + b + 1], p[t][0], p[t][1], p[t][2], p[t][3], f2, f3);
-          }
+          for (int t = 0; t < NQ; ++t) mma16816(o[t][2 * x + b], a0, a1, a2, a3, pb[t][0], pb[t][1]);
         }
       if (i + 1 < n) load_v(next);
       at = next;
@@ -341,42 +338,39 @@ __global__ void __launch_bounds__(WARPS * 32) kv_decode_kernel(const AttArgs g) 
   }
 
   // join the warps, then write the rows or leave them as a partial result
-  const bool whole = ranges == 1;
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
+  for (int t = 0; t < NQ; ++t) {
     __syncthreads();
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
       float sum = l[t][y];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const int r = y * 8 + gr;
-      if (c == 0) { sh_m[warp][r] = m[t][y]; sh_l[warp][r] = sum; }
-      // columns 2 c and 2 c + 1 of the column tiles are D / 4 consecutive elements of the row
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int x = 4; x < 32; x *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      const int r = 2 * c + y;
+      if (gr == 0) { sh_m[warp][r] = m[t][y]; sh_l[warp][r] = sum; }
+      // tiles' rows gr and gr + 8 are elements 2 j and 2 j + 1 of the lane's run of D / 8
 #pragma unroll
-        for (int j = 0; j < NT; j += 4)
-          *reinterpret_cast<float4*>(&sh_o[warp][r][(2 * c + e) * (D / 8) + j]) =
-              make_float4(o[t][j][2 * y + e], o[t][j + 1][2 * y + e], o[t][j + 2][2 * y + e], o[t][j + 3][2 * y + e]);
+      for (int j = 0; j < KS; j += 2)
+        *reinterpret_cast<float4*>(&sh_o[warp][r][gr * (D / 8) + 2 * j]) = make_float4(o[t][j][y], o[t][j][2 + y], o[t][j + 1][y], o[t][j + 1][2 + y]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (D / 8); i += WARPS * 32) {
+    for (int i = threadIdx.x; i < 8 * (D / 8); i += WARPS * 32) {
       const int r = i / (D / 8), j = (i % (D / 8)) * 8;
-      if (t * 16 + r >= rows) continue;
+      if (t * 8 + r >= w.rows) continue;
       float top = sh_m[0][r];
 #pragma unroll
-      for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sh_m[w][r]);
+      for (int x = 1; x < WARPS; ++x) top = fmaxf(top, sh_m[x][r]);
       float sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = sh_m[w][r] == -INFINITY ? 0.f : ex2(sh_m[w][r] - top);
-        sum = fmaf(sh_l[w][r], f, sum);
+      for (int x = 0; x < WARPS; ++x) {
+        const float f = sh_m[x][r] == -INFINITY ? 0.f : ex2(sh_m[x][r] - top);
+        sum = fmaf(sh_l[x][r], f, sum);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(sh_o[w][r][j + e], f, v[e]);
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(sh_o[x][r][j + e], f, v[e]);
       }
-      const int row = tile * R + t * 16 + r, tok = q.first + row / g.group, qh = head * g.group + row % g.group;
-      if (whole) {
+      const int row = w.tile * R + t * 8 + r, tok = w.q.first + row / g.group, qh = w.head * g.group + row % g.group;
+      if (sh_nan) nan_fixup(g, w, row, j, v);
+      if (w.ranges == 1) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;    // a row that sees nothing: 0, and -inf below
         uint4 pk;
         pk.x = half2_of(v[0] * inv, v[1] * inv); pk.y = half2_of(v[2] * inv, v[3] * inv);
@@ -384,94 +378,125 @@ __global__ void __launch_bounds__(WARPS * 32) kv_decode_kernel(const AttArgs g) 
         *reinterpret_cast<uint4*>(g.out + tok * g.ot + qh * g.oh + j) = pk;
         if (g.lse && j == 0) g.lse[(long long)tok * g.q_heads + qh] = sum == 0.f ? -INFINITY : (top - LIFT + log2f(sum)) * 0.6931471805599453f;
       } else {
-        float* dst = g.part_o + ((long long)blockIdx.x * R + t * 16 + r) * D + j;
+        float* dst = g.part_o + ((long long)blockIdx.x * R + t * 8 + r) * D + j;
         *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        if (j == 0) g.part_ml[(long long)blockIdx.x * R + t * 16 + r] = make_float2(top, sum);
+        if (j == 0) g.part_ml[(long long)blockIdx.x * R + t * 8 + r] = make_float2(top, sum);
       }
     }
   }
 }
 
-// One warp per row: the ranges' partial results in their order.
-template <int D, int MT>
-__global__ void __launch_bounds__(256) kv_combine_kernel(const AttArgs g) {
-  constexpr int R = 16 * MT, N = D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int r = (int)(unit % R);
-  unsigned rest = (unsigned)(unit / R);
-  const int tile = (int)(rest % (unsigned)g.tiles); rest /= (unsigned)g.tiles;
-  const int head = (int)(rest % (unsigned)g.cache.heads), s = (int)(rest / (unsigned)g.cache.heads);
-  if (s >= g.batch.seqs) return;
-  const Seq q = load_seq(g.batch, g.cache, s);
-  if (!q.ok) return;
-  const int rows = min(q.m * g.group - tile * R, R);
-  if (r >= rows) return;
-  const int lo_tile = view_of(g, q, tile * R).lo, hi_tile = view_of(g, q, tile * R + rows - 1).hi;
-  const int ranges = hi_tile > lo_tile ? (hi_tile - 1) / g.range - lo_tile / g.range + 1 : 1;
-  if (ranges == 1) return;                                 // written already
-  const long long cta0 = (unit / R) * g.splits;
+// One CTA per row: the ranges' partial results, every (128 / (D / 4))-th to one of its parts, these in order.
+template <int D, int R>
+__global__ void __launch_bounds__(128) kv_combine_kernel(const AttArgs g) {
+  constexpr int COLS = D / 4, PARTS = 128 / COLS;          // 4, 5, 8 or 16 ranges at a time
+  __shared__ float sh_top[4];
+  __shared__ float4 sh_v[PARTS][COLS];
+  __shared__ float sh_sum[PARTS];
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // the partial results are complete and visible
+  const unsigned unit = blockIdx.x / R;
+  const int r = (int)(blockIdx.x % R);
+  Work w;
+  if (!work_of<R>(g, unit, 0, w) || r >= w.rows || w.ranges == 1) return;
+  const long long cta0 = (long long)unit * g.splits;
   float top = -INFINITY;
-  for (int x = 0; x < ranges; ++x) top = fmaxf(top, g.part_ml[(cta0 + x) * R + r].x);
-  float sum = 0.f, v[N];
+  for (int x = threadIdx.x; x < w.ranges; x += 128) top = fmaxf(top, g.part_ml[(cta0 + x) * R + r].x);
 #pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = 0.f;
-  for (int x = 0; x < ranges; ++x) {
-    const float2 ml = g.part_ml[(cta0 + x) * R + r];
-    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-    const float* src = g.part_o + ((cta0 + x) * R + r) * D + lane * N;
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = fmaf(src[e], f, v[e]);
+  for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  if ((threadIdx.x & 31) == 0) sh_top[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(sh_top[0], sh_top[1]), fmaxf(sh_top[2], sh_top[3]));
+  const int part = threadIdx.x / COLS, col = threadIdx.x % COLS;
+  float sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (part < PARTS) {
+#pragma unroll 4
+    for (int x = part; x < w.ranges; x += PARTS) {
+      const float2 ml = g.part_ml[(cta0 + x) * R + r];
+      const float4 o = *reinterpret_cast<const float4*>(g.part_o + ((cta0 + x) * R + r) * D + col * 4);
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+      sum = fmaf(ml.y, f, sum);
+      v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
+    }
+    sh_v[part][col] = v;
+    if (col == 0) sh_sum[part] = sum;
   }
-  const int row = tile * R + r, tok = q.first + row / g.group, qh = head * g.group + row % g.group;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  __half* dst = g.out + tok * g.ot + qh * g.oh + lane * N;
+  __syncthreads();
+  if (part) return;
 #pragma unroll
-  for (int e = 0; e < N; ++e) dst[e] = __float2half_rn(v[e] * inv);
-  if (g.lse && lane == 0) g.lse[(long long)tok * g.q_heads + qh] = sum == 0.f ? -INFINITY : (top - LIFT + log2f(sum)) * 0.6931471805599453f;
+  for (int x = 1; x < PARTS; ++x) {
+    const float4 o = sh_v[x][col];
+    sum += sh_sum[x];
+    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+  }
+  const int row = w.tile * R + r, tok = w.q.first + row / g.group, qh = w.head * g.group + row % g.group;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint2*>(g.out + tok * g.ot + qh * g.oh + col * 4) = make_uint2(half2_of(v.x * inv, v.y * inv), half2_of(v.z * inv, v.w * inv));
+  if (g.lse && col == 0) g.lse[(long long)tok * g.q_heads + qh] = sum == 0.f ? -INFINITY : (top - LIFT + log2f(sum)) * 0.6931471805599453f;
 }
 
-struct Plan { int mt, tiles, splits, range; long long ctas; };
+struct Plan {
+  int nq, tiles, splits, range;
+  long long units, ctas;           // row tiles; row tiles * splits
+  size_t part_floats() const { return splits == 1 ? 0 : (size_t)ctas * 8 * nq; }     // times d + 2
+};
 
 // How the rows and slots of a call are cut.  Everything follows from what the host knows: the lengths stay on the device,
 // the page table's width bounds them.
 Plan plan_of(const Cache& c, const Batch& b, int64_t q_heads, int64_t window, int causal, int sms) {
   Plan p;
   const int64_t group = q_heads / c.heads, rows = (int64_t)b.max_new * group;
-  p.mt = rows > 16 ? 2 : 1;
-  const int64_t tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
+  p.nq = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
+  const int64_t tiles = (rows + 8 * p.nq - 1) / (8 * p.nq);
   int64_t bound = (int64_t)b.max_pages << c.page_log2;
   if (window && causal && bound > window + b.max_new) bound = window + b.max_new + 1;
-  const int64_t base = (int64_t)b.seqs * c.heads * tiles;
-  // Ranges long enough that a CTA's start and its partial result cost little next to its reading (256 slots of d = 128
-  // are 64 KB), and no more of them than eight rounds of CTAs: what the bound overstates is CTAs that return at once.
-  int64_t range = 256;
-  const int64_t most = (int64_t)sms * 3 * 8;
-  while (range < bound && base * ((bound + range - 1) / range) > most) range *= 2;
+  p.units = (int64_t)b.seqs * c.heads * tiles;
+  // One sequence is cut into as many ranges as make one round of CTAs.  Several are cut finer, four rounds if all were as
+  // long as the bound: shorter ones leave CTAs that return at once, and the ranges' equal length evens out the others.
+  // No range is shorter than 256 slots (64 KB at d = 128), below which a CTA's start and its partial result cost as
+  // much as its reading.
+  const int64_t round = (int64_t)sms * (p.nq == 1 ? 4 : p.nq == 2 ? 3 : 2), want = round * (b.seqs == 1 ? 1 : 4);
+  int64_t parts = want / (p.units > 0 ? p.units : 1);
+  if (parts < 1) parts = 1;
+  int64_t range = (bound + parts - 1) / parts;
+  range = (range + 63) / 64 * 64;
+  if (range < 256) range = 256;
   p.range = (int)(range > (1 << 30) ? (1 << 30) : range);
   p.splits = (int)((bound + p.range - 1) / p.range) + (window ? 1 : 0);
   if (p.splits < 1) p.splits = 1;
   p.tiles = (int)tiles;
-  p.ctas = base * p.splits;
+  p.ctas = p.units * p.splits;
   return p;
 }
 
-template <int D, int MT>
-int launch_decode(const AttArgs& g, long long ctas, cudaStream_t stream) {
-  kv_decode_kernel<D, MT><<<(unsigned)ctas, WARPS * 32, 0, stream>>>(g);
-  count_launch(false);
+template <int D, int NQ>
+int launch_decode(const AttArgs& g, const Plan& p, cudaStream_t stream) {
+  kv_decode_kernel<D, NQ><<<(unsigned)p.ctas, WARPS * 32, 0, stream>>>(g);
+  count_launch(true);
   int rc = note_cuda_error(cudaGetLastError(), "cache attention launch");
   if (rc || g.splits == 1) return rc;
-  const long long rows = ctas / g.splits * 16 * MT;
-  kv_combine_kernel<D, MT><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(g);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.units * 8 * NQ));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute early;                               // its launch overlaps the end of the kernel before it
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  rc = note_cuda_error(cudaLaunchKernelEx(&cfg, kv_combine_kernel<D, 8 * NQ>, g), "cache attention join launch");
   count_launch(false);
-  return note_cuda_error(cudaGetLastError(), "cache attention join launch");
+  return rc;
 }
 template <int D>
 int launch_decode_d(const AttArgs& g, const Plan& p, cudaStream_t stream) {
-  return p.mt == 1 ? launch_decode<D, 1>(g, p.ctas, stream) : launch_decode<D, 2>(g, p.ctas, stream);
+  switch (p.nq) {
+    case 1: return launch_decode<D, 1>(g, p, stream);
+    case 2: return launch_decode<D, 2>(g, p, stream);
+    case 3: return launch_decode<D, 3>(g, p, stream);
+    default: return launch_decode<D, 4>(g, p, stream);
+  }
 }
 
 }  // namespace
@@ -483,7 +508,7 @@ size_t kv_cache_attention_workspace_bytes(const b200_kv_cache* cache, const b200
   if (c.pages == 0) b.max_pages = 0;
   const DeviceState* ds = device_state();
   const Plan p = plan_of(c, b, q_heads, window, causal, ds ? ds->sm_count : 148);
-  return p.splits == 1 ? 0 : (size_t)p.ctas * 16 * p.mt * (c.d + 2) * sizeof(float);
+  return p.part_floats() * (c.d + 2) * sizeof(float);
 }
 
 int kv_cache_attention(int dtype, const b200_kv_cache* cache, const b200_kv_batch* batch, int64_t q_heads, const void* q,
@@ -505,8 +530,8 @@ int kv_cache_attention(int dtype, const b200_kv_cache* cache, const b200_kv_batc
   if (((uintptr_t)q | (uintptr_t)out) & 15) return B200_ERR_UNSUPPORTED;
   if (qs[0] % 8 || qs[1] % 8 || os[0] % 8 || os[1] % 8) return B200_ERR_UNSUPPORTED;
   const Plan p = plan_of(g.cache, g.batch, q_heads, window, causal, ds->sm_count);
-  if (p.ctas > 0x7fffffff || p.ctas / p.splits * 16 * p.mt > 0x7fffffff) return B200_ERR_LIMIT;
-  const size_t need = p.splits == 1 ? 0 : (size_t)p.ctas * 16 * p.mt * (g.cache.d + 2) * sizeof(float);
+  if (p.ctas > 0x7fffffff || p.units * 8 * p.nq > 0x7fffffff) return B200_ERR_LIMIT;
+  const size_t need = p.part_floats() * (g.cache.d + 2) * sizeof(float);
   if (need && (!workspace || ((uintptr_t)workspace & 15))) return B200_ERR_NULL;
   if (workspace_bytes < need) return B200_ERR_WORKSPACE;
   g.q_heads = (int)q_heads; g.group = (int)(q_heads / g.cache.heads);
@@ -517,7 +542,7 @@ int kv_cache_attention(int dtype, const b200_kv_cache* cache, const b200_kv_batc
   g.out = (__half*)out; g.ot = os[0]; g.oh = os[1];
   g.lse = lse;
   g.part_o = (float*)workspace;
-  g.part_ml = (float2*)((float*)workspace + (size_t)p.ctas * 16 * p.mt * g.cache.d);
+  g.part_ml = (float2*)((float*)workspace + p.part_floats() * g.cache.d);
   g.status = ds->status;
   switch (g.cache.d) {
     case 32: return launch_decode_d<32>(g, p, stream);

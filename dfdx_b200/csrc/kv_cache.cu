@@ -6,7 +6,7 @@
 //                     the codes, so that each input is read once and no other CTA ever touches the block.  A block
 //                     whose scale grows under earlier rows has these moved to the new scale, a power-of-two step.
 //                     Further CTAs take the queries.  A page's scale starts anew with its first row.
-//   kv_read_kernel    codes times scale, 16 codes a thread.
+//   kv_read_kernel    codes times scale, 8 codes a thread and step.
 // Which (sequence, page) a CTA has follows from cu_tokens alone: a sequence that ends at token e can touch at most
 // m / page + 2 pages, so the CTAs from cu[s] / page + 2 s on are its own and those behind its last page return.  No
 // launch plan is made on the host, which does not know the lengths.
@@ -50,97 +50,82 @@ __device__ __forceinline__ int owner_of(const int* cu, int n, int tok) {
 
 template <typename T, int LPR, bool INTER, bool VEC>
 __device__ __forceinline__ void append_queries(const AppendArgs& g, unsigned cta) {
-  constexpr int GROUPS = THREADS / LPR, U = 2;
+  constexpr int GROUPS = THREADS / LPR, U = !VEC ? 1 : sizeof(T) == 2 ? 4 : 2;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const Lane<INTER, VEC> ln(lane, g.cache.d, g.t.pairs);
   const int per_cta = GROUPS / g.per_token, first = group % g.per_token;
   const int tok = (int)cta * per_cta + group / g.per_token;
-  Turns turns;
-  turns.init(g.t, ln.j0);
   bool on = tok < g.batch.tokens;
   int slot = 0;
-  if (on && !(g.pos && g.t.pairs)) {
+  if (on) {
     const int s = g.batch.max_new == 1 && g.batch.tokens == g.batch.seqs ? tok : owner_of(g.batch.cu, g.batch.seqs, tok);
     const Seq q = load_seq(g.batch, g.cache, s);
     on = q.ok && tok >= q.first && tok < q.first + q.m;    // a token of no sequence is left alone
     slot = q.len - q.m + (tok - q.first);
-  } else if (on) {
-    const int s = owner_of(g.batch.cu, g.batch.seqs, tok);
-    on = tok >= g.batch.cu[s] && tok < g.batch.cu[s + 1];
   }
-  const bool own_pos = g.pos && on;
-  const int p0 = own_pos ? g.pos[tok] : slot;
-  const int p1 = own_pos && g.axes > 1 ? g.pos[g.batch.tokens + tok] : p0;
-  const int p2 = own_pos && g.axes > 2 ? g.pos[2 * g.batch.tokens + tok] : p0;
+  const Place at = place_of(on ? g.pos : nullptr, g.axes, g.batch.tokens, tok, slot);
   on = on && ln.live;
-  float ga[4], gb[4], c[4], s[4];
-  const T* gain = reinterpret_cast<const T*>(g.q_gain);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    ga[e] = gain && ln.has(e) ? to_f(gain[ln.at(e)]) : 1.f;
-    gb[e] = gain && ln.has(e) ? to_f(gain[ln.at(4 + e)]) : 1.f;
-  }
   const T* q = reinterpret_cast<const T*>(g.q) + tok * g.qt;
   T* qo = reinterpret_cast<T*>(g.q_out) + tok * g.qot;
   const float inv_d = 1.f / (float)g.cache.d;
-  bool turned = false;
-  for (int r0 = first; r0 - first < g.q_heads; r0 += U * g.per_token) {
-    float a[U][4], b[U][4];
+  Coef k;
+  for (int r0 = 0; r0 < g.q_heads; r0 += U * g.per_token) {
+    Raw<T, VEC> raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * g.per_token;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) a[u][e] = b[u][e] = 0.f;
-      if (on && r < g.q_heads) ln.load(q + r * g.qh, a[u], b[u]);
+      const int r = r0 + u * g.per_token + first;
+      ln.clear(raw[u]);
+      if (on && r < g.q_heads) ln.load(q + r * g.qh, raw[u]);
     }
-    if (!turned) {
-      turns.at(p0, p1, p2, c, s);
-      turned = true;
+    if (r0 == 0) {
+      k = coef(angle_at(g.t, ln.j0, at.p0, at.p1, at.p2), ln.gain(reinterpret_cast<const T*>(g.q_gain)));
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * g.per_token;
-      if (g.t.normalize) {
-        const float rs = rsqrtf(group_sum<LPR>(sum8(a[u], b[u], a[u], b[u])) * inv_d + g.t.eps);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { a[u][e] *= rs * ga[e]; b[u][e] *= rs * gb[e]; }
-      }
-      turn<false>(a[u], b[u], c, s, g.t.pairs - ln.j0);
-      if (on && r < g.q_heads) ln.store(qo + r * g.qoh, a[u], b[u]);
+      const int r = r0 + u * g.per_token + first;
+      const Row y = transformed<LPR, VEC>(ln.row(raw[u]), k, g.t, ln.j0, inv_d);
+      if (on && r < g.q_heads) ln.store(qo + r * g.qoh, y);
     }
   }
 }
 
-// Four values of a row to their codes: a word where the rows may be written in vectors.
+// A lane's eight values of a row to their codes: words where the rows may be written in vectors.
 template <bool INTER, bool VEC>
-__device__ __forceinline__ void store_codes(const Lane<INTER, VEC>& ln, uint8_t* row, const float (&a)[4], const float (&b)[4], float inv) {
-  if constexpr (VEC) {
-    if constexpr (INTER) {
-      const float u[4] = {a[0], b[0], a[1], b[1]}, v[4] = {a[2], b[2], a[3], b[3]};
-      *reinterpret_cast<uint2*>(row + ln.off_u) = make_uint2(codes4(u, inv), codes4(v, inv));
-    } else {
-      *reinterpret_cast<uint32_t*>(row + ln.off_u) = codes4(a, inv);
-      *reinterpret_cast<uint32_t*>(row + ln.off_v) = codes4(b, inv);
-    }
+__device__ __forceinline__ void store_codes(const Lane<INTER, VEC>& ln, uint8_t* row, const Row& x, float inv) {
+  float u[4], v[4];
+  ln.values(x, u, v);
+  const uint32_t cu = codes4(u, inv), cv = codes4(v, inv);
+  if constexpr (VEC && INTER) {
+    *reinterpret_cast<uint2*>(row + ln.off_u) = make_uint2(cu, cv);
+  } else if constexpr (VEC) {
+    *reinterpret_cast<uint32_t*>(row + ln.off_u) = cu;
+    *reinterpret_cast<uint32_t*>(row + ln.off_v) = cv;
   } else {
-    const uint32_t x = codes4(a, inv), y = codes4(b, inv);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (ln.has(e)) {
-        row[ln.at(e)] = (uint8_t)(x >> (8 * e));
-        row[ln.at(4 + e)] = (uint8_t)(y >> (8 * e));
+        row[ln.at(e)] = (uint8_t)(cu >> (8 * e));
+        row[ln.at(4 + e)] = (uint8_t)(cv >> (8 * e));
       }
   }
 }
+template <bool INTER, bool VEC>
+__device__ __forceinline__ float top_of(const Lane<INTER, VEC>& ln, const Row& x) {
+  float u[4], v[4], top = 0.f;
+  ln.values(x, u, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(finite_abs(u[e]), finite_abs(v[e])));
+  return top;
+}
 
-template <typename T, int LPR, bool INTER, bool VEC>
-__global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendArgs g) {
+// ROWS: rows that a group of lanes holds, page / (THREADS / LPR) rounded up.
+template <typename T, int LPR, bool INTER, bool VEC, int ROWS>
+__global__ void __launch_bounds__(THREADS, ROWS == 8 || !VEC ? 2 : 3) kv_append_kernel(const AppendArgs g) {
   if (blockIdx.x >= g.block_ctas) {
     append_queries<T, LPR, INTER, VEC>(g, blockIdx.x - g.block_ctas);
     return;
   }
   constexpr int GROUPS = THREADS / LPR;
-  constexpr int ROWS = 128 / GROUPS;                       // rows a group can hold: a page has at most 128
   __shared__ float warp_top[THREADS / 32];
   const bool values = blockIdx.x & 1;
   const unsigned rest = blockIdx.x >> 1;
@@ -184,52 +169,30 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendArgs g) 
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const Lane<INTER, VEC> ln(lane, g.cache.d, g.t.pairs);
   const float inv_d = 1.f / (float)g.cache.d;
-  float a[ROWS][4], b[ROWS][4];
-  float top = 0.f;
   const T* base = values ? reinterpret_cast<const T*>(g.v) + head * g.vh : reinterpret_cast<const T*>(g.k) + head * g.kh;
   const long long step = values ? g.vt : g.kt;
+  Raw<T, VEC> raw[ROWS];
+  Row x[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int r = group + i * GROUPS;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) a[i][e] = b[i][e] = 0.f;
-    if (r < rows && ln.live) ln.load(base + (tok0 + r) * step, a[i], b[i]);
+    ln.clear(raw[i]);
+    if (r < rows && ln.live) ln.load(base + (tok0 + r) * step, raw[i]);
   }
-  if (!values && (g.t.normalize || g.t.pairs)) {
-    Turns turns;
-    turns.init(g.t, ln.j0);
-    float ga[4], gb[4];
-    const T* gain = reinterpret_cast<const T*>(g.k_gain);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      ga[e] = gain && ln.has(e) ? to_f(gain[ln.at(e)]) : 1.f;
-      gb[e] = gain && ln.has(e) ? to_f(gain[ln.at(4 + e)]) : 1.f;
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const int r = group + i * GROUPS;
-      if (i * GROUPS >= rows) break;                       // the same in every group: the sums below stay whole
-      if (g.t.normalize) {
-        const float rs = rsqrtf(group_sum<LPR>(sum8(a[i], b[i], a[i], b[i])) * inv_d + g.t.eps);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { a[i][e] *= rs * ga[e]; b[i][e] *= rs * gb[e]; }
-      }
-      if (g.t.pairs) {
-        float c[4], sn[4];
-        const int tok = tok0 + min(r, rows - 1);
-        const int p0 = g.pos ? g.pos[tok] : slot0 + r;
-        const int p1 = g.pos && g.axes > 1 ? g.pos[g.batch.tokens + tok] : p0;
-        const int p2 = g.pos && g.axes > 2 ? g.pos[2 * g.batch.tokens + tok] : p0;
-        turns.at(p0, p1, p2, c, sn);
-        turn<false>(a[i], b[i], c, sn, g.t.pairs - ln.j0);
-      }
-    }
-  }
+  const bool change = !values && (g.t.normalize || g.t.pairs);
+  const Row gain = ln.gain(change ? reinterpret_cast<const T*>(g.k_gain) : nullptr);
+  float top = 0.f;
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    if (group + i * GROUPS >= rows || !ln.live) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(finite_abs(a[i][e]), finite_abs(b[i][e])));
+    x[i] = ln.row(raw[i]);
+    if (i * GROUPS < rows) {                               // the same in every group: the sums inside stay whole
+      const int r = min(group + i * GROUPS, rows - 1);
+      if (change) {
+        const Place at = place_of(g.pos, g.axes, g.batch.tokens, tok0 + r, slot0 + r);
+        x[i] = transformed<LPR, VEC>(x[i], coef(angle_at(g.t, ln.j0, at.p0, at.p1, at.p2), gain), g.t, ln.j0, inv_d);
+      }
+      top = fmaxf(top, top_of(ln, x[i]));                  // rows behind the last are zeros
+    }
   }
   top = group_max<32>(top);
   if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
@@ -241,7 +204,7 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendArgs g) 
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int r = group + i * GROUPS;
-    if (r < rows && ln.live) store_codes(ln, codes + (long long)(row0 + r) * g.cache.d, a[i], b[i], inv);
+    if (r < rows && ln.live) store_codes(ln, codes + (long long)(row0 + r) * g.cache.d, x[i], inv);
   }
   if (now != old) {
     if (row0) {                                            // the block's other rows move to the new scale
@@ -251,9 +214,7 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendArgs g) 
         const int r = i / words;
         if (r >= row0 && r < row0 + rows) continue;
         uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
-        const uint32_t x = *w, lo = values2(x), hi = values2(x >> 16);
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        const float2 f = halves(values2(*w)), h = halves(values2(*w >> 16));
         const float v[4] = {f.x, f.y, h.x, h.y};
         *w = codes4(v, ratio);
       }
@@ -262,50 +223,48 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendArgs g) 
   }
 }
 
-// Block i of the output is page pages[i]: (heads, page, d) values.
+// Block i of the output is page pages[i]: (heads, page, d) values.  One CTA per block of one head and keys or values.
 template <typename T>
-__global__ void __launch_bounds__(256) kv_read_kernel(const Cache c, const int* __restrict__ pages, long long blocks, T* k_out,
-                                                      T* v_out, int* status) {
-  const int per_block = c.page * c.d / 16;                 // chunks of 16 codes
-  const long long chunks = blocks * per_block;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < 2 * chunks; i += (long long)gridDim.x * blockDim.x) {
-    const bool values = i >= chunks;
-    const long long j = values ? i - chunks : i, blk = j / per_block;
-    const int at = (int)(j - blk * per_block), head = (int)(blk % c.heads);
-    const int id = pages[blk / c.heads];
-    uint4 x = make_uint4(0, 0, 0, 0);
-    float scale = 0.f;
-    if (id >= 0 && id < c.pages) {
-      const long long from = (long long)id * c.heads + head;
-      x = *reinterpret_cast<const uint4*>((values ? c.v : c.k) + (from * per_block + at) * 16);
-      scale = (values ? c.v_scale : c.k_scale)[from];
+__global__ void __launch_bounds__(256) kv_read_kernel(const Cache c, const int* __restrict__ pages, T* __restrict__ k_out,
+                                                      T* __restrict__ v_out, int* status) {
+  const bool values = blockIdx.x & 1;
+  const unsigned blk = blockIdx.x >> 1, head = blk % (unsigned)c.heads;
+  const int id = pages[blk / (unsigned)c.heads];
+  const int chunks = c.page * c.d / 8;                     // of 8 codes
+  T* out = (values ? v_out : k_out) + (long long)blk * c.page * c.d;
+  const bool ok = id >= 0 && id < c.pages;
+  const long long from = (long long)(ok ? id : 0) * c.heads + head;
+  const uint2* codes = reinterpret_cast<const uint2*>((values ? c.v : c.k) + from * c.page * c.d);
+  const float scale = ok ? (values ? c.v_scale : c.k_scale)[from] : 0.f;
+  if (!ok && threadIdx.x == 0) flag_index(status);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < chunks; i += 256) {
+    const uint2 x = ok ? codes[i] : make_uint2(0, 0);
+    const float2 a = halves(values2(x.x)), b = halves(values2(x.x >> 16)), e = halves(values2(x.y)), f = halves(values2(x.y >> 16));
+    if constexpr (sizeof(T) == 2) {
+      reinterpret_cast<uint4*>(out)[i] = make_uint4(half2_of(a.x * scale, a.y * scale), half2_of(b.x * scale, b.y * scale),
+                                                    half2_of(e.x * scale, e.y * scale), half2_of(f.x * scale, f.y * scale));
     } else {
-      flag_index(status);
-    }
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    T* out = (values ? v_out : k_out) + j * 16;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t lo = values2(w[e]), hi = values2(w[e] >> 16);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-      const float v[4] = {f.x * scale, f.y * scale, h.x * scale, h.y * scale};
-      store4(out + 4 * e, v);
+      reinterpret_cast<float4*>(out)[2 * i] = make_float4(a.x * scale, a.y * scale, b.x * scale, b.y * scale);
+      reinterpret_cast<float4*>(out)[2 * i + 1] = make_float4(e.x * scale, e.y * scale, f.x * scale, f.y * scale);
     }
   }
 }
 
-template <typename T, int LPR>
-int launch_append(const AppendArgs& g, bool inter, bool vec, unsigned grid, cudaStream_t stream) {
-  if (inter) {
-    if (vec) kv_append_kernel<T, LPR, true, true><<<grid, THREADS, 0, stream>>>(g);
-    else kv_append_kernel<T, LPR, true, false><<<grid, THREADS, 0, stream>>>(g);
-  } else {
-    if (vec) kv_append_kernel<T, LPR, false, true><<<grid, THREADS, 0, stream>>>(g);
-    else kv_append_kernel<T, LPR, false, false><<<grid, THREADS, 0, stream>>>(g);
-  }
+template <typename T, int LPR, bool INTER, bool VEC, int ROWS>
+int launch_append_rows(const AppendArgs& g, unsigned grid, cudaStream_t stream) {
+  kv_append_kernel<T, LPR, INTER, VEC, ROWS><<<grid, THREADS, 0, stream>>>(g);
   count_launch(false);
   return note_cuda_error(cudaGetLastError(), "cache append launch");
+}
+template <typename T, int LPR, bool INTER>
+int launch_append_vec(const AppendArgs& g, bool vec, unsigned grid, cudaStream_t stream) {
+  constexpr int MOST = 128 * LPR / THREADS;
+  const int rows = g.batch.max_new == 1 ? 1 : g.cache.page * LPR / THREADS;
+  if (!vec) return launch_append_rows<T, LPR, INTER, false, MOST>(g, grid, stream);
+  if (rows <= 1) return launch_append_rows<T, LPR, INTER, true, 1>(g, grid, stream);
+  if (rows <= MOST / 2) return launch_append_rows<T, LPR, INTER, true, MOST / 2>(g, grid, stream);
+  return launch_append_rows<T, LPR, INTER, true, MOST>(g, grid, stream);
 }
 
 bool vec_ok(int64_t es, const void* p, int64_t t, int64_t h) { return ((uintptr_t)p % (4 * es)) == 0 && t % 4 == 0 && h % 4 == 0; }
@@ -338,7 +297,7 @@ int kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* 
   const int64_t units = g.batch.max_new == 1 ? g.batch.seqs : (int64_t)(g.batch.tokens >> g.cache.page_log2) + 2 * (int64_t)g.batch.seqs;
   const int64_t block_ctas = units * g.cache.heads * 2;
   const bool inter = op->interleaved != 0;
-  bool vec = (inter || g.t.pairs % 4 == 0) && vec_ok(es, k, ks[0], ks[1]) && vec_ok(es, v, vs[0], vs[1]);
+  bool vec = g.t.pairs % 4 == 0 && vec_ok(es, k, ks[0], ks[1]) && vec_ok(es, v, vs[0], vs[1]);
   if (g.q_heads) vec = vec && vec_ok(es, q, qs[0], qs[1]) && vec_ok(es, q_out, qos[0], qos[1]);
   const int lpr = g.cache.d <= 64 ? 8 : 16, groups = THREADS / lpr;
   // groups that share a token's queries, as in the dense norm and rotation
@@ -349,9 +308,12 @@ int kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* 
   if (units > 0x7fffffff || block_ctas + q_ctas > 0x7fffffff) return B200_ERR_LIMIT;
   g.block_ctas = (unsigned)block_ctas;
   const unsigned grid = (unsigned)(block_ctas + q_ctas);
-  if (dtype == B200_F32)
-    return lpr == 8 ? launch_append<float, 8>(g, inter, vec, grid, stream) : launch_append<float, 16>(g, inter, vec, grid, stream);
-  return lpr == 8 ? launch_append<__half, 8>(g, inter, vec, grid, stream) : launch_append<__half, 16>(g, inter, vec, grid, stream);
+  if (dtype == B200_F32) {
+    if (lpr == 8) return inter ? launch_append_vec<float, 8, true>(g, vec, grid, stream) : launch_append_vec<float, 8, false>(g, vec, grid, stream);
+    return inter ? launch_append_vec<float, 16, true>(g, vec, grid, stream) : launch_append_vec<float, 16, false>(g, vec, grid, stream);
+  }
+  if (lpr == 8) return inter ? launch_append_vec<__half, 8, true>(g, vec, grid, stream) : launch_append_vec<__half, 8, false>(g, vec, grid, stream);
+  return inter ? launch_append_vec<__half, 16, true>(g, vec, grid, stream) : launch_append_vec<__half, 16, false>(g, vec, grid, stream);
 }
 
 int kv_cache_read(int dtype, const b200_kv_cache* cache, int64_t n, const int32_t* pages, void* k_out, void* v_out, cudaStream_t stream) {
@@ -361,11 +323,10 @@ int kv_cache_read(int dtype, const b200_kv_cache* cache, int64_t n, const int32_
   if (n == 0) return B200_OK;
   const DeviceState* ds = device_state();
   if (!ds) return note_cuda_error(cudaErrorInitializationError, "b200_init not called on this device");
-  const int64_t blocks = n * c.heads, work = 2 * blocks * (c.page * c.d / 16);
-  int64_t grid = (work + 255) / 256;
-  if (grid > (int64_t)ds->sm_count * 32) grid = (int64_t)ds->sm_count * 32;
-  if (dtype == B200_F32) kv_read_kernel<float><<<(unsigned)grid, 256, 0, stream>>>(c, pages, blocks, (float*)k_out, (float*)v_out, ds->status);
-  else kv_read_kernel<__half><<<(unsigned)grid, 256, 0, stream>>>(c, pages, blocks, (__half*)k_out, (__half*)v_out, ds->status);
+  const int64_t ctas = 2 * n * c.heads;
+  if (ctas > 0x7fffffff) return B200_ERR_LIMIT;
+  if (dtype == B200_F32) kv_read_kernel<float><<<(unsigned)ctas, 256, 0, stream>>>(c, pages, (float*)k_out, (float*)v_out, ds->status);
+  else kv_read_kernel<__half><<<(unsigned)ctas, 256, 0, stream>>>(c, pages, (__half*)k_out, (__half*)v_out, ds->status);
   count_launch(false);
   return note_cuda_error(cudaGetLastError(), "cache read launch");
 }

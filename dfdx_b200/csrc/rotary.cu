@@ -35,159 +35,116 @@ struct QkArgs {
 
 constexpr int THREADS = 256;
 
-// The gains in f32, in register order: [q or k][lane][a0..a3, b0..b3].
 template <typename T, int LPR, bool INTER, bool VEC>
-__device__ __forceinline__ void stage_gains(const QkArgs& g, float* sh) {
-  for (int i = threadIdx.x; i < 2 * LPR; i += THREADS) {
-    const Lane<INTER, VEC> ln(i % LPR, g.d, g.t.pairs);
-    const T* gain = reinterpret_cast<const T*>(i < LPR ? g.q_gain : g.k_gain);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sh[i * 8 + e] = gain && ln.has(e & 3) ? to_f(gain[ln.at(e)]) : 1.f;
-  }
-}
-__device__ __forceinline__ void gains_of(const float* sh, int slot, float (&a)[4], float (&b)[4]) {
-  const float4 x = *reinterpret_cast<const float4*>(sh + slot * 8), y = *reinterpret_cast<const float4*>(sh + slot * 8 + 4);
-  a[0] = x.x; a[1] = x.y; a[2] = x.z; a[3] = x.w;
-  b[0] = y.x; b[1] = y.y; b[2] = y.z; b[3] = y.w;
-}
-
-template <typename T, int LPR, bool INTER, bool VEC>
-__global__ void __launch_bounds__(THREADS) qk_forward_kernel(const QkArgs g) {
-  constexpr int GROUPS = THREADS / LPR, U = 4;
-  __shared__ __align__(16) float gains[2 * LPR * 8];
-  stage_gains<T, LPR, INTER, VEC>(g, gains);
-  __syncthreads();
+__global__ void __launch_bounds__(THREADS, 3) qk_forward_kernel(const QkArgs g) {
+  constexpr int GROUPS = THREADS / LPR, U = !VEC ? 1 : sizeof(T) == 2 ? 4 : 2;   // rows on their way per group
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const Lane<INTER, VEC> ln(lane, g.d, g.t.pairs);
-  Turns turns;
-  turns.init(g.t, ln.j0);
-  const int turning = g.t.pairs - ln.j0;                   // slots [0, turning) rotate
-  const int per_cta = GROUPS / g.per_token, first = group % g.per_token;
+  const int per_cta = GROUPS / g.per_token, part = group % g.per_token;
   const float inv_d = 1.f / (float)g.d;
-  for (long long t0 = (long long)blockIdx.x * per_cta; t0 < g.tokens; t0 += (long long)gridDim.x * per_cta) {
-    const long long tok = t0 + group / g.per_token;
-    const bool on = tok < g.tokens && ln.live;
-    const long long tc = tok < g.tokens ? tok : 0;
-    const int ib = (int)tc / g.seq, is = (int)tc % g.seq;
-    const int p0 = g.pos ? g.pos[tc] : is;
-    const int p1 = g.pos && g.axes > 1 ? g.pos[g.tokens + tc] : p0;
-    const int p2 = g.pos && g.axes > 2 ? g.pos[2 * g.tokens + tc] : p0;
-    const T* q = reinterpret_cast<const T*>(g.q) + ib * g.qb + is * g.qt;
-    const T* k = reinterpret_cast<const T*>(g.k) + ib * g.kb + is * g.kt;
-    T* qo = reinterpret_cast<T*>(g.q_out) + ib * g.qob + is * g.qot;
-    T* ko = reinterpret_cast<T*>(g.k_out) + ib * g.kob + is * g.kot;
-    float c[4], s[4];
-    bool turned = false;
-    for (int r0 = first; r0 - first < g.rows; r0 += U * g.per_token) {      // the same trip count in every group
-      float a[U][4], b[U][4];
+  const long long tok = (long long)blockIdx.x * per_cta + group / g.per_token;
+  const bool on = tok < g.tokens && ln.live;
+  const int tc = tok < g.tokens ? (int)tok : 0;
+  const int ib = tc / g.seq, is = tc % g.seq;
+  const Place at = place_of(g.pos, g.axes, g.tokens, tc, is);
+  Angle angle;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {                            // queries, then keys; the next group begins where the last ended
+    const T* src = w == 0 ? reinterpret_cast<const T*>(g.q) + ib * g.qb + is * g.qt : reinterpret_cast<const T*>(g.k) + ib * g.kb + is * g.kt;
+    T* dst = w == 0 ? reinterpret_cast<T*>(g.q_out) + ib * g.qob + is * g.qot : reinterpret_cast<T*>(g.k_out) + ib * g.kob + is * g.kot;
+    const long long sh = w == 0 ? g.qh : g.kh, dh = w == 0 ? g.qoh : g.koh;
+    const int heads = w == 0 ? g.q_heads : g.rows - g.q_heads;
+    const int first = w == 0 ? part : (part - g.q_heads) & (g.per_token - 1);
+    Coef k;
+    for (int r0 = 0; r0 < heads; r0 += U * g.per_token) {  // the same trip count in every group
+      Raw<T, VEC> raw[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * g.per_token;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[u][e] = b[u][e] = 0.f;
-        if (on && r < g.rows) ln.load(r < g.q_heads ? q + r * g.qh : k + (r - g.q_heads) * g.kh, a[u], b[u]);
+        const int r = r0 + u * g.per_token + first;
+        ln.clear(raw[u]);
+        if (on && r < heads) ln.load(src + r * sh, raw[u]);
       }
-      if (!turned) {                                       // under the first loads
-        turns.at(p0, p1, p2, c, s);
-        turned = true;
+      if (r0 == 0) {                                       // under the first loads
+        if (w == 0 || g.q_heads == 0) angle = angle_at(g.t, ln.j0, at.p0, at.p1, at.p2);
+        k = coef(angle, ln.gain(reinterpret_cast<const T*>(w == 0 ? g.q_gain : g.k_gain)));
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * g.per_token;
-        if (g.t.normalize) {
-          const float rs = rsqrtf(group_sum<LPR>(sum8(a[u], b[u], a[u], b[u])) * inv_d + g.t.eps);
-          float ga[4], gb[4];
-          gains_of(gains, lane + (r < g.q_heads ? 0 : LPR), ga, gb);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { a[u][e] *= rs * ga[e]; b[u][e] *= rs * gb[e]; }
-        }
-        turn<false>(a[u], b[u], c, s, turning);
-        if (on && r < g.rows) ln.store(r < g.q_heads ? qo + r * g.qoh : ko + (r - g.q_heads) * g.koh, a[u], b[u]);
+        const int r = r0 + u * g.per_token + first;
+        const Row y = transformed<LPR, VEC>(ln.row(raw[u]), k, g.t, ln.j0, inv_d);
+        if (on && r < heads) ln.store(dst + r * dh, y);
       }
     }
   }
 }
 
 template <typename T, int LPR, bool INTER, bool VEC>
-__global__ void __launch_bounds__(THREADS) qk_backward_kernel(const QkArgs g) {
-  constexpr int GROUPS = THREADS / LPR, U = 2;
-  __shared__ __align__(16) float gains[2 * LPR * 8];
+__global__ void __launch_bounds__(THREADS, 2) qk_backward_kernel(const QkArgs g) {
+  constexpr int GROUPS = THREADS / LPR, U = VEC ? 2 : 1;
   __shared__ float sums[THREADS * 8];
-  stage_gains<T, LPR, INTER, VEC>(g, gains);
-  __syncthreads();
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const Lane<INTER, VEC> ln(lane, g.d, g.t.pairs);
-  Turns turns;
-  turns.init(g.t, ln.j0);
-  const int turning = g.t.pairs - ln.j0;                   // slots [0, turning) rotate
-  const int per_cta = GROUPS / g.per_token, first = group % g.per_token;
+  const int per_cta = GROUPS / g.per_token, part = group % g.per_token;
   const float inv_d = 1.f / (float)g.d;
-  float acc[2][8];                                         // the gains' gradients: queries, keys
-#pragma unroll
-  for (int e = 0; e < 8; ++e) acc[0][e] = acc[1][e] = 0.f;
+  const Row zero = {{0, 0}, {0, 0}};
+  Row acc[2] = {zero, zero};                               // the gains' gradients: queries, keys
   for (long long t0 = (long long)blockIdx.x * per_cta; t0 < g.tokens; t0 += (long long)gridDim.x * per_cta) {
     const long long tok = t0 + group / g.per_token;
     const bool on = tok < g.tokens && ln.live;
-    const long long tc = tok < g.tokens ? tok : 0;
-    const int ib = (int)tc / g.seq, is = (int)tc % g.seq;
-    const int p0 = g.pos ? g.pos[tc] : is;
-    const int p1 = g.pos && g.axes > 1 ? g.pos[g.tokens + tc] : p0;
-    const int p2 = g.pos && g.axes > 2 ? g.pos[2 * g.tokens + tc] : p0;
-    const T* q = reinterpret_cast<const T*>(g.q) + ib * g.qb + is * g.qt;
-    const T* k = reinterpret_cast<const T*>(g.k) + ib * g.kb + is * g.kt;
-    const T* gq = reinterpret_cast<const T*>(g.gq) + ib * g.gqb + is * g.gqt;
-    const T* gk = reinterpret_cast<const T*>(g.gk) + ib * g.gkb + is * g.gkt;
-    T* qo = reinterpret_cast<T*>(g.q_out) + ib * g.qob + is * g.qot;
-    T* ko = reinterpret_cast<T*>(g.k_out) + ib * g.kob + is * g.kot;
-    float c[4], s[4];
-    bool turned = false;
-    for (int r0 = first; r0 - first < g.rows; r0 += U * g.per_token) {
-      float a[U][4], b[U][4], ha[U][4], hb[U][4];
+    const int tc = tok < g.tokens ? (int)tok : 0;
+    const int ib = tc / g.seq, is = tc % g.seq;
+    const Place at = place_of(g.pos, g.axes, g.tokens, tc, is);
+    Angle angle;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * g.per_token;
-        const bool isq = r < g.q_heads;
+    for (int w = 0; w < 2; ++w) {
+      const T* src = w == 0 ? reinterpret_cast<const T*>(g.q) + ib * g.qb + is * g.qt : reinterpret_cast<const T*>(g.k) + ib * g.kb + is * g.kt;
+      const T* up = w == 0 ? reinterpret_cast<const T*>(g.gq) + ib * g.gqb + is * g.gqt : reinterpret_cast<const T*>(g.gk) + ib * g.gkb + is * g.gkt;
+      T* dst = w == 0 ? reinterpret_cast<T*>(g.q_out) + ib * g.qob + is * g.qot : reinterpret_cast<T*>(g.k_out) + ib * g.kob + is * g.kot;
+      const long long sh = w == 0 ? g.qh : g.kh, uh = w == 0 ? g.gqh : g.gkh, dh = w == 0 ? g.qoh : g.koh;
+      const int heads = w == 0 ? g.q_heads : g.rows - g.q_heads;
+      const int first = w == 0 ? part : (part - g.q_heads) & (g.per_token - 1);
+      Row gain;
+      for (int r0 = 0; r0 < heads; r0 += U * g.per_token) {
+        Raw<T, VEC> rx[U], rg[U];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[u][e] = b[u][e] = ha[u][e] = hb[u][e] = 0.f;
-        if (on && r < g.rows) {
-          if (g.t.normalize) ln.load(isq ? q + r * g.qh : k + (r - g.q_heads) * g.kh, a[u], b[u]);
-          ln.load(isq ? gq + r * g.gqh : gk + (r - g.q_heads) * g.gkh, ha[u], hb[u]);
-        }
-      }
-      if (!turned) {
-        turns.at(p0, p1, p2, c, s);
-        turned = true;
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * g.per_token;
-        const bool isq = r < g.q_heads;
-        turn<true>(ha[u], hb[u], c, s, turning);
-        if (g.t.normalize) {
-          const float rs = rsqrtf(group_sum<LPR>(sum8(a[u], b[u], a[u], b[u])) * inv_d + g.t.eps);
-          float ga[4], gb[4];
-          gains_of(gains, lane + (isq ? 0 : LPR), ga, gb);
-          const float wq = isq ? 1.f : 0.f, wk = 1.f - wq;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            a[u][e] *= rs;
-            b[u][e] *= rs;
-            const float ta = ha[u][e] * a[u][e], tb = hb[u][e] * b[u][e];
-            acc[0][e] = fmaf(ta, wq, acc[0][e]);
-            acc[0][4 + e] = fmaf(tb, wq, acc[0][4 + e]);
-            acc[1][e] = fmaf(ta, wk, acc[1][e]);
-            acc[1][4 + e] = fmaf(tb, wk, acc[1][4 + e]);
-            ha[u][e] *= ga[e];
-            hb[u][e] *= gb[e];
-          }
-          const float m = group_sum<LPR>(sum8(ha[u], hb[u], a[u], b[u])) * inv_d;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            ha[u][e] = rs * fmaf(-a[u][e], m, ha[u][e]);
-            hb[u][e] = rs * fmaf(-b[u][e], m, hb[u][e]);
+        for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * g.per_token + first;
+          ln.clear(rx[u]);
+          ln.clear(rg[u]);
+          if (on && r < heads) {
+            if (g.t.normalize) ln.load(src + r * sh, rx[u]);
+            ln.load(up + r * uh, rg[u]);
           }
         }
-        if (on && r < g.rows) ln.store(isq ? qo + r * g.qoh : ko + (r - g.q_heads) * g.koh, ha[u], hb[u]);
+        if (r0 == 0) {
+          if (w == 0 || g.q_heads == 0) {
+            angle = angle_at(g.t, ln.j0, at.p0, at.p1, at.p2);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) angle.s[e] = neg2(angle.s[e]);       // the gradient turns back
+          }
+          if (g.t.normalize) gain = ln.gain(reinterpret_cast<const T*>(w == 0 ? g.q_gain : g.k_gain));
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * g.per_token + first;
+          Row h = turned<VEC>(ln.row(rg[u]), angle.c, angle.s, ln.j0, g.t.pairs);
+          if (g.t.normalize) {
+            // both sums before the reciprocal root is known:  sum x^2  and  sum h gain x
+            const Row x = ln.row(rx[u]), hx = times(h, x);
+            float sq, hg;
+            group_sum_pair<LPR>(dot(x, x), dot(hx, gain), sq, hg);
+            const float rs = rsqrtf(sq * inv_d + g.t.eps);
+            const f2 rs2 = both(rs), back = both(-(hg * inv_d) * rs * rs * rs);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              acc[w].a[e] = fma2(hx.a[e], rs2, acc[w].a[e]);
+              acc[w].b[e] = fma2(hx.b[e], rs2, acc[w].b[e]);
+              h.a[e] = fma2(h.a[e], mul2(gain.a[e], rs2), mul2(x.a[e], back));
+              h.b[e] = fma2(h.b[e], mul2(gain.b[e], rs2), mul2(x.b[e], back));
+            }
+          }
+          if (on && r < heads) ln.store(dst + r * dh, h);
+        }
       }
     }
   }
@@ -195,18 +152,21 @@ __global__ void __launch_bounds__(THREADS) qk_backward_kernel(const QkArgs g) {
   float* out = g.partial + (long long)blockIdx.x * 2 * g.d;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
+    float x[8];
+    unpack(acc[w].a[0], x[0], x[1]); unpack(acc[w].a[1], x[2], x[3]);
+    unpack(acc[w].b[0], x[4], x[5]); unpack(acc[w].b[1], x[6], x[7]);
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[(group * 8 + e) * LPR + lane] = acc[w][e];
+    for (int e = 0; e < 8; ++e) sums[(group * 8 + e) * LPR + lane] = x[e];
     __syncthreads();
     for (int i = threadIdx.x; i < 8 * LPR; i += THREADS) {
-      float x = 0.f;
+      float sum = 0.f;
 #pragma unroll
-      for (int k2 = 0; k2 < GROUPS; ++k2) x += sums[k2 * 8 * LPR + i];
+      for (int j = 0; j < GROUPS; ++j) sum += sums[j * 8 * LPR + i];
       const int e = i / LPR;
+      // INTER: a Row's values are a0..a3, b0..b3 whatever the runs' order
       const Lane<INTER, VEC> who(i % LPR, g.d, g.t.pairs);
-      if (!who.has(e & 3)) continue;
-      out[w * g.d + who.at(e)] = x;
+      if (who.has(e & 3)) out[w * g.d + who.at(e)] = sum;
     }
   }
 }
@@ -285,7 +245,7 @@ int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq
   g.kob = out_strides[1][0]; g.kot = out_strides[1][1]; g.koh = out_strides[1][2];
   g.q_gain = op->q_gain; g.k_gain = op->k_gain;
   const bool inter = op->interleaved != 0;
-  bool vec = d % 8 == 0 && (inter || g.t.pairs % 4 == 0);
+  bool vec = d % 8 == 0 && g.t.pairs % 4 == 0;
   for (int i = 0; i < (backward ? 4 : 2); ++i) vec = vec && vec_ok(es, in[i], in_strides[i][0], in_strides[i][1], in_strides[i][2]);
   for (int i = 0; i < 2; ++i) vec = vec && vec_ok(es, out[i], out_strides[i][0], out_strides[i][1], out_strides[i][2]);
   // Groups that share a token: as few as still give every SM's 2048 threads a group (the sines are then computed for

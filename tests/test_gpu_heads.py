@@ -8,10 +8,11 @@ Tolerances, with u = 2^-24 (f32) and h = half a step of the output's type relati
               the formula adds values; gains' sums over n rows: (n + 64) u of the sum of magnitudes.
   codes       half an e4m3 step of the exact value (2^-4 of it, 2^-10 of the scale below 2^-6), plus the transform's.
   attention   probabilities rounded to f16 (2^-11 of each), scores wrong by d u alpha sum |q k| and exponentials by
-              2^-21: that share of sum w |v|; plus 2^-11 of the value for the output.  A probability p' below 2^-29 of
-              the largest p'* (which counts its block's value scale in) is rounded to steps: off by 2^-40 p'*.  It meets
-              a code of at most 448 and the sum l >= p'* / sv*, so n slots add at most n 2^-40 448 sv* with sv* the
-              largest scale among the visible blocks, itself at most 2 / 448 of their largest value: n 2^-39 max |v|.
+              2^-21: that share of sum w |v|; plus 2^-11 of the value for the output.  A probability p' is held as
+              2^14 at the running maximum p'* (which counts its block's value scale in); one below 2^-14 is rounded to
+              steps of 2^-24: off by 2^-25 2^-14 p'*.  It meets a code of at most 448 and the sum l >= p'* / sv*, so n
+              slots add at most n 2^-39 448 sv* with sv* the largest scale among the visible blocks, itself at most
+              2 / 448 of their largest value: n 2^-38 max |v|.
 """
 import math
 
@@ -355,7 +356,7 @@ def check_attention(dev, sv, q, out, lse, alpha, causal=True, window=0):
         want, wlse, size = ref.attention(q64, k, v, alpha, vis)
         score = abs(alpha) * d * U * (q64.abs().amax((0, 2)).max() * (k.nan_to_num(0.0).abs().sum(-1).max() if n else 0.0)) / math.sqrt(d) * 8
         big = v.nan_to_num(0.0).abs().max() if n else 0.0
-        tol = (2.0 ** -11 + 2 * score + 2.0 ** -20) * size + 2.0 ** -11 * want.abs() + n * 2.0 ** -39 * big + 2.0 ** -25
+        tol = (2.0 ** -11 + 2 * score + 2.0 ** -20) * size + 2.0 ** -11 * want.abs() + n * 2.0 ** -38 * big + 2.0 ** -25
         within(out[at:at + m], want, tol, f"sequence {s}")
         if lse is not None:
             within(lse[at:at + m], wlse, 2 * score + 2.0 ** -19 + 4 * U * wlse.abs().nan_to_num(0, 0, 0), f"lse {s}")
@@ -420,7 +421,7 @@ def test_attention_scores_far_apart_and_scales_far_apart(cuda_dev, new):
             err = 64 * U * abs(alpha) * float((q.cpu().double().abs().amax() * kk.abs().sum(-1).amax()))
             fine = want.abs() < 60000
             within(torch.where(fine, out[at:at + new].cpu().double(), 0.0), torch.where(fine, want, 0.0),
-                   (2.0 ** -11 + 2 * err) * sz + 2.0 ** -11 * want.abs() + 2.0 ** -25 + n * 2.0 ** -39 * float(vv.abs().max()), f"{alpha} {s}")
+                   (2.0 ** -11 + 2 * err) * sz + 2.0 ** -11 * want.abs() + 2.0 ** -25 + n * 2.0 ** -38 * float(vv.abs().max()), f"{alpha} {s}")
             within(lse[at:at + new], wlse, 2 * err + 2.0 ** -19 + 4 * U * wlse.abs(), f"lse {alpha} {s}")
             at += new
     assert dev.device_status() == 0
