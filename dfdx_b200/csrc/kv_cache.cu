@@ -24,18 +24,18 @@ struct AppendArgs {
   Transform t;
   Cache cache;
   Batch batch;
-  unsigned block_ctas;             // (sequence, page) candidates * heads * 2; the CTAs behind them take queries
+  int key_heads;                   // heads that a key CTA takes one after another
+  unsigned k_ctas, v_ctas;         // candidates (sequence, page) * head groups; candidates * heads; the CTAs behind take queries
   int q_heads, per_token;
   int axes;
   const int* pos;                  // axes x tokens, or nullptr: the token's slot on every axis
   const void *q, *k, *v;
   void* q_out;
-  long long qt, qh, kt, kh, vt, vh, qot, qoh;      // element strides of the token and head axes
+  long long qt, kt, vt, qot;       // element strides of the token and head axes
+  int qh, kh, vh, qoh;
   const void *q_gain, *k_gain;
   int* status;
 };
-
-constexpr int THREADS = 256;
 
 // The sequence of a new token, by bisection over cu (the last s with cu[s] <= tok).
 __device__ __forceinline__ int owner_of(const int* cu, int n, int tok) {
@@ -47,89 +47,99 @@ __device__ __forceinline__ int owner_of(const int* cu, int n, int tok) {
   }
   return lo;
 }
+// A token's slot in its sequence; -1 for a token of no sequence.
+__device__ __forceinline__ int slot_of(const AppendArgs& g, int tok) {
+  if (tok >= g.batch.tokens) return -1;
+  const int s = g.batch.max_new == 1 && g.batch.tokens == g.batch.seqs ? tok : owner_of(g.batch.cu, g.batch.seqs, tok);
+  const Seq q = load_seq(g.batch, g.cache, s);
+  return q.ok && tok >= q.first && tok < q.first + q.m && q.m <= q.len ? q.len - q.m + (tok - q.first) : -1;
+}
 
-template <typename T, int LPR, bool INTER, bool VEC>
-__device__ __forceinline__ void append_queries(const AppendArgs& g, unsigned cta) {
-  constexpr int GROUPS = THREADS / LPR, U = !VEC ? 1 : sizeof(T) == 2 ? 4 : 2;
-  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const Lane<INTER, VEC> ln(lane, g.cache.d, g.t.pairs);
-  const int per_cta = GROUPS / g.per_token, first = group % g.per_token;
-  const int tok = (int)cta * per_cta + group / g.per_token;
-  bool on = tok < g.batch.tokens;
-  int slot = 0;
-  if (on) {
-    const int s = g.batch.max_new == 1 && g.batch.tokens == g.batch.seqs ? tok : owner_of(g.batch.cu, g.batch.seqs, tok);
-    const Seq q = load_seq(g.batch, g.cache, s);
-    on = q.ok && tok >= q.first && tok < q.first + q.m;    // a token of no sequence is left alone
-    slot = q.len - q.m + (tok - q.first);
-  }
-  const Place at = place_of(on ? g.pos : nullptr, g.axes, g.batch.tokens, tok, slot);
-  on = on && ln.live;
-  const T* q = reinterpret_cast<const T*>(g.q) + tok * g.qt;
-  T* qo = reinterpret_cast<T*>(g.q_out) + tok * g.qot;
+template <typename T, int LPR, bool INTER, bool VEC, int NT>
+__device__ __forceinline__ void append_queries(const AppendArgs& g, unsigned cta, float2* table) {
+  constexpr int GROUPS = NT / LPR, U = !VEC ? 1 : sizeof(T) == 2 ? 4 : 2;      // rows on their way per group
+  __shared__ int slots[GROUPS];
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR, pairs = g.t.pairs;
+  const Lane<T, INTER, VEC> ln(lane, g.cache.d, pairs);
+  const int per_cta = GROUPS / g.per_token, first = group % g.per_token, mine = group / g.per_token, step = g.per_token;
+  const int t0 = (int)cta * per_cta, tok = t0 + mine, heads = g.q_heads;
+  const int tc = min(tok, g.batch.tokens - 1);
+  const T* q = reinterpret_cast<const T*>(g.q) + tc * g.qt;
+  T* qo = reinterpret_cast<T*>(g.q_out) + tc * g.qot;
   const float inv_d = 1.f / (float)g.cache.d;
-  Coef k;
-  for (int r0 = 0; r0 < g.q_heads; r0 += U * g.per_token) {
-    Raw<T, VEC> raw[U];
+  Raw<T, VEC> raw[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    ln.clear(raw[u]);
+    ln.load(q + (long long)min(u * step + first, heads - 1) * g.qh, raw[u]);
+  }
+  if (threadIdx.x < per_cta) slots[threadIdx.x] = slot_of(g, t0 + threadIdx.x);
+  const Row gain = ln.gain(g.q_gain);
+  __syncthreads();
+  for (int i = threadIdx.x; i < per_cta * pairs; i += NT) {
+    const int t = i / pairs;
+    if (slots[t] >= 0) table[i] = cos_sin(g.t, i % pairs, place_of(g.pos, g.axes, g.batch.tokens, t0 + t, slots[t]));
+  }
+  __syncthreads();
+  const bool on = slots[mine] >= 0;                        // a token of no sequence is left alone
+  const Coef k = coef(angle_from(table + mine * pairs, ln.j0, on ? pairs : 0), gain);
+  for (int r0 = 0;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * g.per_token + first;
-      ln.clear(raw[u]);
-      if (on && r < g.q_heads) ln.load(q + r * g.qh, raw[u]);
-    }
-    if (r0 == 0) {
-      k = coef(angle_at(g.t, ln.j0, at.p0, at.p1, at.p2), ln.gain(reinterpret_cast<const T*>(g.q_gain)));
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * g.per_token + first;
+      const int r = r0 + u * step + first;
       const Row y = transformed<LPR, VEC>(ln.row(raw[u]), k, g.t, ln.j0, inv_d);
-      if (on && r < g.q_heads) ln.store(qo + r * g.qoh, y);
+      if (on && r < heads) ln.store(qo + (long long)r * g.qoh, y);
     }
+    r0 += U * step;
+    if (r0 >= heads) break;
+#pragma unroll
+    for (int u = 0; u < U; ++u) ln.load(q + (long long)min(r0 + u * step + first, heads - 1) * g.qh, raw[u]);
   }
 }
 
 // A lane's eight values of a row to their codes: words where the rows may be written in vectors.
-template <bool INTER, bool VEC>
-__device__ __forceinline__ void store_codes(const Lane<INTER, VEC>& ln, uint8_t* row, const Row& x, float inv) {
-  float u[4], v[4];
+template <typename T, bool INTER, bool VEC>
+__device__ __forceinline__ void store_codes(const Lane<T, INTER, VEC>& ln, uint8_t* row, const Row& x, float inv) {
+  float u[S], v[S];
   ln.values(x, u, v);
   const uint32_t cu = codes4(u, inv), cv = codes4(v, inv);
-  if constexpr (VEC && INTER) {
-    *reinterpret_cast<uint2*>(row + ln.off_u) = make_uint2(cu, cv);
-  } else if constexpr (VEC) {
-    *reinterpret_cast<uint32_t*>(row + ln.off_u) = cu;
-    *reinterpret_cast<uint32_t*>(row + ln.off_v) = cv;
-  } else {
+  if constexpr (!VEC) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < S; ++e)
       if (ln.has(e)) {
         row[ln.at(e)] = (uint8_t)(cu >> (8 * e));
-        row[ln.at(4 + e)] = (uint8_t)(cv >> (8 * e));
+        row[ln.at(S + e)] = (uint8_t)(cv >> (8 * e));
       }
+  } else if (ln.live) {
+    *reinterpret_cast<uint32_t*>(row + ln.off_u) = cu;
+    *reinterpret_cast<uint32_t*>(row + ln.off_v) = cv;
   }
 }
-template <bool INTER, bool VEC>
-__device__ __forceinline__ float top_of(const Lane<INTER, VEC>& ln, const Row& x) {
-  float u[4], v[4], top = 0.f;
+template <typename T, bool INTER, bool VEC>
+__device__ __forceinline__ float top_of(const Lane<T, INTER, VEC>& ln, const Row& x) {
+  float u[S], v[S], top = 0.f;
   ln.values(x, u, v);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(finite_abs(u[e]), finite_abs(v[e])));
+  for (int e = 0; e < S; ++e) top = fmaxf(top, fmaxf(finite_abs(u[e]), finite_abs(v[e])));
   return top;
 }
 
-// ROWS: rows that a group of lanes holds, page / (THREADS / LPR) rounded up.
-template <typename T, int LPR, bool INTER, bool VEC, int ROWS>
-__global__ void __launch_bounds__(THREADS, ROWS == 8 || !VEC ? 2 : 3) kv_append_kernel(const AppendArgs g) {
-  if (blockIdx.x >= g.block_ctas) {
-    append_queries<T, LPR, INTER, VEC>(g, blockIdx.x - g.block_ctas);
+// NT threads; ROWS: new rows of a block that a group of lanes holds, at most page / (NT / LPR) rounded up.
+template <typename T, int LPR, bool INTER, bool VEC, int NT, int ROWS>
+__global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC ? 3 : 2) : 8) kv_append_kernel(const __grid_constant__ AppendArgs g) {
+  extern __shared__ float2 table[];                        // cos and sin: new rows of the block (tokens of the CTA) x pairs
+  if (blockIdx.x >= g.k_ctas + g.v_ctas) {
+    append_queries<T, LPR, INTER, VEC, NT>(g, blockIdx.x - g.k_ctas - g.v_ctas, table);
     return;
   }
-  constexpr int GROUPS = THREADS / LPR;
-  __shared__ float warp_top[THREADS / 32];
-  const bool values = blockIdx.x & 1;
-  const unsigned rest = blockIdx.x >> 1;
-  const int head = (int)(rest % (unsigned)g.cache.heads), unit = (int)(rest / (unsigned)g.cache.heads);
+  constexpr int GROUPS = NT / LPR;
+  constexpr bool AHEAD = VEC && ROWS * sizeof(T) <= 16;    // registers for the next head's rows beside this one's
+  __shared__ float warp_top[2][NT / 32];
+  const bool values = blockIdx.x >= g.k_ctas;
+  const int per_unit = values ? g.cache.heads : (g.cache.heads + g.key_heads - 1) / g.key_heads;
+  const unsigned at = blockIdx.x - (values ? g.k_ctas : 0);
+  const int unit = (int)(at / (unsigned)per_unit), head0 = (int)(at % (unsigned)per_unit) * (values ? 1 : g.key_heads);
+  const int head1 = min(head0 + (values ? 1 : g.key_heads), g.cache.heads);
   const int page = g.cache.page, shift = g.cache.page_log2;
   // unit -> (sequence, which of its touched pages)
   int s, nth;
@@ -160,57 +170,69 @@ __global__ void __launch_bounds__(THREADS, ROWS == 8 || !VEC ? 2 : 3) kv_append_
     if (threadIdx.x == 0) flag_index(g.status);
     return;
   }
-  const int rows = slot1 - slot0, row0 = slot0 & (page - 1), tok0 = q.first + (slot0 - start);
-  const long long block = (long long)id * g.cache.heads + head;
-  float* scale = (values ? g.cache.v_scale : g.cache.k_scale) + block;
-  uint8_t* codes = (values ? g.cache.v : g.cache.k) + block * page * g.cache.d;
-  const float old = row0 ? *scale : 0.f;
-
+  const int rows = slot1 - slot0, row0 = slot0 & (page - 1), tok0 = q.first + (slot0 - start), pairs = g.t.pairs;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const Lane<INTER, VEC> ln(lane, g.cache.d, g.t.pairs);
+  const Lane<T, INTER, VEC> ln(lane, g.cache.d, pairs);
   const float inv_d = 1.f / (float)g.cache.d;
-  const T* base = values ? reinterpret_cast<const T*>(g.v) + head * g.vh : reinterpret_cast<const T*>(g.k) + head * g.kh;
+  const T* src = values ? reinterpret_cast<const T*>(g.v) + tok0 * g.vt : reinterpret_cast<const T*>(g.k) + tok0 * g.kt;
   const long long step = values ? g.vt : g.kt;
+  const int hs = values ? g.vh : g.kh;
+  const bool change = !values && (g.t.normalize || pairs);
   Raw<T, VEC> raw[ROWS];
-  Row x[ROWS];
+  auto load = [&](int head) {
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int r = group + i * GROUPS;
-    ln.clear(raw[i]);
-    if (r < rows && ln.live) ln.load(base + (tok0 + r) * step, raw[i]);
-  }
-  const bool change = !values && (g.t.normalize || g.t.pairs);
-  const Row gain = ln.gain(change ? reinterpret_cast<const T*>(g.k_gain) : nullptr);
-  float top = 0.f;
+    for (int i = 0; i < ROWS; ++i)                         // groups without a row take the last one again
+      if (i * GROUPS < rows) ln.load(src + (long long)head * hs + min(group + i * GROUPS, rows - 1) * step, raw[i]);
+  };
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    x[i] = ln.row(raw[i]);
-    if (i * GROUPS < rows) {                               // the same in every group: the sums inside stay whole
-      const int r = min(group + i * GROUPS, rows - 1);
-      if (change) {
-        const Place at = place_of(g.pos, g.axes, g.batch.tokens, tok0 + r, slot0 + r);
-        x[i] = transformed<LPR, VEC>(x[i], coef(angle_at(g.t, ln.j0, at.p0, at.p1, at.p2), gain), g.t, ln.j0, inv_d);
-      }
-      top = fmaxf(top, top_of(ln, x[i]));                  // rows behind the last are zeros
+  for (int i = 0; i < ROWS; ++i) ln.clear(raw[i]);
+  load(head0);
+  Row gain;
+  if (change) {
+    gain = ln.gain(g.k_gain);
+    for (int i = threadIdx.x; i < rows * pairs; i += NT) {
+      const int r = i / pairs;
+      table[i] = cos_sin(g.t, i % pairs, place_of(g.pos, g.axes, g.batch.tokens, tok0 + r, slot0 + r));
     }
+    __syncthreads();
   }
-  top = group_max<32>(top);
-  if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
-  __syncthreads();
+  for (int head = head0; head < head1; ++head) {
+    const long long block = (long long)id * g.cache.heads + head;
+    float* scale = (values ? g.cache.v_scale : g.cache.k_scale) + block;
+    uint8_t* codes = (values ? g.cache.v : g.cache.k) + block * page * g.cache.d;
+    const float old = row0 ? *scale : 0.f;
+    if (!AHEAD && head > head0) load(head);
+    Row x[ROWS];
+    float top = 0.f;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, warp_top[w]);
-  const float fresh = pow2(scale_exp(top));
-  const float now = fmaxf(old, fresh), inv = 1.f / now;    // powers of two: exact
+    for (int i = 0; i < ROWS; ++i) {
+      if (i * GROUPS >= rows) break;                       // the same in every group: the sums inside stay whole
+      x[i] = ln.row(raw[i]);
+      if (change) {
+        const Angle t = angle_from(table + min(group + i * GROUPS, rows - 1) * pairs, ln.j0, pairs);
+        x[i] = transformed<LPR, VEC>(x[i], coef(t, gain), g.t, ln.j0, inv_d);
+      }
+      top = fmaxf(top, top_of(ln, x[i]));
+    }
+    if (AHEAD && head + 1 < head1) load(head + 1);
+    top = warp_max(top);
+    float* tops = warp_top[head & 1];                      // two sets: the next head's may be written before all have read
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int r = group + i * GROUPS;
-    if (r < rows && ln.live) store_codes(ln, codes + (long long)(row0 + r) * g.cache.d, x[i], inv);
-  }
-  if (now != old) {
+    for (int w = 0; w < NT / 32; ++w) top = fmaxf(top, tops[w]);
+    const float fresh = pow2(scale_exp(top));
+    const float now = fmaxf(old, fresh), inv = 1.f / now;  // powers of two: exact
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = group + i * GROUPS;
+      if (r < rows) store_codes(ln, codes + (long long)(row0 + r) * g.cache.d, x[i], inv);
+    }
+    if (now == old) continue;
     if (row0) {                                            // the block's other rows move to the new scale
       const float ratio = old * inv;
       const int words = g.cache.d / 4;
-      for (int i = threadIdx.x; i < page * words; i += THREADS) {
+      for (int i = threadIdx.x; i < page * words; i += NT) {
         const int r = i / words;
         if (r >= row0 && r < row0 + rows) continue;
         uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
@@ -219,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, ROWS == 8 || !VEC ? 2 : 3) kv_append_
         *w = codes4(v, ratio);
       }
     }
-    if (threadIdx.x == 0) *scale = now;
+    if (threadIdx.x == 0) *scale = now;                    // read by all before the barrier
   }
 }
 
@@ -251,23 +273,36 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const Cache c, const int* 
   }
 }
 
-template <typename T, int LPR, bool INTER, bool VEC, int ROWS>
-int launch_append_rows(const AppendArgs& g, unsigned grid, cudaStream_t stream) {
-  kv_append_kernel<T, LPR, INTER, VEC, ROWS><<<grid, THREADS, 0, stream>>>(g);
+// One new token a sequence: two warps have a row and a block to themselves.  Otherwise 256 threads hold a block's rows.
+constexpr int NT_ONE = 64, NT_MANY = 256;
+
+template <typename T, int LPR, bool INTER, bool VEC, int NT, int ROWS>
+int launch_rows(const AppendArgs& g, unsigned grid, cudaStream_t stream) {
+  const int rows = NT == NT_ONE ? 1 : g.cache.page, tokens = NT / LPR;
+  const size_t smem = (size_t)(rows > tokens ? rows : tokens) * g.t.pairs * sizeof(float2);
+  if (smem > 40 << 10) {                                   // 64 KB at most: pages of 128, heads of 128
+    const int rc = note_cuda_error(cudaFuncSetAttribute(kv_append_kernel<T, LPR, INTER, VEC, NT, ROWS>,
+                                                        cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute(cache append)");
+    if (rc) return rc;
+  }
+  kv_append_kernel<T, LPR, INTER, VEC, NT, ROWS><<<grid, NT, smem, stream>>>(g);
   count_launch(false);
   return note_cuda_error(cudaGetLastError(), "cache append launch");
 }
-template <typename T, int LPR, bool INTER>
-int launch_append_vec(const AppendArgs& g, bool vec, unsigned grid, cudaStream_t stream) {
-  constexpr int MOST = 128 * LPR / THREADS;
-  const int rows = g.batch.max_new == 1 ? 1 : g.cache.page * LPR / THREADS;
-  if (!vec) return launch_append_rows<T, LPR, INTER, false, MOST>(g, grid, stream);
-  if (rows <= 1) return launch_append_rows<T, LPR, INTER, true, 1>(g, grid, stream);
-  if (rows <= MOST / 2) return launch_append_rows<T, LPR, INTER, true, MOST / 2>(g, grid, stream);
-  return launch_append_rows<T, LPR, INTER, true, MOST>(g, grid, stream);
+template <typename T, int LPR, bool INTER, bool VEC>
+int launch_page(const AppendArgs& g, unsigned grid, cudaStream_t stream) {
+  constexpr int MOST = 128 * LPR / NT_MANY;                // rows of a group with the largest page
+  if (g.batch.max_new == 1) return launch_rows<T, LPR, INTER, VEC, NT_ONE, 1>(g, grid, stream);
+  if (g.cache.page * LPR / NT_MANY > MOST / 2) return launch_rows<T, LPR, INTER, VEC, NT_MANY, MOST>(g, grid, stream);
+  return launch_rows<T, LPR, INTER, VEC, NT_MANY, MOST / 2>(g, grid, stream);
 }
-
-bool vec_ok(int64_t es, const void* p, int64_t t, int64_t h) { return ((uintptr_t)p % (4 * es)) == 0 && t % 4 == 0 && h % 4 == 0; }
+template <typename T>
+int launch_type(const AppendArgs& g, int lpr, bool inter, bool vec, unsigned grid, cudaStream_t stream) {
+  if (!vec)                                                // rows that cannot be moved four elements at a time
+    return inter ? launch_page<T, 16, true, false>(g, grid, stream) : launch_page<T, 16, false, false>(g, grid, stream);
+  if (lpr == 8) return inter ? launch_page<T, 8, true, true>(g, grid, stream) : launch_page<T, 8, false, true>(g, grid, stream);
+  return inter ? launch_page<T, 16, true, true>(g, grid, stream) : launch_page<T, 16, false, true>(g, grid, stream);
+}
 
 }  // namespace
 
@@ -290,30 +325,31 @@ int kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* 
   g.q_heads = q ? (int)q_heads : 0;
   g.pos = positions;
   g.q = q; g.k = k; g.v = v; g.q_out = q_out;
-  g.qt = qs[0]; g.qh = qs[1]; g.kt = ks[0]; g.kh = ks[1]; g.vt = vs[0]; g.vh = vs[1]; g.qot = qos[0]; g.qoh = qos[1];
+  if (qs[1] > 0x7fffffff || ks[1] > 0x7fffffff || vs[1] > 0x7fffffff || qos[1] > 0x7fffffff) return B200_ERR_LIMIT;
+  g.qt = qs[0]; g.qh = (int)qs[1]; g.kt = ks[0]; g.kh = (int)ks[1];
+  g.vt = vs[0]; g.vh = (int)vs[1]; g.qot = qos[0]; g.qoh = (int)qos[1];
   g.q_gain = op->q_gain; g.k_gain = op->k_gain;
   g.status = ds->status;
+  const bool inter = op->interleaved != 0;
+  bool vec = g.t.pairs % 4 == 0 && vec_ok(es, k, 0, ks[0], ks[1]) && vec_ok(es, v, 0, vs[0], vs[1]);
+  if (g.q_heads) vec = vec && vec_ok(es, q, 0, qs[0], qs[1]) && vec_ok(es, q_out, 0, qos[0], qos[1]);
+  const int lpr = vec && g.cache.d <= 64 ? 8 : 16, groups = (g.batch.max_new == 1 ? NT_ONE : NT_MANY) / lpr;
   // a sequence's m new tokens touch at most (m - 1) / page + 2 pages, one token only one
   const int64_t units = g.batch.max_new == 1 ? g.batch.seqs : (int64_t)(g.batch.tokens >> g.cache.page_log2) + 2 * (int64_t)g.batch.seqs;
-  const int64_t block_ctas = units * g.cache.heads * 2;
-  const bool inter = op->interleaved != 0;
-  bool vec = g.t.pairs % 4 == 0 && vec_ok(es, k, ks[0], ks[1]) && vec_ok(es, v, vs[0], vs[1]);
-  if (g.q_heads) vec = vec && vec_ok(es, q, qs[0], qs[1]) && vec_ok(es, q_out, qos[0], qos[1]);
-  const int lpr = g.cache.d <= 64 ? 8 : 16, groups = THREADS / lpr;
+  // A key CTA computes its rows' sines once for several heads, as long as two CTAs an SM remain.
+  g.key_heads = 1;
+  while (g.key_heads < g.cache.heads && units * ((g.cache.heads + 2 * g.key_heads - 1) / (2 * g.key_heads)) >= 2 * ds->sm_count) g.key_heads *= 2;
+  const int64_t k_ctas = units * ((g.cache.heads + g.key_heads - 1) / g.key_heads), v_ctas = units * g.cache.heads;
   // groups that share a token's queries, as in the dense norm and rotation
   const int64_t want = (int64_t)ds->sm_count * (2048 / lpr);
   g.per_token = 1;
-  while (g.per_token < groups && g.per_token < g.q_heads && (int64_t)g.batch.tokens * g.per_token < want) g.per_token *= 2;
+  while (g.per_token < groups && g.per_token < g.q_heads && (g.q_heads > 8 * g.per_token || (int64_t)g.batch.tokens * g.per_token < want)) g.per_token *= 2;
   const int64_t per_cta = groups / g.per_token, q_ctas = g.q_heads ? (g.batch.tokens + per_cta - 1) / per_cta : 0;
-  if (units > 0x7fffffff || block_ctas + q_ctas > 0x7fffffff) return B200_ERR_LIMIT;
-  g.block_ctas = (unsigned)block_ctas;
-  const unsigned grid = (unsigned)(block_ctas + q_ctas);
-  if (dtype == B200_F32) {
-    if (lpr == 8) return inter ? launch_append_vec<float, 8, true>(g, vec, grid, stream) : launch_append_vec<float, 8, false>(g, vec, grid, stream);
-    return inter ? launch_append_vec<float, 16, true>(g, vec, grid, stream) : launch_append_vec<float, 16, false>(g, vec, grid, stream);
-  }
-  if (lpr == 8) return inter ? launch_append_vec<__half, 8, true>(g, vec, grid, stream) : launch_append_vec<__half, 8, false>(g, vec, grid, stream);
-  return inter ? launch_append_vec<__half, 16, true>(g, vec, grid, stream) : launch_append_vec<__half, 16, false>(g, vec, grid, stream);
+  if (units > 0x7fffffff || k_ctas + v_ctas + q_ctas > 0x7fffffff) return B200_ERR_LIMIT;
+  g.k_ctas = (unsigned)k_ctas;
+  g.v_ctas = (unsigned)v_ctas;
+  const unsigned grid = (unsigned)(k_ctas + v_ctas + q_ctas);
+  return dtype == B200_F32 ? launch_type<float>(g, lpr, inter, vec, grid, stream) : launch_type<__half>(g, lpr, inter, vec, grid, stream);
 }
 
 int kv_cache_read(int dtype, const b200_kv_cache* cache, int64_t n, const int32_t* pages, void* k_out, void* v_out, cudaStream_t stream) {

@@ -18,183 +18,199 @@ namespace {
 
 using namespace heads;
 
+struct Side {                      // queries or keys
+  const void *x, *up;              // input; upstream gradient (backward)
+  void* y;                         // output; gradient (backward)
+  const void* gain;
+  int heads, per_token;            // per_token: groups that share a token
+  int xh, uh, yh;                  // element strides of the head, batch and token axes
+  long long xb, xt, ub, ut, yb, yt;
+};
 struct QkArgs {
   Transform t;
-  long long tokens;                // batch * tokens
-  int seq, q_heads, rows;          // rows = q_heads + k_heads of one token
-  int d, axes, per_token;          // groups that share a token
+  Side side[2];
+  unsigned q_ctas;                 // the CTAs behind them have keys
+  int tokens, seq;                 // batch * tokens of a sequence
+  int d, axes;
   const int* pos;                  // axes x tokens, or nullptr: the index in the sequence on every axis
-  const void *q, *k, *gq, *gk;     // inputs; upstream gradients (backward)
-  void *q_out, *k_out;             // outputs; gradients (backward)
-  long long qb, qt, qh, kb, kt, kh;          // element strides of the batch, token and head axes
-  long long gqb, gqt, gqh, gkb, gkt, gkh;
-  long long qob, qot, qoh, kob, kot, koh;
-  const void *q_gain, *k_gain;
-  float* partial;                  // backward: gridDim.x rows of 2 * d sums, or nullptr
+  float* partial;                  // backward: a row of d sums per CTA, or nullptr
 };
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 128;
 
-template <typename T, int LPR, bool INTER, bool VEC>
-__global__ void __launch_bounds__(THREADS, 3) qk_forward_kernel(const QkArgs g) {
-  constexpr int GROUPS = THREADS / LPR, U = !VEC ? 1 : sizeof(T) == 2 ? 4 : 2;   // rows on their way per group
-  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const Lane<INTER, VEC> ln(lane, g.d, g.t.pairs);
-  const int per_cta = GROUPS / g.per_token, part = group % g.per_token;
-  const float inv_d = 1.f / (float)g.d;
-  const long long tok = (long long)blockIdx.x * per_cta + group / g.per_token;
-  const bool on = tok < g.tokens && ln.live;
-  const int tc = tok < g.tokens ? (int)tok : 0;
-  const int ib = tc / g.seq, is = tc % g.seq;
-  const Place at = place_of(g.pos, g.axes, g.tokens, tc, is);
-  Angle angle;
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {                            // queries, then keys; the next group begins where the last ended
-    const T* src = w == 0 ? reinterpret_cast<const T*>(g.q) + ib * g.qb + is * g.qt : reinterpret_cast<const T*>(g.k) + ib * g.kb + is * g.kt;
-    T* dst = w == 0 ? reinterpret_cast<T*>(g.q_out) + ib * g.qob + is * g.qot : reinterpret_cast<T*>(g.k_out) + ib * g.kob + is * g.kot;
-    const long long sh = w == 0 ? g.qh : g.kh, dh = w == 0 ? g.qoh : g.koh;
-    const int heads = w == 0 ? g.q_heads : g.rows - g.q_heads;
-    const int first = w == 0 ? part : (part - g.q_heads) & (g.per_token - 1);
-    Coef k;
-    for (int r0 = 0; r0 < heads; r0 += U * g.per_token) {  // the same trip count in every group
-      Raw<T, VEC> raw[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * g.per_token + first;
-        ln.clear(raw[u]);
-        if (on && r < heads) ln.load(src + r * sh, raw[u]);
-      }
-      if (r0 == 0) {                                       // under the first loads
-        if (w == 0 || g.q_heads == 0) angle = angle_at(g.t, ln.j0, at.p0, at.p1, at.p2);
-        k = coef(angle, ln.gain(reinterpret_cast<const T*>(w == 0 ? g.q_gain : g.k_gain)));
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * g.per_token + first;
-        const Row y = transformed<LPR, VEC>(ln.row(raw[u]), k, g.t, ln.j0, inv_d);
-        if (on && r < heads) ln.store(dst + r * dh, y);
-      }
-    }
+__device__ __forceinline__ Place place_at(const QkArgs& g, int tok) { return place_of(g.pos, g.axes, g.tokens, tok, tok % g.seq); }
+
+// cos and sin of all pairs at the CTA's tokens t0 .. t0 + n - 1, each computed once for all its heads.
+__device__ __forceinline__ void fill_table(const QkArgs& g, float2* table, int t0, int n) {
+  const int pairs = g.t.pairs;
+  for (int i = threadIdx.x; i < n * pairs; i += THREADS) {
+    const int tok = t0 + i / pairs;
+    if (tok < g.tokens) table[i] = cos_sin(g.t, i % pairs, place_at(g, tok));
   }
 }
 
 template <typename T, int LPR, bool INTER, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2) qk_backward_kernel(const QkArgs g) {
-  constexpr int GROUPS = THREADS / LPR, U = VEC ? 2 : 1;
-  __shared__ float sums[THREADS * 8];
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && VEC ? 7 : 5) qk_forward_kernel(const __grid_constant__ QkArgs g) {
+  constexpr int GROUPS = THREADS / LPR, U = !VEC ? 1 : sizeof(T) == 2 ? 4 : 2;   // rows on their way per group
+  __shared__ float2 table[GROUPS * LPR * S];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const Lane<INTER, VEC> ln(lane, g.d, g.t.pairs);
-  const int per_cta = GROUPS / g.per_token, part = group % g.per_token;
+  const bool keys = blockIdx.x >= g.q_ctas;
+  const Side& sd = g.side[keys];
+  const Lane<T, INTER, VEC> ln(lane, g.d, g.t.pairs);
+  const int per_cta = GROUPS / sd.per_token, first = group % sd.per_token, mine = group / sd.per_token;
+  const int t0 = (int)(blockIdx.x - (keys ? g.q_ctas : 0)) * per_cta, tok = t0 + mine;
+  const bool on = tok < g.tokens;
+  const int tc = min(tok, g.tokens - 1), ib = tc / g.seq, is = tc % g.seq;   // a group without a token works on the last one
+  const T* src = reinterpret_cast<const T*>(sd.x) + ib * sd.xb + is * sd.xt;
+  T* dst = reinterpret_cast<T*>(sd.y) + ib * sd.yb + is * sd.yt;
   const float inv_d = 1.f / (float)g.d;
-  const Row zero = {{0, 0}, {0, 0}};
-  Row acc[2] = {zero, zero};                               // the gains' gradients: queries, keys
-  for (long long t0 = (long long)blockIdx.x * per_cta; t0 < g.tokens; t0 += (long long)gridDim.x * per_cta) {
-    const long long tok = t0 + group / g.per_token;
-    const bool on = tok < g.tokens && ln.live;
-    const int tc = tok < g.tokens ? (int)tok : 0;
-    const int ib = tc / g.seq, is = tc % g.seq;
-    const Place at = place_of(g.pos, g.axes, g.tokens, tc, is);
-    Angle angle;
+  const int step = sd.per_token, heads = sd.heads;
+  Raw<T, VEC> raw[U];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const T* src = w == 0 ? reinterpret_cast<const T*>(g.q) + ib * g.qb + is * g.qt : reinterpret_cast<const T*>(g.k) + ib * g.kb + is * g.kt;
-      const T* up = w == 0 ? reinterpret_cast<const T*>(g.gq) + ib * g.gqb + is * g.gqt : reinterpret_cast<const T*>(g.gk) + ib * g.gkb + is * g.gkt;
-      T* dst = w == 0 ? reinterpret_cast<T*>(g.q_out) + ib * g.qob + is * g.qot : reinterpret_cast<T*>(g.k_out) + ib * g.kob + is * g.kot;
-      const long long sh = w == 0 ? g.qh : g.kh, uh = w == 0 ? g.gqh : g.gkh, dh = w == 0 ? g.qoh : g.koh;
-      const int heads = w == 0 ? g.q_heads : g.rows - g.q_heads;
-      const int first = w == 0 ? part : (part - g.q_heads) & (g.per_token - 1);
-      Row gain;
-      for (int r0 = 0; r0 < heads; r0 += U * g.per_token) {
-        Raw<T, VEC> rx[U], rg[U];
+  for (int u = 0; u < U; ++u) {
+    ln.clear(raw[u]);
+    ln.load(src + (long long)min(u * step + first, heads - 1) * sd.xh, raw[u]);
+  }
+  fill_table(g, table, t0, per_cta);                       // under the first loads
+  const Row gain = ln.gain(sd.gain);
+  __syncthreads();
+  const Coef k = coef(angle_from(table + mine * g.t.pairs, ln.j0, on ? g.t.pairs : 0), gain);
+  for (int r0 = 0;;) {                                     // the same trip count in every group
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int r = r0 + u * g.per_token + first;
-          ln.clear(rx[u]);
-          ln.clear(rg[u]);
-          if (on && r < heads) {
-            if (g.t.normalize) ln.load(src + r * sh, rx[u]);
-            ln.load(up + r * uh, rg[u]);
-          }
-        }
-        if (r0 == 0) {
-          if (w == 0 || g.q_heads == 0) {
-            angle = angle_at(g.t, ln.j0, at.p0, at.p1, at.p2);
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * step + first;
+      const Row y = transformed<LPR, VEC>(ln.row(raw[u]), k, g.t, ln.j0, inv_d);
+      if (on && r < heads) ln.store(dst + (long long)r * sd.yh, y);
+    }
+    r0 += U * step;
+    if (r0 >= heads) break;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) angle.s[e] = neg2(angle.s[e]);       // the gradient turns back
-          }
-          if (g.t.normalize) gain = ln.gain(reinterpret_cast<const T*>(w == 0 ? g.q_gain : g.k_gain));
-        }
+    for (int u = 0; u < U; ++u) ln.load(src + (long long)min(r0 + u * step + first, heads - 1) * sd.xh, raw[u]);
+  }
+}
+
+template <typename T, int LPR, bool INTER, bool VEC>
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && VEC ? 5 : 4) qk_backward_kernel(const __grid_constant__ QkArgs g) {
+  constexpr int GROUPS = THREADS / LPR, U = VEC ? 2 : 1;
+  __shared__ float2 table[GROUPS * LPR * S];
+  __shared__ float sums[THREADS * 2 * S];
+  asm volatile("griddepcontrol.launch_dependents;");       // the sum of the partial rows may be brought in; it waits for this
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
+  const bool keys = blockIdx.x >= g.q_ctas;
+  const Side& sd = g.side[keys];
+  const Lane<T, INTER, VEC> ln(lane, g.d, g.t.pairs);
+  const int per_cta = GROUPS / sd.per_token, first = group % sd.per_token, mine = group / sd.per_token;
+  const int step = sd.per_token, heads = sd.heads, pairs = g.t.pairs;
+  const int cta = (int)(blockIdx.x - (keys ? g.q_ctas : 0)), ctas = (int)(keys ? gridDim.x - g.q_ctas : g.q_ctas);
+  const float inv_d = 1.f / (float)g.d;
+  Row acc, gain;                                           // the gain's gradient; the gain
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int r = r0 + u * g.per_token + first;
-          Row h = turned<VEC>(ln.row(rg[u]), angle.c, angle.s, ln.j0, g.t.pairs);
-          if (g.t.normalize) {
-            // both sums before the reciprocal root is known:  sum x^2  and  sum h gain x
-            const Row x = ln.row(rx[u]), hx = times(h, x);
-            float sq, hg;
-            group_sum_pair<LPR>(dot(x, x), dot(hx, gain), sq, hg);
-            const float rs = rsqrtf(sq * inv_d + g.t.eps);
-            const f2 rs2 = both(rs), back = both(-(hg * inv_d) * rs * rs * rs);
+  for (int e = 0; e < S / 2; ++e) acc.a[e] = acc.b[e] = 0;
+  if (g.t.normalize) gain = ln.gain(sd.gain);
+  Raw<T, VEC> rx[U], rg[U];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              acc[w].a[e] = fma2(hx.a[e], rs2, acc[w].a[e]);
-              acc[w].b[e] = fma2(hx.b[e], rs2, acc[w].b[e]);
-              h.a[e] = fma2(h.a[e], mul2(gain.a[e], rs2), mul2(x.a[e], back));
-              h.b[e] = fma2(h.b[e], mul2(gain.b[e], rs2), mul2(x.b[e], back));
-            }
-          }
-          if (on && r < heads) ln.store(dst + r * dh, h);
-        }
+  for (int u = 0; u < U; ++u) {
+    ln.clear(rx[u]);
+    ln.clear(rg[u]);
+  }
+  for (int t0 = cta * per_cta; t0 < g.tokens; t0 += ctas * per_cta) {
+    const int tok = t0 + mine;
+    const bool on = tok < g.tokens;
+    const int tc = min(tok, g.tokens - 1), ib = tc / g.seq, is = tc % g.seq;
+    const T* src = reinterpret_cast<const T*>(sd.x) + ib * sd.xb + is * sd.xt;
+    const T* up = reinterpret_cast<const T*>(sd.up) + ib * sd.ub + is * sd.ut;
+    T* dst = reinterpret_cast<T*>(sd.y) + ib * sd.yb + is * sd.yt;
+    auto load = [&](int r0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = min(r0 + u * step + first, heads - 1);
+        if (g.t.normalize) ln.load(src + (long long)r * sd.xh, rx[u]);
+        ln.load(up + (long long)r * sd.uh, rg[u]);
       }
+    };
+    load(0);
+    __syncthreads();                                       // the table's last readers are done
+    fill_table(g, table, t0, per_cta);
+    __syncthreads();
+    Angle angle = angle_from(table + mine * pairs, ln.j0, on ? pairs : 0);
+#pragma unroll
+    for (int e = 0; e < S / 2; ++e) angle.s[e] = neg2(angle.s[e]);           // the gradient turns back
+    for (int r0 = 0;;) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * step + first;
+        const bool live = on && r < heads;
+        Row h = turned<VEC>(ln.row(rg[u]), angle, ln.j0, pairs);
+        if (g.t.normalize) {
+          // both sums before the reciprocal root is known:  sum x^2  and  sum h gain x
+          const Row x = ln.row(rx[u]), hx = times(h, x);
+          float sq, hg;
+          group_sum_pair<LPR>(dot(x, x), dot(hx, gain), sq, hg);
+          const float rs = rsqrtf(sq * inv_d + g.t.eps), b = -(hg * inv_d) * rs * rs * rs;
+          const f2 rs2 = pack(rs, rs), back = pack(b, b);
+#pragma unroll
+          for (int e = 0; e < S / 2; ++e) {
+            if (live) {
+              acc.a[e] = fma2(hx.a[e], rs2, acc.a[e]);
+              acc.b[e] = fma2(hx.b[e], rs2, acc.b[e]);
+            }
+            h.a[e] = fma2(h.a[e], mul2(gain.a[e], rs2), mul2(x.a[e], back));
+            h.b[e] = fma2(h.b[e], mul2(gain.b[e], rs2), mul2(x.b[e], back));
+          }
+        }
+        if (live) ln.store(dst + (long long)r * sd.yh, h);
+      }
+      r0 += U * step;
+      if (r0 >= heads) break;
+      load(r0);
     }
   }
   if (!g.partial) return;
-  float* out = g.partial + (long long)blockIdx.x * 2 * g.d;
+  float* out = g.partial + (long long)blockIdx.x * g.d;
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    float x[8];
-    unpack(acc[w].a[0], x[0], x[1]); unpack(acc[w].a[1], x[2], x[3]);
-    unpack(acc[w].b[0], x[4], x[5]); unpack(acc[w].b[1], x[6], x[7]);
-    __syncthreads();
+  for (int e = 0; e < S / 2; ++e) {
+    float x, y;
+    unpack(acc.a[e], x, y);
+    sums[(group * 2 * S + 2 * e) * LPR + lane] = x;
+    sums[(group * 2 * S + 2 * e + 1) * LPR + lane] = y;
+    unpack(acc.b[e], x, y);
+    sums[(group * 2 * S + S + 2 * e) * LPR + lane] = x;
+    sums[(group * 2 * S + S + 2 * e + 1) * LPR + lane] = y;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * S * LPR; i += THREADS) {
+    float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[(group * 8 + e) * LPR + lane] = x[e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 8 * LPR; i += THREADS) {
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < GROUPS; ++j) sum += sums[j * 8 * LPR + i];
-      const int e = i / LPR;
-      // INTER: a Row's values are a0..a3, b0..b3 whatever the runs' order
-      const Lane<INTER, VEC> who(i % LPR, g.d, g.t.pairs);
-      if (who.has(e & 3)) out[w * g.d + who.at(e)] = sum;
-    }
+    for (int j = 0; j < GROUPS; ++j) sum += sums[j * 2 * S * LPR + i];
+    const Lane<T, INTER, VEC> who(i % LPR, g.d, g.t.pairs);
+    if (who.has(i / LPR % S)) out[who.at(i / LPR)] = sum;
   }
 }
 
-// out[w][j] (+)= sum over the CTAs' rows, 8 rows at a time and their sums in order.
-__global__ void __launch_bounds__(256) gain_sum_kernel(const float* __restrict__ partial, int parts, int d,
-                                                       float* __restrict__ gq, float* __restrict__ gk, int accumulate) {
-  __shared__ float sh[8][33];
-  const int j = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+// Adds the CTAs' rows: each of 32 warps every 32nd of the queries' (or keys') rows, then the warps in order.
+__global__ void __launch_bounds__(1024) gain_sum_kernel(const float* __restrict__ partial, int q_parts, int k_parts, int d,
+                                                        float* __restrict__ gq, float* __restrict__ gk, int accumulate) {
+  __shared__ float sh[32][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // the rows are complete and visible
+  const bool keys = blockIdx.y;
+  const int lane = threadIdx.x & 31, j = blockIdx.x * 32 + lane, y = threadIdx.x >> 5;
+  const int parts = keys ? k_parts : q_parts;
+  if (keys) partial += (long long)q_parts * d;
   float x = 0.f;
-  if (j < 2 * d)
-    for (int p = y; p < parts; p += 8) x += partial[(long long)p * 2 * d + j];
-  sh[y][threadIdx.x & 31] = x;
+  if (j < d) {
+#pragma unroll 8
+    for (int p = y; p < parts; p += 32) x += partial[(long long)p * d + j];
+  }
+  sh[y][lane] = x;
   __syncthreads();
-  if (y || j >= 2 * d) return;
+  float* out = keys ? gk : gq;
+  if (y || j >= d || !out) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) x += sh[i][threadIdx.x];
-  float* out = j < d ? gq : gk;
-  if (!out) return;
-  out += j < d ? j : j - d;
-  *out = accumulate ? *out + x : x;
+  for (int i = 1; i < 32; ++i) x += sh[i][lane];
+  out[j] = accumulate ? out[j] + x : x;
 }
 
-constexpr int MAX_PARTS = 1024;
-
-bool vec_ok(int64_t es, const void* p, int64_t b, int64_t t, int64_t h) {
-  return ((uintptr_t)p % (4 * es)) == 0 && b % 4 == 0 && t % 4 == 0 && h % 4 == 0;
-}
+constexpr int MAX_PARTS = 2048;
 
 template <typename T, int LPR, bool INTER, bool VEC>
 int launch_one(const QkArgs& g, bool backward, unsigned grid, cudaStream_t stream) {
@@ -211,6 +227,7 @@ int launch_lpr(const QkArgs& g, bool inter, bool vec, bool backward, unsigned gr
 template <typename T>
 int launch_type(const QkArgs& g, bool inter, bool vec, bool backward, unsigned grid, cudaStream_t stream) {
   switch (lanes_per_row(g.d)) {
+    case 4: return launch_lpr<T, 4>(g, inter, vec, backward, grid, stream);
     case 8: return launch_lpr<T, 8>(g, inter, vec, backward, grid, stream);
     case 16: return launch_lpr<T, 16>(g, inter, vec, backward, grid, stream);
     default: return launch_lpr<T, 32>(g, inter, vec, backward, grid, stream);
@@ -219,7 +236,7 @@ int launch_type(const QkArgs& g, bool inter, bool vec, bool backward, unsigned g
 
 }  // namespace
 
-size_t qk_norm_rotary_backward_workspace_bytes(int64_t d) { return (size_t)MAX_PARTS * 2 * (size_t)d * sizeof(float); }
+size_t qk_norm_rotary_backward_workspace_bytes(int64_t d) { return (size_t)MAX_PARTS * (size_t)d * sizeof(float); }
 
 // Strides are [batch, token, head] of q, k, the upstream gradients (backward) and the outputs.
 int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t d,
@@ -232,42 +249,66 @@ int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq
   const DeviceState* ds = device_state();
   if (!ds) return note_cuda_error(cudaErrorInitializationError, "b200_init not called on this device");
   const int64_t es = dtype == B200_F32 ? 4 : 2;
-  g.tokens = batch * seq;
-  g.seq = (int)seq; g.q_heads = (int)q_heads; g.rows = (int)(q_heads + k_heads); g.d = (int)d;
+  g.tokens = (int)(batch * seq);
+  g.seq = (int)seq; g.d = (int)d;
   g.pos = positions;
-  g.q = in[0]; g.k = in[1]; g.gq = in[2]; g.gk = in[3];
-  g.q_out = out[0]; g.k_out = out[1];
-  g.qb = in_strides[0][0]; g.qt = in_strides[0][1]; g.qh = in_strides[0][2];
-  g.kb = in_strides[1][0]; g.kt = in_strides[1][1]; g.kh = in_strides[1][2];
-  g.gqb = in_strides[2][0]; g.gqt = in_strides[2][1]; g.gqh = in_strides[2][2];
-  g.gkb = in_strides[3][0]; g.gkt = in_strides[3][1]; g.gkh = in_strides[3][2];
-  g.qob = out_strides[0][0]; g.qot = out_strides[0][1]; g.qoh = out_strides[0][2];
-  g.kob = out_strides[1][0]; g.kot = out_strides[1][1]; g.koh = out_strides[1][2];
-  g.q_gain = op->q_gain; g.k_gain = op->k_gain;
   const bool inter = op->interleaved != 0;
   bool vec = d % 8 == 0 && g.t.pairs % 4 == 0;
-  for (int i = 0; i < (backward ? 4 : 2); ++i) vec = vec && vec_ok(es, in[i], in_strides[i][0], in_strides[i][1], in_strides[i][2]);
-  for (int i = 0; i < 2; ++i) vec = vec && vec_ok(es, out[i], out_strides[i][0], out_strides[i][1], out_strides[i][2]);
-  // Groups that share a token: as few as still give every SM's 2048 threads a group (the sines are then computed for
-  // the most heads), and no more than the token has rows.
   const int lpr = lanes_per_row(d), groups = THREADS / lpr;
-  const int64_t want = (int64_t)ds->sm_count * (2048 / lpr);
-  g.per_token = 1;
-  while (g.per_token < groups && g.per_token < g.rows && g.tokens * g.per_token < want) g.per_token *= 2;
-  const int64_t per_cta = groups / g.per_token;
-  int64_t grid = (g.tokens + per_cta - 1) / per_cta;
+  const int64_t want = (int64_t)ds->sm_count * (2048 / lpr);                 // groups that fill every SM
+  int64_t ctas[2] = {0, 0}, work = 0;
+  for (int w = 0; w < 2; ++w) {
+    Side& sd = g.side[w];
+    sd.x = in[w]; sd.up = in[2 + w]; sd.y = out[w];
+    sd.gain = w == 0 ? op->q_gain : op->k_gain;
+    sd.heads = (int)(w == 0 ? q_heads : k_heads);
+    const int64_t *xs = in_strides[w], *us = in_strides[2 + w], *ys = out_strides[w];
+    if (xs[2] > 0x7fffffff || us[2] > 0x7fffffff || ys[2] > 0x7fffffff) return B200_ERR_LIMIT;
+    sd.xb = xs[0]; sd.xt = xs[1]; sd.xh = (int)xs[2];
+    sd.ub = us[0]; sd.ut = us[1]; sd.uh = (int)us[2];
+    sd.yb = ys[0]; sd.yt = ys[1]; sd.yh = (int)ys[2];
+    sd.per_token = 1;
+    if (sd.heads == 0 || g.tokens == 0) continue;
+    vec = vec && vec_ok(es, sd.x, sd.xb, sd.xt, sd.xh) && vec_ok(es, sd.y, sd.yb, sd.yt, sd.yh);
+    if (backward) vec = vec && vec_ok(es, sd.up, sd.ub, sd.ut, sd.uh);
+    // Groups that share a token: at most eight heads each, so that CTAs are short and end together, and more while the
+    // groups of all tokens would leave SMs without work.
+    while (sd.per_token < groups && sd.per_token < sd.heads && (sd.heads > 8 * sd.per_token || (int64_t)g.tokens * sd.per_token < want))
+      sd.per_token *= 2;
+    ctas[w] = (g.tokens + groups / sd.per_token - 1) / (groups / sd.per_token);
+    work += ctas[w];
+  }
+  // Backward: what is resident at once, shared out by the work; each CTA's sums are a row to add up at the end.
+  const int64_t resident = (int64_t)ds->sm_count * (es == 2 && vec ? 5 : 4), most = resident < MAX_PARTS ? resident : MAX_PARTS;
+  if (backward && work > most) {
+    const int64_t share = ctas[0] * most / work;
+    ctas[0] = ctas[0] ? (share > 0 ? share : 1) : 0;
+    ctas[1] = ctas[1] ? (most - ctas[0] > 0 ? most - ctas[0] : 1) : 0;
+  }
   const bool sums = backward && g.t.normalize && (q_gain_grad || k_gain_grad);
   g.partial = sums ? (float*)workspace : nullptr;
-  if (backward && grid > (int64_t)ds->sm_count * 4) grid = (int64_t)ds->sm_count * 4;
-  if (backward && grid > MAX_PARTS) grid = MAX_PARTS;
-  if (grid > 0x7fffffff) grid = 0x7fffffff;
-  if (g.rows == 0) grid = 0;
-  int rc2 = grid == 0 ? B200_OK : dtype == B200_F32 ? launch_type<float>(g, inter, vec, backward, (unsigned)grid, stream)
-                              : launch_type<__half>(g, inter, vec, backward, (unsigned)grid, stream);   // an empty batch: sums over nothing follow
-  if (rc2 || !sums) return rc2;
-  gain_sum_kernel<<<(unsigned)((2 * d + 31) / 32), 256, 0, stream>>>(g.partial, (int)grid, (int)d, q_gain_grad, k_gain_grad, accumulate);
+  g.q_ctas = (unsigned)ctas[0];
+  const int64_t grid = ctas[0] + ctas[1];
+  if (grid > 0x7fffffff) return B200_ERR_LIMIT;
+  if (grid) {                                              // an empty batch: sums over nothing follow
+    const int rc2 = dtype == B200_F32 ? launch_type<float>(g, inter, vec, backward, (unsigned)grid, stream)
+                                      : launch_type<__half>(g, inter, vec, backward, (unsigned)grid, stream);
+    if (rc2) return rc2;
+  }
+  if (!sums) return B200_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((d + 31) / 32), 2);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = stream;
+  cudaLaunchAttribute early;                               // its launch overlaps the end of the kernel before it
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  const int rc3 = note_cuda_error(cudaLaunchKernelEx(&cfg, gain_sum_kernel, (const float*)g.partial, (int)ctas[0], (int)ctas[1], (int)d,
+                                                     q_gain_grad, k_gain_grad, accumulate), "gain gradient launch");
   count_launch(false);
-  return note_cuda_error(cudaGetLastError(), "gain gradient launch");
+  return rc3;
 }
 
 }  // namespace b200
