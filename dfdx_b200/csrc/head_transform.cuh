@@ -23,7 +23,6 @@ namespace b200 {
 namespace heads {
 
 constexpr int MAX_D = 256;
-constexpr int S = 4;               // slots of a lane
 constexpr int AXES = 3;
 
 struct Transform {
@@ -39,43 +38,30 @@ __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x); }
 
-// Two f32 in one register pair: Blackwell's packed multiply, add and multiply-add take one issue slot for both.
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 pack(float x, float y) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpack(f2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-  f2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f2 neg2(f2 v) { return v ^ 0x8000000080000000ull; }
+// Two f32 side by side.  (Blackwell's packed f32x2 instructions were tried here: what they save in arithmetic goes into
+// moving values into register pairs, 70 us against 66 for the forward of 16384 tokens, 40 heads of 128.)
+struct f2 { float x, y; };
+__device__ __forceinline__ f2 pack(float x, float y) { return {x, y}; }
+__device__ __forceinline__ void unpack(f2 v, float& x, float& y) { x = v.x; y = v.y; }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { return {a.x * b.x, a.y * b.y}; }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { return {a.x + b.x, a.y + b.y}; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { return {fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)}; }
+__device__ __forceinline__ f2 neg2(f2 v) { return {-v.x, -v.y}; }
 
 // A lane's 2 S elements of a row: the pairs' first elements a = (a0, a1), (a2, a3), ... and their second ones b.
-struct Row {
+template <int S> struct Row {
   f2 a[S / 2], b[S / 2];
 };
-__device__ __forceinline__ f2 dot(const Row& x, const Row& y) {          // two partial sums
+template <int S>
+__device__ __forceinline__ f2 dot(const Row<S>& x, const Row<S>& y) {          // two partial sums
   f2 r = mul2(x.a[0], y.a[0]), t = mul2(x.b[0], y.b[0]);
 #pragma unroll
   for (int e = 1; e < S / 2; ++e) { r = fma2(x.a[e], y.a[e], r); t = fma2(x.b[e], y.b[e], t); }
   return add2(r, t);
 }
-__device__ __forceinline__ Row times(const Row& x, const Row& y) {
-  Row r;
+template <int S>
+__device__ __forceinline__ Row<S> times(const Row<S>& x, const Row<S>& y) {
+  Row<S> r;
 #pragma unroll
   for (int e = 0; e < S / 2; ++e) { r.a[e] = mul2(x.a[e], y.a[e]); r.b[e] = mul2(x.b[e], y.b[e]); }
   return r;
@@ -83,9 +69,10 @@ __device__ __forceinline__ Row times(const Row& x, const Row& y) {
 
 // A row's elements as they were loaded: two runs of S (VEC), f16 still packed.  Holding these rather than the f32 values
 // lets a lane have several rows on their way in few registers.
-template <typename T, bool VEC> struct Raw { float x[2 * S]; };
-template <> struct Raw<__half, true> { uint2 u, v; };
-template <> struct Raw<float, true> { uint4 u, v; };
+template <typename T, int S, bool VEC> struct Raw { float x[2 * S]; };
+template <> struct Raw<__half, 8, true> { uint4 u, v; };
+template <> struct Raw<__half, 4, true> { uint2 u, v; };
+template <> struct Raw<float, 4, true> { uint4 u, v; };
 
 __device__ __forceinline__ float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ uint32_t half2_of(float x, float y) {
@@ -96,7 +83,7 @@ __device__ __forceinline__ uint32_t half2_of(float x, float y) {
 // Where a lane's 2 S elements lie.  off_u and off_v start the two runs of S that a vector access moves (VEC: whole lanes
 // rotate or none of it, the number of pairs being a multiple of S); a and b are the pairs' elements.  Interleaved, the
 // elements are consecutive and a, b alternate through them.
-template <typename T, bool INTER, bool VEC>
+template <typename T, int S, bool INTER, bool VEC>
 struct Lane {
   int j0, d, pairs, off_u, off_v;
   bool live;                       // the lane has elements
@@ -116,9 +103,9 @@ struct Lane {
     return e < S ? at_a(e) : at_b(e - S);
   }
 
-  typedef Raw<T, VEC> R;
+  typedef Raw<T, S, VEC> R;
   __device__ __forceinline__ void clear(R& r) const {      // what a lane without elements holds
-    if constexpr (VEC && sizeof(T) == 2) {
+    if constexpr (VEC && sizeof(T) * S == 8) {
       r.u = r.v = make_uint2(0, 0);
     } else if constexpr (VEC) {
       r.u = r.v = make_uint4(0, 0, 0, 0);
@@ -138,8 +125,8 @@ struct Lane {
         if (has(e % S)) r.x[e] = to_f(row[at(e)]);
     }
   }
-  __device__ __forceinline__ Row row(const R& r) const {
-    Row x;
+  __device__ __forceinline__ Row<S> row(const R& r) const {
+    Row<S> x;
     if constexpr (!VEC) {
 #pragma unroll
       for (int e = 0; e < S / 2; ++e) { x.a[e] = pack(r.x[2 * e], r.x[2 * e + 1]); x.b[e] = pack(r.x[S + 2 * e], r.x[S + 2 * e + 1]); }
@@ -149,6 +136,11 @@ struct Lane {
         const float2 p = halves(r.u.x), q = halves(r.u.y), w = halves(r.v.x), z = halves(r.v.y);
         u[0] = p.x; u[1] = p.y; u[2] = q.x; u[3] = q.y;
         v[0] = w.x; v[1] = w.y; v[2] = z.x; v[3] = z.y;
+        if constexpr (S == 8) {
+          const float2 p2 = halves(r.u.z), q2 = halves(r.u.w), w2 = halves(r.v.z), z2 = halves(r.v.w);
+          u[4] = p2.x; u[5] = p2.y; u[6] = q2.x; u[7] = q2.y;
+          v[4] = w2.x; v[5] = w2.y; v[6] = z2.x; v[7] = z2.y;
+        }
       } else {
         u[0] = __uint_as_float(r.u.x); u[1] = __uint_as_float(r.u.y); u[2] = __uint_as_float(r.u.z); u[3] = __uint_as_float(r.u.w);
         v[0] = __uint_as_float(r.v.x); v[1] = __uint_as_float(r.v.y); v[2] = __uint_as_float(r.v.z); v[3] = __uint_as_float(r.v.w);
@@ -168,7 +160,7 @@ struct Lane {
     return x;
   }
   // the values in the runs' order (VEC); otherwise the a, then the b
-  __device__ __forceinline__ void values(const Row& x, float (&u)[S], float (&v)[S]) const {
+  __device__ __forceinline__ void values(const Row<S>& x, float (&u)[S], float (&v)[S]) const {
 #pragma unroll
     for (int e = 0; e < S / 2; ++e) {
       if constexpr (INTER && VEC) {
@@ -181,7 +173,7 @@ struct Lane {
       }
     }
   }
-  __device__ __forceinline__ void store(T* row, const Row& x) const {
+  __device__ __forceinline__ void store(T* row, const Row<S>& x) const {
     float u[S], v[S];
     values(x, u, v);
     if constexpr (!VEC) {
@@ -190,20 +182,25 @@ struct Lane {
         if (has(e)) { put(row + at(e), u[e]); put(row + at(S + e), v[e]); }
     } else if constexpr (sizeof(T) == 2) {
       if (!live) return;
-      *reinterpret_cast<uint2*>(row + off_u) = make_uint2(half2_of(u[0], u[1]), half2_of(u[2], u[3]));
-      *reinterpret_cast<uint2*>(row + off_v) = make_uint2(half2_of(v[0], v[1]), half2_of(v[2], v[3]));
+      if constexpr (S == 8) {
+        *reinterpret_cast<uint4*>(row + off_u) = make_uint4(half2_of(u[0], u[1]), half2_of(u[2], u[3]), half2_of(u[4], u[5]), half2_of(u[6], u[7]));
+        *reinterpret_cast<uint4*>(row + off_v) = make_uint4(half2_of(v[0], v[1]), half2_of(v[2], v[3]), half2_of(v[4], v[5]), half2_of(v[6], v[7]));
+      } else {
+        *reinterpret_cast<uint2*>(row + off_u) = make_uint2(half2_of(u[0], u[1]), half2_of(u[2], u[3]));
+        *reinterpret_cast<uint2*>(row + off_v) = make_uint2(half2_of(v[0], v[1]), half2_of(v[2], v[3]));
+      }
     } else {
       if (!live) return;
       *reinterpret_cast<float4*>(row + off_u) = make_float4(u[0], u[1], u[2], u[3]);
       *reinterpret_cast<float4*>(row + off_v) = make_float4(v[0], v[1], v[2], v[3]);
     }
   }
-  __device__ __forceinline__ Row gain(const void* p) const {
+  __device__ __forceinline__ Row<S> gain(const void* p) const {
     const T* g = reinterpret_cast<const T*>(p);
     float x[2 * S];
 #pragma unroll
     for (int e = 0; e < 2 * S; ++e) x[e] = g && has(e % S) ? to_f(g[at(e)]) : 1.f;
-    Row r;
+    Row<S> r;
 #pragma unroll
     for (int e = 0; e < S / 2; ++e) { r.a[e] = pack(x[2 * e], x[2 * e + 1]); r.b[e] = pack(x[S + 2 * e], x[S + 2 * e + 1]); }
     return r;
@@ -211,33 +208,35 @@ struct Lane {
 };
 
 // cos and sin of a lane's slots at a token's positions; 1 and 0 where nothing rotates.
-struct Angle {
+template <int S> struct Angle {
   f2 c[S / 2], s[S / 2];
 };
-// cos and sin of pair j at a place.
 struct Place { int p0, p1, p2; };
-__device__ __forceinline__ float2 cos_sin(const Transform& t, int j, const Place& p) {
-  double x = (double)(j < t.end0 ? p.p0 : j < t.end1 ? p.p1 : p.p2) * (__ldg(t.freq + j) * 0.15915494309189535);
+// cos and sin of pair j at a place, from the pair's turns per position.
+__device__ __forceinline__ double turns_of(const Transform& t, int j) { return __ldg(t.freq + j) * 0.15915494309189535; }
+__device__ __forceinline__ float2 cos_sin(const Transform& t, int j, double per_pos, const Place& p) {
+  double x = (double)(j < t.end0 ? p.p0 : j < t.end1 ? p.p1 : p.p2) * per_pos;
   x -= rint(x);
   float2 r;
   sincospif(2.f * (float)x, &r.y, &r.x);
   return r;
 }
-__device__ __forceinline__ Angle angle_at(const Transform& t, int j0, const Place& p) {
-  Angle r;
-#pragma unroll
-  for (int i = 0; i < S / 2; ++i) {
-    const int j = j0 + 2 * i;
-    const float2 x = j < t.pairs ? cos_sin(t, j, p) : make_float2(1.f, 0.f);
-    const float2 y = j + 1 < t.pairs ? cos_sin(t, j + 1, p) : make_float2(1.f, 0.f);
-    r.c[i] = pack(x.x, y.x);
-    r.s[i] = pack(x.y, y.y);
+// Fills table[i * pairs + j] with cos and sin of pair j at place_at(i) for i < n: a thread keeps to one pair.
+template <int NT, typename At>
+__device__ __forceinline__ void fill_table(const Transform& t, float2* table, int n, At place_at) {
+  if (t.pairs == 0) return;
+  const int lead = t.pairs < NT ? t.pairs : NT;            // pairs at a time; the threads beyond take further places
+  const int j0 = threadIdx.x % lead, i0 = threadIdx.x / lead, stride = NT / lead;
+  if (i0 >= stride) return;
+  for (int j = j0; j < t.pairs; j += lead) {
+    const double per_pos = turns_of(t, j);
+    for (int i = i0; i < n; i += stride) table[i * t.pairs + j] = cos_sin(t, j, per_pos, place_at(i));
   }
-  return r;
 }
-// The same from a table of all pairs of one place.
-__device__ __forceinline__ Angle angle_from(const float2* table, int j0, int pairs) {
-  Angle r;
+// A lane's from a table of all pairs of one place.
+template <int S>
+__device__ __forceinline__ Angle<S> angle_from(const float2* table, int j0, int pairs) {
+  Angle<S> r;
 #pragma unroll
   for (int i = 0; i < S / 2; ++i) {
     const int j = j0 + 2 * i;
@@ -257,10 +256,10 @@ __device__ __forceinline__ f2 kept(f2 turned, f2 plain, int j, int pairs) {
   return pack(j < pairs ? t[0] : p[0], j + 1 < pairs ? t[1] : p[1]);
 }
 
-template <bool VEC>
-__device__ __forceinline__ Row turned(const Row& x, const Angle& t, int j0, int pairs) {
+template <int S, bool VEC>
+__device__ __forceinline__ Row<S> turned(const Row<S>& x, const Angle<S>& t, int j0, int pairs) {
   if (VEC && j0 >= pairs) return x;
-  Row y;
+  Row<S> y;
 #pragma unroll
   for (int e = 0; e < S / 2; ++e) {
     y.a[e] = fma2(x.b[e], neg2(t.s[e]), mul2(x.a[e], t.c[e]));
@@ -290,7 +289,7 @@ __device__ __forceinline__ void group_sum_pair(f2 v, f2 w, float& x, float& y) {
   unpack(w, c, d);
   f2 z = add2(pack(a, c), pack(b, d));
 #pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) z = add2(z, __shfl_xor_sync(0xffffffffu, z, o));
+  for (int o = LPR / 2; o > 0; o >>= 1) z = add2(z, f2{__shfl_xor_sync(0xffffffffu, z.x, o), __shfl_xor_sync(0xffffffffu, z.y, o)});
   unpack(z, x, y);
 }
 __device__ __forceinline__ float warp_max(float x) {
@@ -301,11 +300,12 @@ __device__ __forceinline__ float warp_max(float x) {
 
 // gain * x / sqrt(mean(x^2) + eps), then the turn: the whole forward transform of a row.  The gain is folded into the
 // angle, which serves all heads of a token: what is left is one scale by the reciprocal root.
-struct Coef {
+template <int S> struct Coef {
   f2 ac[S / 2], bs[S / 2], bc[S / 2], as[S / 2];           // gain_a cos, -gain_b sin, gain_b cos, gain_a sin
 };
-__device__ __forceinline__ Coef coef(const Angle& t, const Row& gain) {
-  Coef k;
+template <int S>
+__device__ __forceinline__ Coef<S> coef(const Angle<S>& t, const Row<S>& gain) {
+  Coef<S> k;
 #pragma unroll
   for (int e = 0; e < S / 2; ++e) {
     k.ac[e] = mul2(gain.a[e], t.c[e]);
@@ -315,10 +315,10 @@ __device__ __forceinline__ Coef coef(const Angle& t, const Row& gain) {
   }
   return k;
 }
-template <int LPR, bool VEC>
-__device__ __forceinline__ Row transformed(const Row& x, const Coef& k, const Transform& t, int j0, float inv_d) {
-  Row y;
-  f2 rs = 0;
+template <int S, int LPR, bool VEC>
+__device__ __forceinline__ Row<S> transformed(const Row<S>& x, const Coef<S>& k, const Transform& t, int j0, float inv_d) {
+  Row<S> y;
+  f2 rs = {0.f, 0.f};
   if (t.normalize) {
     const float r = rsqrtf(group_sum<LPR>(dot(x, x)) * inv_d + t.eps);
     rs = pack(r, r);
@@ -371,12 +371,16 @@ inline int parse(const b200_head_op* op, size_t d, Transform* t, int* axes) {
   return B200_OK;
 }
 
-// Whether the rows of an operand can be moved four elements at a time.
-inline bool vec_ok(int64_t es, const void* p, int64_t s0, int64_t s1, int64_t s2) {
-  return ((uintptr_t)p % (4 * es)) == 0 && s0 % 4 == 0 && s1 % 4 == 0 && s2 % 4 == 0;
+// Whether the rows of an operand can be moved n elements at a time.
+inline bool vec_ok(int n, int64_t es, const void* p, int64_t s0, int64_t s1, int64_t s2) {
+  return ((uintptr_t)p % (n * es)) == 0 && s0 % n == 0 && s1 % n == 0 && s2 % n == 0;
 }
 // Lanes that share a row.
-inline int lanes_per_row(int64_t d) { return d <= 32 ? 4 : d <= 64 ? 8 : d <= 128 ? 16 : 32; }
+inline int lanes_per_row(int64_t d, int slots) {
+  int n = 4;
+  while (n * 2 * slots < d) n *= 2;
+  return n;
+}
 
 }  // namespace heads
 }  // namespace b200

@@ -60,34 +60,31 @@ __device__ __forceinline__ void append_queries(const AppendArgs& g, unsigned cta
   constexpr int GROUPS = NT / LPR, U = !VEC ? 1 : sizeof(T) == 2 ? 4 : 2;      // rows on their way per group
   __shared__ int slots[GROUPS];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR, pairs = g.t.pairs;
-  const Lane<T, INTER, VEC> ln(lane, g.cache.d, pairs);
+  const Lane<T, 4, INTER, VEC> ln(lane, g.cache.d, pairs);
   const int per_cta = GROUPS / g.per_token, first = group % g.per_token, mine = group / g.per_token, step = g.per_token;
   const int t0 = (int)cta * per_cta, tok = t0 + mine, heads = g.q_heads;
   const int tc = min(tok, g.batch.tokens - 1);
   const T* q = reinterpret_cast<const T*>(g.q) + tc * g.qt;
   T* qo = reinterpret_cast<T*>(g.q_out) + tc * g.qot;
   const float inv_d = 1.f / (float)g.cache.d;
-  Raw<T, VEC> raw[U];
+  Raw<T, 4, VEC> raw[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     ln.clear(raw[u]);
     ln.load(q + (long long)min(u * step + first, heads - 1) * g.qh, raw[u]);
   }
   if (threadIdx.x < per_cta) slots[threadIdx.x] = slot_of(g, t0 + threadIdx.x);
-  const Row gain = ln.gain(g.q_gain);
+  const Row<4> gain = ln.gain(g.q_gain);
   __syncthreads();
-  for (int i = threadIdx.x; i < per_cta * pairs; i += NT) {
-    const int t = i / pairs;
-    if (slots[t] >= 0) table[i] = cos_sin(g.t, i % pairs, place_of(g.pos, g.axes, g.batch.tokens, t0 + t, slots[t]));
-  }
+  fill_table<NT>(g.t, table, per_cta, [&](int i) { return place_of(g.pos, g.axes, g.batch.tokens, min(t0 + i, g.batch.tokens - 1), slots[i]); });
   __syncthreads();
   const bool on = slots[mine] >= 0;                        // a token of no sequence is left alone
-  const Coef k = coef(angle_from(table + mine * pairs, ln.j0, on ? pairs : 0), gain);
+  const Coef<4> k = coef(angle_from<4>(table + mine * pairs, ln.j0, on ? pairs : 0), gain);
   for (int r0 = 0;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int r = r0 + u * step + first;
-      const Row y = transformed<LPR, VEC>(ln.row(raw[u]), k, g.t, ln.j0, inv_d);
+      const Row<4> y = transformed<4, LPR, VEC>(ln.row(raw[u]), k, g.t, ln.j0, inv_d);
       if (on && r < heads) ln.store(qo + (long long)r * g.qoh, y);
     }
     r0 += U * step;
@@ -99,16 +96,16 @@ __device__ __forceinline__ void append_queries(const AppendArgs& g, unsigned cta
 
 // A lane's eight values of a row to their codes: words where the rows may be written in vectors.
 template <typename T, bool INTER, bool VEC>
-__device__ __forceinline__ void store_codes(const Lane<T, INTER, VEC>& ln, uint8_t* row, const Row& x, float inv) {
-  float u[S], v[S];
+__device__ __forceinline__ void store_codes(const Lane<T, 4, INTER, VEC>& ln, uint8_t* row, const Row<4>& x, float inv) {
+  float u[4], v[4];
   ln.values(x, u, v);
   const uint32_t cu = codes4(u, inv), cv = codes4(v, inv);
   if constexpr (!VEC) {
 #pragma unroll
-    for (int e = 0; e < S; ++e)
+    for (int e = 0; e < 4; ++e)
       if (ln.has(e)) {
         row[ln.at(e)] = (uint8_t)(cu >> (8 * e));
-        row[ln.at(S + e)] = (uint8_t)(cv >> (8 * e));
+        row[ln.at(4 + e)] = (uint8_t)(cv >> (8 * e));
       }
   } else if (ln.live) {
     *reinterpret_cast<uint32_t*>(row + ln.off_u) = cu;
@@ -116,11 +113,11 @@ __device__ __forceinline__ void store_codes(const Lane<T, INTER, VEC>& ln, uint8
   }
 }
 template <typename T, bool INTER, bool VEC>
-__device__ __forceinline__ float top_of(const Lane<T, INTER, VEC>& ln, const Row& x) {
-  float u[S], v[S], top = 0.f;
+__device__ __forceinline__ float top_of(const Lane<T, 4, INTER, VEC>& ln, const Row<4>& x) {
+  float u[4], v[4], top = 0.f;
   ln.values(x, u, v);
 #pragma unroll
-  for (int e = 0; e < S; ++e) top = fmaxf(top, fmaxf(finite_abs(u[e]), finite_abs(v[e])));
+  for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(finite_abs(u[e]), finite_abs(v[e])));
   return top;
 }
 
@@ -172,13 +169,13 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC 
   }
   const int rows = slot1 - slot0, row0 = slot0 & (page - 1), tok0 = q.first + (slot0 - start), pairs = g.t.pairs;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const Lane<T, INTER, VEC> ln(lane, g.cache.d, pairs);
+  const Lane<T, 4, INTER, VEC> ln(lane, g.cache.d, pairs);
   const float inv_d = 1.f / (float)g.cache.d;
   const T* src = values ? reinterpret_cast<const T*>(g.v) + tok0 * g.vt : reinterpret_cast<const T*>(g.k) + tok0 * g.kt;
   const long long step = values ? g.vt : g.kt;
   const int hs = values ? g.vh : g.kh;
   const bool change = !values && (g.t.normalize || pairs);
-  Raw<T, VEC> raw[ROWS];
+  Raw<T, 4, VEC> raw[ROWS];
   auto load = [&](int head) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)                         // groups without a row take the last one again
@@ -187,13 +184,10 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC 
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) ln.clear(raw[i]);
   load(head0);
-  Row gain;
+  Row<4> gain;
   if (change) {
     gain = ln.gain(g.k_gain);
-    for (int i = threadIdx.x; i < rows * pairs; i += NT) {
-      const int r = i / pairs;
-      table[i] = cos_sin(g.t, i % pairs, place_of(g.pos, g.axes, g.batch.tokens, tok0 + r, slot0 + r));
-    }
+    fill_table<NT>(g.t, table, rows, [&](int i) { return place_of(g.pos, g.axes, g.batch.tokens, tok0 + i, slot0 + i); });
     __syncthreads();
   }
   for (int head = head0; head < head1; ++head) {
@@ -202,15 +196,15 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC 
     uint8_t* codes = (values ? g.cache.v : g.cache.k) + block * page * g.cache.d;
     const float old = row0 ? *scale : 0.f;
     if (!AHEAD && head > head0) load(head);
-    Row x[ROWS];
+    Row<4> x[ROWS];
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       if (i * GROUPS >= rows) break;                       // the same in every group: the sums inside stay whole
       x[i] = ln.row(raw[i]);
       if (change) {
-        const Angle t = angle_from(table + min(group + i * GROUPS, rows - 1) * pairs, ln.j0, pairs);
-        x[i] = transformed<LPR, VEC>(x[i], coef(t, gain), g.t, ln.j0, inv_d);
+        const Angle<4> t = angle_from<4>(table + min(group + i * GROUPS, rows - 1) * pairs, ln.j0, pairs);
+        x[i] = transformed<4, LPR, VEC>(x[i], coef(t, gain), g.t, ln.j0, inv_d);
       }
       top = fmaxf(top, top_of(ln, x[i]));
     }
@@ -331,8 +325,8 @@ int kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* 
   g.q_gain = op->q_gain; g.k_gain = op->k_gain;
   g.status = ds->status;
   const bool inter = op->interleaved != 0;
-  bool vec = g.t.pairs % 4 == 0 && vec_ok(es, k, 0, ks[0], ks[1]) && vec_ok(es, v, 0, vs[0], vs[1]);
-  if (g.q_heads) vec = vec && vec_ok(es, q, 0, qs[0], qs[1]) && vec_ok(es, q_out, 0, qos[0], qos[1]);
+  bool vec = g.t.pairs % 4 == 0 && vec_ok(4, es, k, 0, ks[0], ks[1]) && vec_ok(4, es, v, 0, vs[0], vs[1]);
+  if (g.q_heads) vec = vec && vec_ok(4, es, q, 0, qs[0], qs[1]) && vec_ok(4, es, q_out, 0, qos[0], qos[1]);
   const int lpr = vec && g.cache.d <= 64 ? 8 : 16, groups = (g.batch.max_new == 1 ? NT_ONE : NT_MANY) / lpr;
   // a sequence's m new tokens touch at most (m - 1) / page + 2 pages, one token only one
   const int64_t units = g.batch.max_new == 1 ? g.batch.seqs : (int64_t)(g.batch.tokens >> g.cache.page_log2) + 2 * (int64_t)g.batch.seqs;

@@ -22,180 +22,197 @@ struct Side {                      // queries or keys
   const void *x, *up;              // input; upstream gradient (backward)
   void* y;                         // output; gradient (backward)
   const void* gain;
-  int heads, per_token;            // per_token: groups that share a token
+  int heads;
   int xh, uh, yh;                  // element strides of the head, batch and token axes
   long long xb, xt, ub, ut, yb, yt;
 };
 struct QkArgs {
   Transform t;
   Side side[2];
-  unsigned q_ctas;                 // the CTAs behind them have keys
   int tokens, seq;                 // batch * tokens of a sequence
-  int d, axes;
+  int d, axes, per_token;          // per_token: groups that share a token
   const int* pos;                  // axes x tokens, or nullptr: the index in the sequence on every axis
-  float* partial;                  // backward: a row of d sums per CTA, or nullptr
+  float* partial;                  // backward: 2 x gridDim.x rows of d sums, or nullptr
 };
 
 constexpr int THREADS = 128;
 
-__device__ __forceinline__ Place place_at(const QkArgs& g, int tok) { return place_of(g.pos, g.axes, g.tokens, tok, tok % g.seq); }
-
-// cos and sin of all pairs at the CTA's tokens t0 .. t0 + n - 1, each computed once for all its heads.
-__device__ __forceinline__ void fill_table(const QkArgs& g, float2* table, int t0, int n) {
-  const int pairs = g.t.pairs;
-  for (int i = threadIdx.x; i < n * pairs; i += THREADS) {
-    const int tok = t0 + i / pairs;
-    if (tok < g.tokens) table[i] = cos_sin(g.t, i % pairs, place_at(g, tok));
-  }
-}
-
-template <typename T, int LPR, bool INTER, bool VEC>
-__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && VEC ? 7 : 5) qk_forward_kernel(const __grid_constant__ QkArgs g) {
-  constexpr int GROUPS = THREADS / LPR, U = !VEC ? 1 : sizeof(T) == 2 ? 4 : 2;   // rows on their way per group
+template <typename T, int S, int LPR, bool INTER, bool VEC>
+__global__ void __launch_bounds__(THREADS, S == 8 ? 5 : sizeof(T) == 2 && VEC ? 6 : 5) qk_forward_kernel(const __grid_constant__ QkArgs g) {
+  constexpr int GROUPS = THREADS / LPR, U = !VEC ? 1 : S * sizeof(T) == 8 ? 4 : 2;   // rows on their way per group
   __shared__ float2 table[GROUPS * LPR * S];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const bool keys = blockIdx.x >= g.q_ctas;
-  const Side& sd = g.side[keys];
-  const Lane<T, INTER, VEC> ln(lane, g.d, g.t.pairs);
-  const int per_cta = GROUPS / sd.per_token, first = group % sd.per_token, mine = group / sd.per_token;
-  const int t0 = (int)(blockIdx.x - (keys ? g.q_ctas : 0)) * per_cta, tok = t0 + mine;
+  const Lane<T, S, INTER, VEC> ln(lane, g.d, g.t.pairs);
+  const int step = g.per_token, per_cta = GROUPS / step, part = group % step, mine = group / step;
+  const int t0 = (int)blockIdx.x * per_cta, tok = t0 + mine;
   const bool on = tok < g.tokens;
   const int tc = min(tok, g.tokens - 1), ib = tc / g.seq, is = tc % g.seq;   // a group without a token works on the last one
-  const T* src = reinterpret_cast<const T*>(sd.x) + ib * sd.xb + is * sd.xt;
-  T* dst = reinterpret_cast<T*>(sd.y) + ib * sd.yb + is * sd.yt;
   const float inv_d = 1.f / (float)g.d;
-  const int step = sd.per_token, heads = sd.heads;
-  Raw<T, VEC> raw[U];
+  Raw<T, S, VEC> raw[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    ln.clear(raw[u]);
-    ln.load(src + (long long)min(u * step + first, heads - 1) * sd.xh, raw[u]);
-  }
-  fill_table(g, table, t0, per_cta);                       // under the first loads
-  const Row gain = ln.gain(sd.gain);
-  __syncthreads();
-  const Coef k = coef(angle_from(table + mine * g.t.pairs, ln.j0, on ? g.t.pairs : 0), gain);
-  for (int r0 = 0;;) {                                     // the same trip count in every group
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * step + first;
-      const Row y = transformed<LPR, VEC>(ln.row(raw[u]), k, g.t, ln.j0, inv_d);
-      if (on && r < heads) ln.store(dst + (long long)r * sd.yh, y);
-    }
-    r0 += U * step;
-    if (r0 >= heads) break;
-#pragma unroll
-    for (int u = 0; u < U; ++u) ln.load(src + (long long)min(r0 + u * step + first, heads - 1) * sd.xh, raw[u]);
-  }
-}
-
-template <typename T, int LPR, bool INTER, bool VEC>
-__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && VEC ? 5 : 4) qk_backward_kernel(const __grid_constant__ QkArgs g) {
-  constexpr int GROUPS = THREADS / LPR, U = VEC ? 2 : 1;
-  __shared__ float2 table[GROUPS * LPR * S];
-  __shared__ float sums[THREADS * 2 * S];
-  asm volatile("griddepcontrol.launch_dependents;");       // the sum of the partial rows may be brought in; it waits for this
-  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const bool keys = blockIdx.x >= g.q_ctas;
-  const Side& sd = g.side[keys];
-  const Lane<T, INTER, VEC> ln(lane, g.d, g.t.pairs);
-  const int per_cta = GROUPS / sd.per_token, first = group % sd.per_token, mine = group / sd.per_token;
-  const int step = sd.per_token, heads = sd.heads, pairs = g.t.pairs;
-  const int cta = (int)(blockIdx.x - (keys ? g.q_ctas : 0)), ctas = (int)(keys ? gridDim.x - g.q_ctas : g.q_ctas);
-  const float inv_d = 1.f / (float)g.d;
-  Row acc, gain;                                           // the gain's gradient; the gain
-#pragma unroll
-  for (int e = 0; e < S / 2; ++e) acc.a[e] = acc.b[e] = 0;
-  if (g.t.normalize) gain = ln.gain(sd.gain);
-  Raw<T, VEC> rx[U], rg[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    ln.clear(rx[u]);
-    ln.clear(rg[u]);
-  }
-  for (int t0 = cta * per_cta; t0 < g.tokens; t0 += ctas * per_cta) {
-    const int tok = t0 + mine;
-    const bool on = tok < g.tokens;
-    const int tc = min(tok, g.tokens - 1), ib = tc / g.seq, is = tc % g.seq;
+  for (int u = 0; u < U; ++u) ln.clear(raw[u]);
+  int first = part;
+  bool filled = false;
+  for (int w = 0; w < 2; ++w) {                            // queries, then keys; the next group begins where the last ended
+    const Side& sd = g.side[w];
+    const int heads = sd.heads;
+    if (heads == 0) continue;
     const T* src = reinterpret_cast<const T*>(sd.x) + ib * sd.xb + is * sd.xt;
-    const T* up = reinterpret_cast<const T*>(sd.up) + ib * sd.ub + is * sd.ut;
     T* dst = reinterpret_cast<T*>(sd.y) + ib * sd.yb + is * sd.yt;
     auto load = [&](int r0) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = min(r0 + u * step + first, heads - 1);
-        if (g.t.normalize) ln.load(src + (long long)r * sd.xh, rx[u]);
-        ln.load(up + (long long)r * sd.uh, rg[u]);
-      }
+      for (int u = 0; u < U; ++u) ln.load(src + (long long)min(r0 + u * step + first, heads - 1) * sd.xh, raw[u]);
     };
     load(0);
-    __syncthreads();                                       // the table's last readers are done
-    fill_table(g, table, t0, per_cta);
-    __syncthreads();
-    Angle angle = angle_from(table + mine * pairs, ln.j0, on ? pairs : 0);
-#pragma unroll
-    for (int e = 0; e < S / 2; ++e) angle.s[e] = neg2(angle.s[e]);           // the gradient turns back
-    for (int r0 = 0;;) {
+    const Row<S> gain = ln.gain(sd.gain);
+    if (!filled) {                                         // under the first loads
+      fill_table<THREADS>(g.t, table, per_cta, [&](int i) {    // once for all heads
+        const int x = min(t0 + i, g.tokens - 1);
+        return place_of(g.pos, g.axes, g.tokens, x, x % g.seq);
+      });
+      __syncthreads();
+      filled = true;
+    }
+    const Coef<S> k = coef(angle_from<S>(table + mine * g.t.pairs, ln.j0, on ? g.t.pairs : 0), gain);
+    for (int r0 = 0;;) {                                   // the same trip count in every group
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int r = r0 + u * step + first;
-        const bool live = on && r < heads;
-        Row h = turned<VEC>(ln.row(rg[u]), angle, ln.j0, pairs);
-        if (g.t.normalize) {
-          // both sums before the reciprocal root is known:  sum x^2  and  sum h gain x
-          const Row x = ln.row(rx[u]), hx = times(h, x);
-          float sq, hg;
-          group_sum_pair<LPR>(dot(x, x), dot(hx, gain), sq, hg);
-          const float rs = rsqrtf(sq * inv_d + g.t.eps), b = -(hg * inv_d) * rs * rs * rs;
-          const f2 rs2 = pack(rs, rs), back = pack(b, b);
-#pragma unroll
-          for (int e = 0; e < S / 2; ++e) {
-            if (live) {
-              acc.a[e] = fma2(hx.a[e], rs2, acc.a[e]);
-              acc.b[e] = fma2(hx.b[e], rs2, acc.b[e]);
-            }
-            h.a[e] = fma2(h.a[e], mul2(gain.a[e], rs2), mul2(x.a[e], back));
-            h.b[e] = fma2(h.b[e], mul2(gain.b[e], rs2), mul2(x.b[e], back));
-          }
-        }
-        if (live) ln.store(dst + (long long)r * sd.yh, h);
+        const Row<S> y = transformed<S, LPR, VEC>(ln.row(raw[u]), k, g.t, ln.j0, inv_d);
+        if (on && r < heads) ln.store(dst + (long long)r * sd.yh, y);
       }
       r0 += U * step;
       if (r0 >= heads) break;
       load(r0);
     }
+    first = (part - heads) & (step - 1);
+  }
+}
+
+template <typename T, int S, int LPR, bool INTER, bool VEC>
+__global__ void __launch_bounds__(THREADS, 4) qk_backward_kernel(const __grid_constant__ QkArgs g) {
+  constexpr int GROUPS = THREADS / LPR, U = VEC ? 2 : 1;
+  __shared__ float2 table[GROUPS * LPR * S];
+  __shared__ float sums[THREADS * 2 * S];
+  asm volatile("griddepcontrol.launch_dependents;");       // the sum of the partial rows may be brought in; it waits for this
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
+  const Lane<T, S, INTER, VEC> ln(lane, g.d, g.t.pairs);
+  const int step = g.per_token, per_cta = GROUPS / step, part = group % step, mine = group / step, pairs = g.t.pairs;
+  const float inv_d = 1.f / (float)g.d;
+  Row<S> acc[2];                                           // the gains' gradients: queries, keys
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int e = 0; e < S / 2; ++e) acc[w].a[e] = acc[w].b[e] = f2{0.f, 0.f};
+  Raw<T, S, VEC> rx[U], rg[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    ln.clear(rx[u]);
+    ln.clear(rg[u]);
+  }
+  for (int t0 = (int)blockIdx.x * per_cta; t0 < g.tokens; t0 += (int)gridDim.x * per_cta) {
+    const int tok = t0 + mine;
+    const bool on = tok < g.tokens;
+    const int tc = min(tok, g.tokens - 1), ib = tc / g.seq, is = tc % g.seq;
+    int first = part;
+    bool filled = false;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const Side& sd = g.side[w];
+      const int heads = sd.heads;
+      if (heads == 0) continue;
+      const T* src = reinterpret_cast<const T*>(sd.x) + ib * sd.xb + is * sd.xt;
+      const T* up = reinterpret_cast<const T*>(sd.up) + ib * sd.ub + is * sd.ut;
+      T* dst = reinterpret_cast<T*>(sd.y) + ib * sd.yb + is * sd.yt;
+      auto load = [&](int r0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int r = min(r0 + u * step + first, heads - 1);
+          if (g.t.normalize) ln.load(src + (long long)r * sd.xh, rx[u]);
+          ln.load(up + (long long)r * sd.uh, rg[u]);
+        }
+      };
+      load(0);
+      Row<S> gain;
+      if (g.t.normalize) gain = ln.gain(sd.gain);
+      if (!filled) {
+        __syncthreads();                                   // the table's last readers are done
+        fill_table<THREADS>(g.t, table, per_cta, [&](int i) {    // once for all heads
+          const int x = min(t0 + i, g.tokens - 1);
+          return place_of(g.pos, g.axes, g.tokens, x, x % g.seq);
+        });
+        __syncthreads();
+        filled = true;
+      }
+      Angle<S> angle = angle_from<S>(table + mine * pairs, ln.j0, on ? pairs : 0);
+#pragma unroll
+      for (int e = 0; e < S / 2; ++e) angle.s[e] = neg2(angle.s[e]);         // the gradient turns back
+      for (int r0 = 0;;) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * step + first;
+          const bool live = on && r < heads;
+          Row<S> h = turned<S, VEC>(ln.row(rg[u]), angle, ln.j0, pairs);
+          if (g.t.normalize) {
+            // both sums before the reciprocal root is known:  sum x^2  and  sum h gain x
+            const Row<S> x = ln.row(rx[u]), hx = times(h, x);
+            float sq, hg;
+            group_sum_pair<LPR>(dot(x, x), dot(hx, gain), sq, hg);
+            const float rs = rsqrtf(sq * inv_d + g.t.eps), b = -(hg * inv_d) * rs * rs * rs;
+            const f2 rs2 = pack(rs, rs), back = pack(b, b);
+#pragma unroll
+            for (int e = 0; e < S / 2; ++e) {
+              if (live) {
+                acc[w].a[e] = fma2(hx.a[e], rs2, acc[w].a[e]);
+                acc[w].b[e] = fma2(hx.b[e], rs2, acc[w].b[e]);
+              }
+              h.a[e] = fma2(h.a[e], mul2(gain.a[e], rs2), mul2(x.a[e], back));
+              h.b[e] = fma2(h.b[e], mul2(gain.b[e], rs2), mul2(x.b[e], back));
+            }
+          }
+          if (live) ln.store(dst + (long long)r * sd.yh, h);
+        }
+        r0 += U * step;
+        if (r0 >= heads) break;
+        load(r0);
+      }
+      first = (part - heads) & (step - 1);
+    }
   }
   if (!g.partial) return;
-  float* out = g.partial + (long long)blockIdx.x * g.d;
 #pragma unroll
-  for (int e = 0; e < S / 2; ++e) {
-    float x, y;
-    unpack(acc.a[e], x, y);
-    sums[(group * 2 * S + 2 * e) * LPR + lane] = x;
-    sums[(group * 2 * S + 2 * e + 1) * LPR + lane] = y;
-    unpack(acc.b[e], x, y);
-    sums[(group * 2 * S + S + 2 * e) * LPR + lane] = x;
-    sums[(group * 2 * S + S + 2 * e + 1) * LPR + lane] = y;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * S * LPR; i += THREADS) {
-    float sum = 0.f;
+  for (int w = 0; w < 2; ++w) {
+    float* out = g.partial + ((long long)w * gridDim.x + blockIdx.x) * g.d;
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < GROUPS; ++j) sum += sums[j * 2 * S * LPR + i];
-    const Lane<T, INTER, VEC> who(i % LPR, g.d, g.t.pairs);
-    if (who.has(i / LPR % S)) out[who.at(i / LPR)] = sum;
+    for (int e = 0; e < S / 2; ++e) {
+      float x, y;
+      unpack(acc[w].a[e], x, y);
+      sums[(group * 2 * S + 2 * e) * LPR + lane] = x;
+      sums[(group * 2 * S + 2 * e + 1) * LPR + lane] = y;
+      unpack(acc[w].b[e], x, y);
+      sums[(group * 2 * S + S + 2 * e) * LPR + lane] = x;
+      sums[(group * 2 * S + S + 2 * e + 1) * LPR + lane] = y;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * S * LPR; i += THREADS) {
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) sum += sums[j * 2 * S * LPR + i];
+      const Lane<T, S, INTER, VEC> who(i % LPR, g.d, g.t.pairs);
+      if (who.has(i / LPR % S)) out[who.at(i / LPR)] = sum;
+    }
   }
 }
 
 // Adds the CTAs' rows: each of 32 warps every 32nd of the queries' (or keys') rows, then the warps in order.
-__global__ void __launch_bounds__(1024) gain_sum_kernel(const float* __restrict__ partial, int q_parts, int k_parts, int d,
+__global__ void __launch_bounds__(1024) gain_sum_kernel(const float* __restrict__ partial, int parts, int d,
                                                         float* __restrict__ gq, float* __restrict__ gk, int accumulate) {
   __shared__ float sh[32][33];
   asm volatile("griddepcontrol.wait;" ::: "memory");       // the rows are complete and visible
   const bool keys = blockIdx.y;
   const int lane = threadIdx.x & 31, j = blockIdx.x * 32 + lane, y = threadIdx.x >> 5;
-  const int parts = keys ? k_parts : q_parts;
-  if (keys) partial += (long long)q_parts * d;
+  if (keys) partial += (long long)parts * d;
   float x = 0.f;
   if (j < d) {
 #pragma unroll 8
@@ -210,33 +227,38 @@ __global__ void __launch_bounds__(1024) gain_sum_kernel(const float* __restrict_
   out[j] = accumulate ? out[j] + x : x;
 }
 
-constexpr int MAX_PARTS = 2048;
+constexpr int MAX_PARTS = 1024;
 
-template <typename T, int LPR, bool INTER, bool VEC>
+template <typename T, int S, int LPR, bool INTER, bool VEC>
 int launch_one(const QkArgs& g, bool backward, unsigned grid, cudaStream_t stream) {
-  if (backward) qk_backward_kernel<T, LPR, INTER, VEC><<<grid, THREADS, 0, stream>>>(g);
-  else qk_forward_kernel<T, LPR, INTER, VEC><<<grid, THREADS, 0, stream>>>(g);
+  if constexpr (S == 4) {
+    if (backward) qk_backward_kernel<T, S, LPR, INTER, VEC><<<grid, THREADS, 0, stream>>>(g);
+  }
+  if (!backward) qk_forward_kernel<T, S, LPR, INTER, VEC><<<grid, THREADS, 0, stream>>>(g);
   count_launch(false);
   return note_cuda_error(cudaGetLastError(), "query/key norm and rotation launch");
 }
-template <typename T, int LPR>
-int launch_lpr(const QkArgs& g, bool inter, bool vec, bool backward, unsigned grid, cudaStream_t stream) {
-  if (inter) return vec ? launch_one<T, LPR, true, true>(g, backward, grid, stream) : launch_one<T, LPR, true, false>(g, backward, grid, stream);
-  return vec ? launch_one<T, LPR, false, true>(g, backward, grid, stream) : launch_one<T, LPR, false, false>(g, backward, grid, stream);
-}
-template <typename T>
-int launch_type(const QkArgs& g, bool inter, bool vec, bool backward, unsigned grid, cudaStream_t stream) {
-  switch (lanes_per_row(g.d)) {
-    case 4: return launch_lpr<T, 4>(g, inter, vec, backward, grid, stream);
-    case 8: return launch_lpr<T, 8>(g, inter, vec, backward, grid, stream);
-    case 16: return launch_lpr<T, 16>(g, inter, vec, backward, grid, stream);
-    default: return launch_lpr<T, 32>(g, inter, vec, backward, grid, stream);
+template <typename T, int S, bool VEC>
+int launch_lpr(const QkArgs& g, bool inter, int lpr, bool backward, unsigned grid, cudaStream_t stream) {
+  switch (lpr) {
+    case 4: return inter ? launch_one<T, S, 4, true, VEC>(g, backward, grid, stream) : launch_one<T, S, 4, false, VEC>(g, backward, grid, stream);
+    case 8: return inter ? launch_one<T, S, 8, true, VEC>(g, backward, grid, stream) : launch_one<T, S, 8, false, VEC>(g, backward, grid, stream);
+    case 16: return inter ? launch_one<T, S, 16, true, VEC>(g, backward, grid, stream) : launch_one<T, S, 16, false, VEC>(g, backward, grid, stream);
+    default:
+      if constexpr (S == 8) return B200_ERR_LIMIT;         // 16 lanes of 16 elements hold the largest head
+      else return inter ? launch_one<T, S, 32, true, VEC>(g, backward, grid, stream) : launch_one<T, S, 32, false, VEC>(g, backward, grid, stream);
   }
+}
+int launch(const QkArgs& g, int dtype, bool inter, int run, int lpr, bool backward, unsigned grid, cudaStream_t stream) {
+  if (dtype == B200_F32) return run ? launch_lpr<float, 4, true>(g, inter, lpr, backward, grid, stream) : launch_lpr<float, 4, false>(g, inter, lpr, backward, grid, stream);
+  return run == 8 ? launch_lpr<__half, 8, true>(g, inter, lpr, backward, grid, stream)
+         : run == 4 ? launch_lpr<__half, 4, true>(g, inter, lpr, backward, grid, stream)
+                    : launch_lpr<__half, 4, false>(g, inter, lpr, backward, grid, stream);
 }
 
 }  // namespace
 
-size_t qk_norm_rotary_backward_workspace_bytes(int64_t d) { return (size_t)MAX_PARTS * (size_t)d * sizeof(float); }
+size_t qk_norm_rotary_backward_workspace_bytes(int64_t d) { return (size_t)MAX_PARTS * 2 * (size_t)d * sizeof(float); }
 
 // Strides are [batch, token, head] of q, k, the upstream gradients (backward) and the outputs.
 int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t d,
@@ -253,10 +275,17 @@ int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq
   g.seq = (int)seq; g.d = (int)d;
   g.pos = positions;
   const bool inter = op->interleaved != 0;
-  bool vec = d % 8 == 0 && g.t.pairs % 4 == 0;
-  const int lpr = lanes_per_row(d), groups = THREADS / lpr;
-  const int64_t want = (int64_t)ds->sm_count * (2048 / lpr);                 // groups that fill every SM
-  int64_t ctas[2] = {0, 0}, work = 0;
+  // Elements that a lane moves at a time.  Eight of f16 (16 bytes) halve the forward's instructions; the backward, with
+  // twice the rows in registers, would lose half its warps to them (186 us against 130 for 2 x 8192 tokens of 36 heads).
+  int run = 0;
+  for (int n = es == 2 && !backward ? 8 : 4; n >= 4 && !run; n /= 2) {
+    bool ok = d % (2 * n) == 0 && g.t.pairs % n == 0;
+    const int64_t heads[2] = {q_heads, k_heads};
+    for (int i = 0; i < (backward ? 4 : 2); ++i) ok = ok && (heads[i & 1] == 0 || vec_ok(n, es, in[i], in_strides[i][0], in_strides[i][1], in_strides[i][2]));
+    for (int i = 0; i < 2; ++i) ok = ok && (heads[i] == 0 || vec_ok(n, es, out[i], out_strides[i][0], out_strides[i][1], out_strides[i][2]));
+    if (ok) run = n;
+  }
+  const int lpr = lanes_per_row(d, run ? run : 4), groups = THREADS / lpr;
   for (int w = 0; w < 2; ++w) {
     Side& sd = g.side[w];
     sd.x = in[w]; sd.up = in[2 + w]; sd.y = out[w];
@@ -267,32 +296,27 @@ int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq
     sd.xb = xs[0]; sd.xt = xs[1]; sd.xh = (int)xs[2];
     sd.ub = us[0]; sd.ut = us[1]; sd.uh = (int)us[2];
     sd.yb = ys[0]; sd.yt = ys[1]; sd.yh = (int)ys[2];
-    sd.per_token = 1;
-    if (sd.heads == 0 || g.tokens == 0) continue;
-    vec = vec && vec_ok(es, sd.x, sd.xb, sd.xt, sd.xh) && vec_ok(es, sd.y, sd.yb, sd.yt, sd.yh);
-    if (backward) vec = vec && vec_ok(es, sd.up, sd.ub, sd.ut, sd.uh);
-    // Groups that share a token: at most eight heads each, so that CTAs are short and end together, and more while the
-    // groups of all tokens would leave SMs without work.
-    while (sd.per_token < groups && sd.per_token < sd.heads && (sd.heads > 8 * sd.per_token || (int64_t)g.tokens * sd.per_token < want))
-      sd.per_token *= 2;
-    ctas[w] = (g.tokens + groups / sd.per_token - 1) / (groups / sd.per_token);
-    work += ctas[w];
   }
-  // Backward: what is resident at once, shared out by the work; each CTA's sums are a row to add up at the end.
-  const int64_t resident = (int64_t)ds->sm_count * (es == 2 && vec ? 5 : 4), most = resident < MAX_PARTS ? resident : MAX_PARTS;
-  if (backward && work > most) {
-    const int64_t share = ctas[0] * most / work;
-    ctas[0] = ctas[0] ? (share > 0 ? share : 1) : 0;
-    ctas[1] = ctas[1] ? (most - ctas[0] > 0 ? most - ctas[0] : 1) : 0;
+  // Groups that share a token: at most ten heads each, so that CTAs are short and end together, and more while the groups
+  // of all tokens would leave SMs without work.
+  const int rows = (int)(q_heads + k_heads);
+  const int64_t want = (int64_t)ds->sm_count * (2048 / lpr);                 // groups that fill every SM
+  g.per_token = 1;
+  while (g.per_token < groups && g.per_token < rows && (rows > 10 * g.per_token || (int64_t)g.tokens * g.per_token < want)) g.per_token *= 2;
+  if (backward) {
+    // CTAs stay and loop there: as few groups a token as leave each CTA six rounds, so that the last one costs little.
+    const int64_t ctas = (int64_t)ds->sm_count * 4;
+    g.per_token = 1;
+    while (g.per_token < groups && g.per_token < rows && g.tokens * g.per_token < 6 * ctas * groups) g.per_token *= 2;
   }
+  int64_t grid = rows ? (g.tokens + groups / g.per_token - 1) / (groups / g.per_token) : 0;
+  // Backward: what is resident at once; each CTA's sums are two rows to add up at the end.
+  if (backward && grid > (int64_t)ds->sm_count * 4) grid = (int64_t)ds->sm_count * 4;
+  if (backward && grid > MAX_PARTS) grid = MAX_PARTS;
   const bool sums = backward && g.t.normalize && (q_gain_grad || k_gain_grad);
   g.partial = sums ? (float*)workspace : nullptr;
-  g.q_ctas = (unsigned)ctas[0];
-  const int64_t grid = ctas[0] + ctas[1];
-  if (grid > 0x7fffffff) return B200_ERR_LIMIT;
   if (grid) {                                              // an empty batch: sums over nothing follow
-    const int rc2 = dtype == B200_F32 ? launch_type<float>(g, inter, vec, backward, (unsigned)grid, stream)
-                                      : launch_type<__half>(g, inter, vec, backward, (unsigned)grid, stream);
+    const int rc2 = launch(g, dtype, inter, run, lpr, backward, (unsigned)grid, stream);
     if (rc2) return rc2;
   }
   if (!sums) return B200_OK;
@@ -305,7 +329,7 @@ int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  const int rc3 = note_cuda_error(cudaLaunchKernelEx(&cfg, gain_sum_kernel, (const float*)g.partial, (int)ctas[0], (int)ctas[1], (int)d,
+  const int rc3 = note_cuda_error(cudaLaunchKernelEx(&cfg, gain_sum_kernel, (const float*)g.partial, (int)grid, (int)d,
                                                      q_gain_grad, k_gain_grad, accumulate), "gain gradient launch");
   count_launch(false);
   return rc3;
