@@ -136,6 +136,7 @@ int b200_init(int ordinal) {
   if ((rc = attention_setup_device())) return rc;
   if ((rc = attention_bwd_setup_device())) return rc;
   if ((rc = rowwise_setup_device())) return rc;
+  if ((rc = kv_attention_setup_device())) return rc;
   if ((rc = conv_noalloc_setup_device())) return rc;
   d.ready = true;
   return B200_OK;

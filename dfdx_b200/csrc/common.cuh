@@ -118,6 +118,7 @@ int kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* 
                     const void* q, const int64_t qs[2], const void* k, const int64_t ks[2], const void* v, const int64_t vs[2],
                     const int32_t* positions, void* q_out, const int64_t qos[2], cudaStream_t stream);
 int kv_cache_read(int dtype, const b200_kv_cache* cache, int64_t n, const int32_t* pages, void* k_out, void* v_out, cudaStream_t stream);
+int kv_attention_setup_device();
 size_t kv_cache_attention_workspace_bytes(const b200_kv_cache* cache, const b200_kv_batch* batch, int64_t q_heads, int64_t window, int causal);
 int kv_cache_attention(int dtype, const b200_kv_cache* cache, const b200_kv_batch* batch, int64_t q_heads, const void* q,
                        const int64_t qs[2], double alpha, int causal, int64_t window, void* out, const int64_t os[2], float* lse,

@@ -22,7 +22,7 @@
 //                       to f16 for the second product only (2^-12 of each, of random sign).
 //   kv_combine_kernel   joins the ranges of a row, in order.
 // A range is a fixed number of slots, not a share of the sequence, so that ragged lengths give CTAs of equal work.
-#include "kv_common.cuh"
+#include "kv_attention.cuh"
 
 namespace b200 {
 
@@ -30,36 +30,8 @@ namespace {
 
 using namespace kv;
 
-struct AttArgs {
-  Cache cache;
-  Batch batch;
-  int q_heads, group;              // group = q_heads / cache.heads
-  int tiles;                       // row tiles of a (sequence, key head)
-  int splits, range;               // ranges per row tile (at most), slots per range
-  int causal, window;
-  float scale_log2;                // alpha * log2(e)
-  const __half* q;
-  long long qt, qh;
-  __half* out;
-  long long ot, oh;
-  float* lse;                      // tokens x q_heads, or nullptr
-  float* part_o;                   // [cta][row][d] unnormalised outputs
-  float2* part_ml;                 // [cta][row] maximum, sum
-  int* status;
-};
-
 constexpr int WARPS = 4;
-constexpr float LIFT = 14.f;       // log2 of the probability at the running maximum, as the second product sees it
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t half2_of(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -84,73 +56,10 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
     for (int i = 0; i < N; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
   }
 }
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {    // 0xff where the code is NaN: 0x7f but for its sign
-  const uint32_t x = (((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-  return x * 0xffu;
-}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {         // an 8 x 8 matrix of f16, two a lane
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-
-// The slots that row r of a sequence sees: [lo, hi).
-struct View { int lo, hi; };
-__device__ __forceinline__ View view_of(const AttArgs& g, const Seq& q, int r) {
-  const int pos = q.len - q.m + r / g.group;
-  View v;
-  v.hi = g.causal ? max(pos + 1, 0) : q.len;
-  v.lo = g.window ? max(pos + 1 - g.window, 0) : 0;
-  return v;
-}
-
-// What a CTA of either kernel works on: a row tile of R rows of one (sequence, key head), and one of its ranges.
-struct Work {
-  Seq q;
-  int s, head, tile, rows;
-  int lo_tile, hi_tile;            // slots that some row sees
-  int lo_all, hi_all;              // slots that every row sees
-  int ranges, begin, end;          // ranges in use; this one's tiles of 16 slots
-};
-template <int R>
-__device__ __forceinline__ bool work_of(const AttArgs& g, unsigned unit, int x, Work& w) {
-  w.tile = (int)(unit % (unsigned)g.tiles); unit /= (unsigned)g.tiles;
-  w.head = (int)(unit % (unsigned)g.cache.heads);
-  w.s = (int)(unit / (unsigned)g.cache.heads);
-  if (w.s >= g.batch.seqs) return false;
-  w.q = load_seq(g.batch, g.cache, w.s);
-  if (!w.q.ok) {
-    if (threadIdx.x == 0) flag_index(g.status);
-    return false;
-  }
-  w.rows = min(w.q.m * g.group - w.tile * R, R);
-  if (w.rows <= 0) return false;
-  const View first = view_of(g, w.q, w.tile * R), last = view_of(g, w.q, w.tile * R + w.rows - 1);
-  w.lo_tile = first.lo; w.hi_tile = last.hi;
-  w.lo_all = last.lo; w.hi_all = first.hi;
-  const int first_range = w.lo_tile / g.range;
-  w.ranges = w.hi_tile > w.lo_tile ? (w.hi_tile - 1) / g.range - first_range + 1 : 1;
-  if (x >= w.ranges) return false;
-  w.begin = max(w.lo_tile, (first_range + x) * g.range) >> 4;
-  w.end = w.hi_tile > w.lo_tile ? (int)min((long long)w.hi_tile, (first_range + x + 1ll) * g.range) + 15 >> 4 : w.begin;
-  return true;
-}
-
-// NaN values in slots that only some rows of a tile see were taken out of the product; this puts them where they belong.
-// Rare enough to read the codes again: eight output elements of one row, over the tiles at the edges of the rows' views.
-__device__ __noinline__ void nan_fixup(const AttArgs& g, const Work& w, int row, int j, float (&v)[8]) {
-  const View view = view_of(g, w.q, row);
-  const int* table = g.batch.table + (long long)w.s * g.batch.table_stride;
-  for (int t = w.begin; t < w.end; ++t) {
-    if (t * 16 >= w.lo_all && t * 16 + 16 <= w.hi_all) continue;
-    const int id = table[(t << 4) >> g.cache.page_log2];
-    if (id < 0 || id >= g.cache.pages) continue;
-    for (int slot = max(t * 16, view.lo); slot < min(t * 16 + 16, view.hi); ++slot) {
-      const uint8_t* p = g.cache.v + (((long long)id * g.cache.heads + w.head) * g.cache.page + (slot & (g.cache.page - 1))) * g.cache.d + j;
-      for (int e = 0; e < 8; ++e)
-        if ((p[e] & 0x7f) == 0x7f) v[e] = NAN;
-    }
-  }
 }
 
 // NQ: eights of rows.  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T: the matrix instruction's 16-row
@@ -369,7 +278,7 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 4 : NQ == 2 ? 3 : 2) kv_
         for (int e = 0; e < 8; ++e) v[e] = fmaf(sh_o[x][r][j + e], f, v[e]);
       }
       const int row = w.tile * R + t * 8 + r, tok = w.q.first + row / g.group, qh = w.head * g.group + row % g.group;
-      if (sh_nan) nan_fixup(g, w, row, j, v);
+      if (sh_nan) nan_fixup(g, w, 1, row, j, v);
       if (w.ranges == 1) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;    // a row that sees nothing: 0, and -inf below
         uint4 pk;
@@ -437,47 +346,64 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(const AttArgs g) {
 }
 
 struct Plan {
-  int nq, tiles, splits, range;
-  long long units, ctas;           // row tiles; row tiles * splits
-  size_t part_floats() const { return splits == 1 ? 0 : (size_t)ctas * 8 * nq; }     // times d + 2
+  bool few, many;                  // which kernels the batch may need
+  int nq;                          // few rows: eights of rows of a tile
+  AttArgs f, m;                    // their tiles, splits, ranges and row limits
+  long long f_units, m_units;      // row tiles
+  long long f_ctas() const { return f_units * f.splits; }
+  long long m_ctas() const { return m_units * m.splits; }
+  // partial results: rows of d + 2 floats
+  size_t f_rows() const { return few && f.splits > 1 ? (size_t)f_ctas() * 8 * nq : 0; }
+  size_t m_rows() const { return many && m.splits > 1 ? (size_t)m_ctas() * TC_ROWS : 0; }
 };
+
+// Sequences with up to this many rows go to the kernel for few rows.
+constexpr int FEW_ROWS = 32;
 
 // How the rows and slots of a call are cut.  Everything follows from what the host knows: the lengths stay on the device,
 // the page table's width bounds them.
 Plan plan_of(const Cache& c, const Batch& b, int64_t q_heads, int64_t window, int causal, int sms) {
   Plan p;
   const int64_t group = q_heads / c.heads, rows = (int64_t)b.max_new * group;
-  p.nq = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
-  const int64_t tiles = (rows + 8 * p.nq - 1) / (8 * p.nq);
   int64_t bound = (int64_t)b.max_pages << c.page_log2;
   if (window && causal && bound > window + b.max_new) bound = window + b.max_new + 1;
-  p.units = (int64_t)b.seqs * c.heads * tiles;
+  p.many = rows > FEW_ROWS;
+  // sequences without new tokens aside, all have max_new of them when these add up to all tokens
+  p.few = !p.many || (int64_t)b.seqs * b.max_new != b.tokens;
+  const int64_t few_rows = p.many ? FEW_ROWS : rows;
+  p.nq = few_rows <= 8 ? 1 : few_rows <= 16 ? 2 : few_rows <= 24 ? 3 : 4;
+  p.f.tiles = 1;
+  p.f_units = (int64_t)b.seqs * c.heads;
+  p.f.rows_over = 0;
+  p.f.rows_most = FEW_ROWS;
   // One sequence is cut into as many ranges as make one round of CTAs.  Several are cut finer, four rounds if all were as
   // long as the bound: shorter ones leave CTAs that return at once, and the ranges' equal length evens out the others.
   // No range is shorter than 256 slots (64 KB at d = 128), below which a CTA's start and its partial result cost as
   // much as its reading.
-  const int64_t round = (int64_t)sms * (p.nq == 1 ? 4 : p.nq == 2 ? 3 : 2), want = round * (b.seqs == 1 ? 1 : 4);
-  int64_t parts = want / (p.units > 0 ? p.units : 1);
-  if (parts < 1) parts = 1;
-  int64_t range = (bound + parts - 1) / parts;
-  range = (range + 63) / 64 * 64;
-  if (range < 256) range = 256;
-  p.range = (int)(range > (1 << 30) ? (1 << 30) : range);
-  p.splits = (int)((bound + p.range - 1) / p.range) + (window ? 1 : 0);
-  if (p.splits < 1) p.splits = 1;
-  p.tiles = (int)tiles;
-  p.ctas = p.units * p.splits;
+  auto cut = [&](AttArgs& a, int64_t units, int64_t want, int64_t least, int64_t unit) {
+    int64_t parts = want / (units > 0 ? units : 1);
+    if (parts < 1) parts = 1;
+    int64_t range = (bound + parts - 1) / parts;
+    range = (range + unit - 1) / unit * unit;
+    if (range < least) range = least;
+    a.range = (int)(range > (1 << 30) ? (1 << 30) : range);
+    a.splits = (int)((bound + a.range - 1) / a.range) + (window ? 1 : 0);
+    if (a.splits < 1) a.splits = 1;
+  };
+  cut(p.f, p.f_units, (int64_t)sms * (p.nq == 1 ? 4 : p.nq == 2 ? 3 : 2) * (b.seqs == 1 ? 1 : 4), 256, 64);
+  // Many rows: tiles of 256, cut along the slots only while there are fewer of them than SMs.
+  p.m.tiles = (int)((rows + TC_ROWS - 1) / TC_ROWS);
+  p.m_units = (int64_t)b.seqs * c.heads * p.m.tiles;
+  p.m.rows_over = FEW_ROWS;
+  p.m.rows_most = 0x7fffffff;
+  cut(p.m, p.m_units, sms, 1024, 128);
   return p;
 }
 
-template <int D, int NQ>
-int launch_decode(const AttArgs& g, const Plan& p, cudaStream_t stream) {
-  kv_decode_kernel<D, NQ><<<(unsigned)p.ctas, WARPS * 32, 0, stream>>>(g);
-  count_launch(true);
-  int rc = note_cuda_error(cudaGetLastError(), "cache attention launch");
-  if (rc || g.splits == 1) return rc;
+template <int D, int R>
+int combine_one(const AttArgs& g, long long units, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.units * 8 * NQ));
+  cfg.gridDim = dim3((unsigned)(units * R));
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cudaLaunchAttribute early;                               // its launch overlaps the end of the kernel before it
@@ -485,17 +411,42 @@ int launch_decode(const AttArgs& g, const Plan& p, cudaStream_t stream) {
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  rc = note_cuda_error(cudaLaunchKernelEx(&cfg, kv_combine_kernel<D, 8 * NQ>, g), "cache attention join launch");
+  const int rc = note_cuda_error(cudaLaunchKernelEx(&cfg, kv_combine_kernel<D, R>, g), "cache attention join launch");
   count_launch(false);
   return rc;
 }
 template <int D>
-int launch_decode_d(const AttArgs& g, const Plan& p, cudaStream_t stream) {
-  switch (p.nq) {
-    case 1: return launch_decode<D, 1>(g, p, stream);
-    case 2: return launch_decode<D, 2>(g, p, stream);
-    case 3: return launch_decode<D, 3>(g, p, stream);
-    default: return launch_decode<D, 4>(g, p, stream);
+int combine_d(const AttArgs& g, int rows, long long units, cudaStream_t stream) {
+  switch (rows) {
+    case 8: return combine_one<D, 8>(g, units, stream);
+    case 16: return combine_one<D, 16>(g, units, stream);
+    case 24: return combine_one<D, 24>(g, units, stream);
+    case 32: return combine_one<D, 32>(g, units, stream);
+    default: return combine_one<D, TC_ROWS>(g, units, stream);
+  }
+}
+int combine(const AttArgs& g, int rows, long long units, cudaStream_t stream) {
+  switch (g.cache.d) {
+    case 32: return combine_d<32>(g, rows, units, stream);
+    case 64: return combine_d<64>(g, rows, units, stream);
+    case 96: return combine_d<96>(g, rows, units, stream);
+    default: return combine_d<128>(g, rows, units, stream);
+  }
+}
+
+template <int D, int NQ>
+int launch_few(const AttArgs& g, long long ctas, cudaStream_t stream) {
+  kv_decode_kernel<D, NQ><<<(unsigned)ctas, WARPS * 32, 0, stream>>>(g);
+  count_launch(true);
+  return note_cuda_error(cudaGetLastError(), "cache attention launch");
+}
+template <int D>
+int launch_few_d(const AttArgs& g, int nq, long long ctas, cudaStream_t stream) {
+  switch (nq) {
+    case 1: return launch_few<D, 1>(g, ctas, stream);
+    case 2: return launch_few<D, 2>(g, ctas, stream);
+    case 3: return launch_few<D, 3>(g, ctas, stream);
+    default: return launch_few<D, 4>(g, ctas, stream);
   }
 }
 
@@ -508,7 +459,7 @@ size_t kv_cache_attention_workspace_bytes(const b200_kv_cache* cache, const b200
   if (c.pages == 0) b.max_pages = 0;
   const DeviceState* ds = device_state();
   const Plan p = plan_of(c, b, q_heads, window, causal, ds ? ds->sm_count : 148);
-  return p.part_floats() * (c.d + 2) * sizeof(float);
+  return (p.f_rows() + p.m_rows()) * (c.d + 2) * sizeof(float);
 }
 
 int kv_cache_attention(int dtype, const b200_kv_cache* cache, const b200_kv_batch* batch, int64_t q_heads, const void* q,
@@ -530,26 +481,46 @@ int kv_cache_attention(int dtype, const b200_kv_cache* cache, const b200_kv_batc
   if (((uintptr_t)q | (uintptr_t)out) & 15) return B200_ERR_UNSUPPORTED;
   if (qs[0] % 8 || qs[1] % 8 || os[0] % 8 || os[1] % 8) return B200_ERR_UNSUPPORTED;
   const Plan p = plan_of(g.cache, g.batch, q_heads, window, causal, ds->sm_count);
-  if (p.ctas > 0x7fffffff || p.units * 8 * p.nq > 0x7fffffff) return B200_ERR_LIMIT;
-  const size_t need = p.part_floats() * (g.cache.d + 2) * sizeof(float);
+  if ((int64_t)g.batch.max_new * (q_heads / g.cache.heads) > 0x3fffffff || p.f_ctas() * 8 * p.nq > 0x7fffffff || p.m_ctas() > 0x7fffffff ||
+      p.m_units * TC_ROWS > 0x7fffffff)
+    return B200_ERR_LIMIT;
+  const size_t need = (p.f_rows() + p.m_rows()) * (g.cache.d + 2) * sizeof(float);
   if (need && (!workspace || ((uintptr_t)workspace & 15))) return B200_ERR_NULL;
   if (workspace_bytes < need) return B200_ERR_WORKSPACE;
   g.q_heads = (int)q_heads; g.group = (int)(q_heads / g.cache.heads);
-  g.tiles = p.tiles; g.splits = p.splits; g.range = p.range;
   g.causal = causal != 0; g.window = (int)window;
   g.scale_log2 = (float)(alpha * 1.4426950408889634);
   g.q = (const __half*)q; g.qt = qs[0]; g.qh = qs[1];
   g.out = (__half*)out; g.ot = os[0]; g.oh = os[1];
   g.lse = lse;
-  g.part_o = (float*)workspace;
-  g.part_ml = (float2*)((float*)workspace + p.part_floats() * g.cache.d);
   g.status = ds->status;
-  switch (g.cache.d) {
-    case 32: return launch_decode_d<32>(g, p, stream);
-    case 64: return launch_decode_d<64>(g, p, stream);
-    case 96: return launch_decode_d<96>(g, p, stream);
-    default: return launch_decode_d<128>(g, p, stream);
+  auto with = [&](const AttArgs& cut, float* part, size_t rows) {
+    AttArgs a = g;
+    a.tiles = cut.tiles; a.splits = cut.splits; a.range = cut.range;
+    a.rows_over = cut.rows_over; a.rows_most = cut.rows_most;
+    a.part_o = part;
+    a.part_ml = (float2*)(part + rows * g.cache.d);
+    return a;
+  };
+  float* part = (float*)workspace;
+  if (p.many) {
+    const AttArgs a = with(p.m, part, p.m_rows());
+    if ((rc = launch_attention_tc(a, p.m_ctas(), stream))) return rc;
+    if (a.splits > 1 && (rc = combine(a, TC_ROWS, p.m_units, stream))) return rc;
+    part += p.m_rows() * (g.cache.d + 2);
   }
+  if (p.few) {
+    const AttArgs a = with(p.f, part, p.f_rows());
+    switch (g.cache.d) {
+      case 32: rc = launch_few_d<32>(a, p.nq, p.f_ctas(), stream); break;
+      case 64: rc = launch_few_d<64>(a, p.nq, p.f_ctas(), stream); break;
+      case 96: rc = launch_few_d<96>(a, p.nq, p.f_ctas(), stream); break;
+      default: rc = launch_few_d<128>(a, p.nq, p.f_ctas(), stream);
+    }
+    if (rc) return rc;
+    if (a.splits > 1 && (rc = combine(a, 8 * p.nq, p.f_units, stream))) return rc;
+  }
+  return B200_OK;
 }
 
 }  // namespace b200
