@@ -7,9 +7,10 @@
 //                    probabilities and writes these as f16 over the scores' own columns: the second product takes its
 //                    left operand from there.  The outputs stay in tensor memory too; they are read, scaled and
 //                    written back only when a row's maximum moves by more than 1.
-//   warp 8, 9        one thread each issues S = Q K^T and O += P V of its tile.  Two issuers, because the tiles' products
-//                    alternate: while one tile's softmax runs, the tensor core has the other's.
-//   warps 12-15      bring the codes: whole 16-byte pieces of a row from global memory into registers, one tile ahead, to
+//   warp 8, 9        one thread each issues S = Q K^T and O += P V of its tile, half a tile of slots at a time: while the
+//                    softmax has one half, the tensor core multiplies the other's probabilities and puts the next
+//                    scores in their place.  (With whole tiles the softmax waited 2500 of 5500 cycles for the two.)
+//   warps 12-19      bring the codes: whole 16-byte pieces of a row from global memory into registers, one tile ahead, to
 //                    f16 (exact), and into the 128B-swizzled layout that both products read; the blocks' scales beside
 //                    them.  TMA cannot: the pages are scattered and the tensor core has no product of f16 with e4m3.
 // Tensor memory: scores (and probabilities) 2 x 128 columns, outputs 2 x DP.  Shared memory at DP = 128: Q 64 KB, two
@@ -26,7 +27,7 @@ using namespace kv;
 using attn::mbar_wait_warp;
 using attn::warp_arrive;
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 640;
 constexpr int STAGES = 2;
 constexpr int SCALE_SETS = 4;
 
@@ -38,9 +39,9 @@ template <int DP> struct Cfg {
   static constexpr int SMEM_BYTES = OFF_V + STAGES * TILE_BYTES + 1024;
   static constexpr uint32_t TM_S = 0, TM_O = 256;
 };
-// 512 threads x 128 registers at launch: 2 x 128 x 184 + 128 x 40 + 128 x 104 = 65536.
-constexpr int REGS_SOFTMAX = 184, REGS_ISSUE = 40, REGS_CODES = 104;
-static_assert(2 * 128 * REGS_SOFTMAX + 128 * REGS_ISSUE + 128 * REGS_CODES <= THREADS * 128, "setmaxnreg budget exceeds the CTA's launch allocation");
+// 640 threads x 96 registers at launch: 2 x 128 x 136 + 128 x 40 + 256 x 80 = 60416 of 61440.
+constexpr int REGS_LAUNCH = 96, REGS_SOFTMAX = 136, REGS_ISSUE = 40, REGS_CODES = 80;
+static_assert(2 * 128 * REGS_SOFTMAX + 128 * REGS_ISSUE + 256 * REGS_CODES <= THREADS * REGS_LAUNCH, "setmaxnreg budget exceeds the CTA's launch allocation");
 
 // D (tensor memory) (+)= A (tensor memory) * B (shared memory), f16 in, f32 out.
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t blo, uint32_t bhi, uint32_t idesc, uint32_t accumulate) {
@@ -59,8 +60,27 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&v
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two f32 in one register pair: the scores come out of tensor memory in neighbouring registers.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 struct TcArgs2 {
   AttArgs a;
+  uint32_t flip;                   // a negative alpha: the queries' signs are turned instead, so that every scale is positive
   long long wait_limit;
 };
 
@@ -70,7 +90,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
   const AttArgs& g = ga.a;
   extern __shared__ uint8_t smem_dyn[];
   __shared__ __align__(8) uint64_t bar_q[2], bar_k_full[STAGES], bar_k_empty[STAGES], bar_v_full[STAGES], bar_v_empty[STAGES];
-  __shared__ __align__(8) uint64_t bar_s_full[2], bar_p_full[2], bar_o_full[2];
+  __shared__ __align__(8) uint64_t bar_s_full[2][2], bar_p_full[2][2], bar_pv_done[2][2];   // per row tile and half of the slots
   __shared__ float4 scales[SCALE_SETS][8];                 // per 16 slots: key scale * alpha log2(e), log2 and reciprocal of the value scale
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag, sh_nan;
@@ -94,14 +114,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&bar_q[t]), 4);
-      mbar_init(smem_u32(&bar_s_full[t]), 1);
-      mbar_init(smem_u32(&bar_p_full[t]), 4);
-      mbar_init(smem_u32(&bar_o_full[t]), 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(smem_u32(&bar_s_full[t][h]), 1);
+        mbar_init(smem_u32(&bar_p_full[t][h]), 4);
+        mbar_init(smem_u32(&bar_pv_done[t][h]), 1);
+      }
     }
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&bar_k_full[s]), 4);
+      mbar_init(smem_u32(&bar_k_full[s]), 8);
       mbar_init(smem_u32(&bar_k_empty[s]), ntile);
-      mbar_init(smem_u32(&bar_v_full[s]), 4);
+      mbar_init(smem_u32(&bar_v_full[s]), 8);
       mbar_init(smem_u32(&bar_v_empty[s]), ntile);
     }
     abort_flag = 0;
@@ -126,50 +148,67 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
       const uint32_t hi_k = (uint32_t)(dk >> 32), hi_v = (uint32_t)(dv >> 32);
       const uint32_t q_lo = (uint32_t)dk + (uint32_t)(t * C::TILE_BYTES >> 4);
       const uint32_t k_lo = (uint32_t)dk + (uint32_t)(C::OFF_K >> 4), v_lo = (uint32_t)dv + (uint32_t)(C::OFF_V >> 4);
-      const uint32_t idesc_qk = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+      const uint32_t idesc_qk = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
       const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
       const uint32_t tm_s = tmem_base + C::TM_S + t * 128, tm_o = tmem_base + C::TM_O + t * 128;
       const int ksteps = d / 16;
-      bool ok = T == 0 || mbar_wait(smem_u32(&bar_q[t]), 0, abortp, ga.wait_limit);
-      for (int j = 0; ok && j < T; ++j) {
-        const int s = j % STAGES;
-        const uint32_t ph = (uint32_t)(j / STAGES) & 1u;
-        // S(j): K_j is in place, and the probabilities that lie over S have been multiplied (P V of tile j - 1)
-        if (!mbar_wait(smem_u32(&bar_k_full[s]), ph, abortp, ga.wait_limit)) break;
-        if (j > 0 && !mbar_wait(smem_u32(&bar_o_full[t]), (uint32_t)(j - 1) & 1u, abortp, ga.wait_limit)) break;
-        tc_fence_after();
-        const uint32_t klo = k_lo + (uint32_t)(s * (C::TILE_BYTES >> 4));
+      // S, half h of tile j: 64 slots
+      auto qk = [&](int j, int h) {
+        const uint32_t klo = k_lo + (uint32_t)((j % STAGES * C::TILE_BYTES + h * 8192) >> 4);
+        if (ksteps == DP / 16) {
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          if (ks < ksteps) {
+          for (int ks = 0; ks < DP / 16; ++ks) {
             const uint32_t off = (uint32_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
-            umma_lohi<2>(tm_s, q_lo + off, hi_k, klo + off, hi_k, idesc_qk, ks > 0 ? 1u : 0u);
+            umma_lohi<2>(tm_s + h * 64, q_lo + off, hi_k, klo + off, hi_k, idesc_qk, ks > 0 ? 1u : 0u);
+          }
+        } else {
+          for (int ks = 0; ks < ksteps; ++ks) {
+            const uint32_t off = (uint32_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
+            umma_lohi<2>(tm_s + h * 64, q_lo + off, hi_k, klo + off, hi_k, idesc_qk, ks > 0 ? 1u : 0u);
           }
         }
-        umma_commit(smem_u32(&bar_s_full[t]));
-        umma_commit(smem_u32(&bar_k_empty[s]));            // one arrival per tile
-        // O(j) += P(j) V_j
-        if (!mbar_wait(smem_u32(&bar_v_full[s]), ph, abortp, ga.wait_limit)) break;
-        if (!mbar_wait(smem_u32(&bar_p_full[t]), (uint32_t)j & 1u, abortp, ga.wait_limit)) break;
+        umma_commit(smem_u32(&bar_s_full[t][h]));
+        if (h == 1) umma_commit(smem_u32(&bar_k_empty[j % STAGES]));          // one arrival per row tile
+      };
+      bool ok = T > 0 && mbar_wait(smem_u32(&bar_q[t]), 0, abortp, ga.wait_limit) &&
+                mbar_wait(smem_u32(&bar_k_full[0]), 0, abortp, ga.wait_limit);
+      if (ok) {
         tc_fence_after();
+        qk(0, 0);
+        qk(0, 1);
+      }
+      for (int j = 0; ok && j < T; ++j) {
+        const int s = j % STAGES;
+        ok = mbar_wait(smem_u32(&bar_v_full[s]), (uint32_t)(j / STAGES) & 1u, abortp, ga.wait_limit);
         const uint32_t vlo = v_lo + (uint32_t)(s * (C::TILE_BYTES >> 4));
+        for (int h = 0; ok && h < 2; ++h) {
+          // O += P V over the half's slots, 16 per product
+          if (!(ok = mbar_wait(smem_u32(&bar_p_full[t][h]), (uint32_t)j & 1u, abortp, ga.wait_limit))) break;
+          tc_fence_after();
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks)                     // 128 slots, 16 per product
-          umma_ts(tm_o, tm_s + ks * 8, vlo + (uint32_t)(ks * 2048 >> 4), hi_v, idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
-        umma_commit(smem_u32(&bar_o_full[t]));
-        umma_commit(smem_u32(&bar_v_empty[s]));
+          for (int ks = 0; ks < 4; ++ks)
+            umma_ts(tm_o, tm_s + h * 64 + ks * 8, vlo + (uint32_t)((h * 4 + ks) * 2048 >> 4), hi_v, idesc_pv, (j > 0 || h > 0 || ks > 0) ? 1u : 0u);
+          umma_commit(smem_u32(&bar_pv_done[t][h]));
+          if (h == 1) umma_commit(smem_u32(&bar_v_empty[s]));
+          if (j + 1 >= T) continue;
+          // the next scores over the probabilities just multiplied
+          if (h == 0 && !(ok = mbar_wait(smem_u32(&bar_k_full[(j + 1) % STAGES]), (uint32_t)((j + 1) / STAGES) & 1u, abortp, ga.wait_limit))) break;
+          if (!(ok = mbar_wait(smem_u32(&bar_pv_done[t][h]), (uint32_t)j & 1u, abortp, ga.wait_limit))) break;
+          tc_fence_after();
+          qk(j + 1, h);
+        }
       }
     }
     __syncwarp();
-  } else if (wg == 3) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+  } else if (wg >= 3) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ---------------------------------------------------------------- codes to f16 tiles
     const int cw = warp - 12;
     const int* table = g.batch.table + (long long)w.s * g.batch.table_stride;
     const int in_page = g.cache.page - 1, shift = g.cache.page_log2;
-    const int row0 = cw * 8 + (lane >> 2), c4 = lane & 3;  // rows row0 + 32 i; 16-code pieces c4 and c4 + 4 of each
+    const int row0 = cw * 8 + (lane >> 2), c4 = lane & 3;  // rows row0 and row0 + 64; 16-code pieces c4 and c4 + 4 of each
     // pieces that do not exist (d < DP) are zeros, written once
-    for (int r = row0; r < 128; r += 32)
+    for (int r = row0; r < 128; r += 64)
       for (int p = c4; p < DP / 16; p += 4)
         if (p * 16 >= d)
           for (int s = 0; s < 2 * STAGES; ++s) {
@@ -178,11 +217,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
             st_shared_v4_u32(row + (((((uint32_t)p & 3u) * 2 + 1) ^ ((uint32_t)r & 7u)) << 4), 0, 0, 0, 0);
           }
     constexpr int PC = (DP / 16 + 3) / 4;                  // pieces of a row that a lane holds: 1 or 2
-    uint4 kc[4][PC], vc[4][PC];
+    uint4 kc[2][PC], vc[2][PC];
     uint32_t bad_groups = 0;
-    // Page of the 16-slot group that this warp's rows row0 + 32 i lie in, for tile j; -1 where there is none.
+    // Page of the 16-slot group that this warp's rows row0 + 64 i lie in, for tile j; -1 where there is none.
     auto page_of = [&](int j, int i) -> int {
-      const int grp = w.begin + j * 8 + i * 2 + (cw >> 1);
+      const int grp = w.begin + j * 8 + i * 4 + (cw >> 1);
       if (grp >= w.end) return -1;
       const int id = __ldg(table + ((grp << 4) >> shift));
       if (id < 0 || id >= g.cache.pages) {
@@ -191,10 +230,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
       }
       return id;
     };
-    auto load = [&](const uint8_t* codes, int j, uint4 (&to)[4][PC], const int (&id)[4]) {
+    auto load = [&](const uint8_t* codes, int j, uint4 (&to)[2][PC], const int (&id)[2]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int slot = base + j * 128 + row0 + 32 * i;
+      for (int i = 0; i < 2; ++i) {
+        const int slot = base + j * 128 + row0 + 64 * i;
         const uint8_t* row = codes + (((long long)max(id[i], 0) * g.cache.heads + w.head) * g.cache.page + (slot & in_page)) * d;
 #pragma unroll
         for (int p = 0; p < PC; ++p) {
@@ -203,10 +242,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
         }
       }
     };
-    auto store = [&](uint32_t tile, const uint4 (&from)[4][PC]) {
+    auto store = [&](uint32_t tile, const uint4 (&from)[2][PC]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t r = (uint32_t)(row0 + 32 * i);
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t r = (uint32_t)(row0 + 64 * i);
 #pragma unroll
         for (int p = 0; p < PC; ++p) {
           if ((c4 + 4 * p) * 16 >= d) continue;
@@ -217,45 +256,50 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
         }
       }
     };
-    int id[4], idv[4];
+    // Scales of the group that lane i < 2 answers for (of rows row0 + 64 i), for the tile whose pages are `id`.
+    auto scale_of = [&](const int (&id)[2]) -> float4 {
+      float4 sc = make_float4(g.scale_log2, -INFINITY, 1.f, 0.f);             // no such slots: their scores count for nothing
+      const int p = lane == 0 ? id[0] : id[1];
+      if ((cw & 1) == 0 && lane < 2 && p >= 0) {
+        const long long blk = (long long)p * g.cache.heads + w.head;
+        const uint32_t sv = __float_as_uint(__ldg(g.cache.v_scale + blk));
+        sc = make_float4(__ldg(g.cache.k_scale + blk) * g.scale_log2, (float)((int)(sv >> 23) - 127), __uint_as_float((254u << 23) - sv), 0.f);
+      }
+      return sc;
+    };
+    // What a tile needs is asked for a tile ahead, the pages two: their latencies would otherwise add up in every round.
+    int id[2], id2[2];
+    float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (T > 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) id[i] = page_of(0, i);
+      for (int i = 0; i < 2; ++i) id[i] = page_of(0, i);
       load(g.cache.k, 0, kc, id);
       load(g.cache.v, 0, vc, id);
+      sc = scale_of(id);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) id2[i] = page_of(1, i);
     }
-    bool ok = true;
-    for (int j = 0; ok && j < T; ++j) {
+    for (int j = 0; j < T; ++j) {
       const int s = j % STAGES;
       const uint32_t ph = (uint32_t)(j / STAGES) & 1u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) idv[i] = id[i];
+      for (int i = 0; i < 2; ++i) id[i] = id2[i];           // of tile j + 1
       if (!mbar_wait_warp(smem_u32(&bar_k_empty[s]), ph ^ 1u, abortp, ga.wait_limit)) break;
-      // the scales: groups i * 2 + (cw >> 1) of the tile, one lane each in every other warp
-      if ((cw & 1) == 0 && lane < 4) {
-        const int grp = lane * 2 + (cw >> 1);
-        const int p = lane == 0 ? idv[0] : lane == 1 ? idv[1] : lane == 2 ? idv[2] : idv[3];
-        float4 sc = make_float4(g.scale_log2, -INFINITY, 1.f, 0.f);         // no such slots: their scores count for nothing
-        if (p >= 0) {
-          const long long blk = (long long)p * g.cache.heads + w.head;
-          const uint32_t sv = __float_as_uint(g.cache.v_scale[blk]);
-          sc = make_float4(g.cache.k_scale[blk] * g.scale_log2, (float)((int)(sv >> 23) - 127), __uint_as_float((254u << 23) - sv), 0.f);
-        }
-        scales[j % SCALE_SETS][grp] = sc;
-      }
+      if ((cw & 1) == 0 && lane < 2) scales[j % SCALE_SETS][lane * 4 + (cw >> 1)] = sc;
       store(smem_base + C::OFF_K + s * C::TILE_BYTES, kc);
       fence_proxy_async_smem();
       warp_arrive(smem_u32(&bar_k_full[s]), lane);
       if (j + 1 < T) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) id[i] = page_of(j + 1, i);
         load(g.cache.k, j + 1, kc, id);
+        sc = scale_of(id);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) id2[i] = page_of(j + 2, i);
       }
       const int slot0 = base + j * 128;
       if (slot0 < w.lo_all || slot0 + 128 > w.hi_all) {    // NaN values in slots that some rows do not see: see nan_fixup
         uint32_t any = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int p = 0; p < PC; ++p) {
             const uint4 q = vc[i][p];
@@ -273,7 +317,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
     }
     if (bad_groups && lane == 0) flag_index(g.status);
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     // ---------------------------------------------------------------- softmax and output (warpgroups 0, 1)
     const int t = wg;
     if (t < ntile) {
@@ -290,52 +334,50 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
         for (int p = 0; p < DP / 8; ++p) {
           uint4 q = make_uint4(0, 0, 0, 0);
           if (p * 8 < d) q = __ldg(reinterpret_cast<const uint4*>(src) + p);
+          q.x ^= ga.flip; q.y ^= ga.flip; q.z ^= ga.flip; q.w ^= ga.flip;
           st_shared_v4_u32(dst + (uint32_t)(p >> 3) * 16384 + ((((uint32_t)p & 7u) ^ ((uint32_t)r & 7u)) << 4), q.x, q.y, q.z, q.w);
         }
         fence_proxy_async_smem();
         warp_arrive(smem_u32(&bar_q[t]), lane);
       }
       const View view = view_of(g, w.q, row);
-      const bool pos = g.scale_log2 >= 0.f;                // key scales are positive
-      const float gone = pos ? -INFINITY : INFINITY;       // a masked score: scaled it is -inf, probability 0
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int j = 0; j < T; ++j) {
-        if (!mbar_wait_warp(smem_u32(&bar_s_full[t]), (uint32_t)j & 1u, abortp, ga.wait_limit)) { ok = false; break; }
+      for (int jh = 0; jh < 2 * T; ++jh) {
+        const int j = jh >> 1, h = jh & 1;
+        if (!mbar_wait_warp(smem_u32(&bar_s_full[t][h]), (uint32_t)j & 1u, abortp, ga.wait_limit)) { ok = false; break; }
         tc_fence_after();
-        uint32_t xr[128];
+        uint32_t xr[64];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(tm_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&xr[c * 32]));
+        for (int c = 0; c < 2; ++c) tmem_ld_32x32(tm_s + h * 64 + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&xr[c * 32]));
         tmem_wait_ld();
-        const int slot0 = base + j * 128;
-        if (slot0 < w.lo_all || slot0 + 128 > w.hi_all) {
+        const int slot0 = base + jh * 64;
+        if (slot0 < w.lo_all || slot0 + 64 > w.hi_all) {
           const int lo = view.lo - slot0, hi = view.hi - slot0;
 #pragma unroll
-          for (int q = 0; q < 128; ++q)
-            if (q < lo || q >= hi) xr[q] = __float_as_uint(gone);
+          for (int q = 0; q < 64; ++q)
+            if (q < lo || q >= hi) xr[q] = __float_as_uint(-INFINITY);
         }
-        const float4* sc = scales[j % SCALE_SETS];
+        const float4* sc = scales[j % SCALE_SETS] + h * 4;
         float top = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < 8; ++b) {
+        for (int b = 0; b < 4; ++b) {
           float e0 = __uint_as_float(xr[b * 16]), e1 = __uint_as_float(xr[b * 16 + 1]);
 #pragma unroll
           for (int q = 2; q < 16; q += 2) {
-            const float v0 = __uint_as_float(xr[b * 16 + q]), v1 = __uint_as_float(xr[b * 16 + q + 1]);
-            e0 = pos ? fmaxf(e0, v0) : fminf(e0, v0);
-            e1 = pos ? fmaxf(e1, v1) : fminf(e1, v1);
+            e0 = fmaxf(e0, __uint_as_float(xr[b * 16 + q]));
+            e1 = fmaxf(e1, __uint_as_float(xr[b * 16 + q + 1]));
           }
-          const float ext = pos ? fmaxf(e0, e1) : fminf(e0, e1);
           const float2 s2 = *reinterpret_cast<const float2*>(&sc[b]);
-          top = fmaxf(top, fmaf(ext, s2.x, s2.y));
+          top = fmaxf(top, fmaf(fmaxf(e0, e1), s2.x, s2.y));   // the scales are positive: see flip
         }
         if (__any_sync(0xffffffffu, top > m + 1.f)) {      // some row's maximum moves: all rows of the warp take theirs
           const float now = fmaxf(m, top);
           const float f = now == -INFINITY ? 1.f : ex2(m - now);
           m = now;
           l *= f;
-          if (j > 0) {
-            if (!mbar_wait_warp(smem_u32(&bar_o_full[t]), (uint32_t)(j - 1) & 1u, abortp, ga.wait_limit)) { ok = false; break; }
+          if (jh > 0) {                                    // once the half before has been added
+            if (!mbar_wait_warp(smem_u32(&bar_pv_done[t][h ^ 1]), (uint32_t)((jh - 1) >> 1) & 1u, abortp, ga.wait_limit)) { ok = false; break; }
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) {
@@ -346,37 +388,41 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
               for (int q = 0; q < 16; ++q) v[q] = __float_as_uint(__uint_as_float(v[q]) * f);
               tmem_st_32x16(tm_o + c * 16, v);
             }
-            tmem_wait_st();
           }
         }
         const float nm = m == -INFINITY ? 0.f : LIFT - m;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int b2 = 0; b2 < 2; ++b2) {
-            const int b = h * 2 + b2;
+            const int b = c * 2 + b2;
             const float4 s4 = sc[b];
             const float shift = s4.y + nm;
-            float s0 = 0.f, s1 = 0.f;
+            const uint64_t sx = pair(s4.x, s4.x), sh = pair(shift, shift);
+            uint64_t sum = 0;
 #pragma unroll
             for (int q = 0; q < 16; q += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(xr[b * 16 + q]), s4.x, shift));
-              const float p1 = ex2(fmaf(__uint_as_float(xr[b * 16 + q + 1]), s4.x, shift));
-              s0 += p0;
-              s1 += p1;
+              float p0, p1;
+              split(fma_pair(pair(__uint_as_float(xr[b * 16 + q]), __uint_as_float(xr[b * 16 + q + 1])), sx, sh), p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+              sum = add_pair(sum, pair(p0, p1));
               pk[b2 * 8 + q / 2] = half2_of(p0, p1);
             }
+            float s0, s1;
+            split(sum, s0, s1);
             l = fmaf(s0 + s1, s4.z, l);
           }
-          tmem_st_32x16(tm_s + h * 16, pk);
+          tmem_st_32x16(tm_s + h * 64 + c * 16, pk);
         }
         tmem_wait_st();
         tc_fence_before();
-        warp_arrive(smem_u32(&bar_p_full[t]), lane);
+        warp_arrive(smem_u32(&bar_p_full[t][h]), lane);
       }
-      if (ok && T > 0) {
-        ok = mbar_wait_warp(smem_u32(&bar_o_full[t]), (uint32_t)(T - 1) & 1u, abortp, ga.wait_limit);
+      if (ok && T > 0) {                                   // the tile's products complete in the order of their issue
+        ok = mbar_wait_warp(smem_u32(&bar_pv_done[t][0]), (uint32_t)(T - 1) & 1u, abortp, ga.wait_limit) &&
+             mbar_wait_warp(smem_u32(&bar_pv_done[t][1]), (uint32_t)(T - 1) & 1u, abortp, ga.wait_limit);
         tc_fence_after();
       }
       if (ok) {
@@ -435,6 +481,8 @@ namespace kv {
 int launch_attention_tc(const AttArgs& g, long long ctas, cudaStream_t stream) {
   TcArgs2 a;
   a.a = g;
+  a.flip = a.a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  a.a.scale_log2 = fabsf(a.a.scale_log2);
   if (a.a.scale_log2 == 0.f) a.a.scale_log2 = 1e-30f;       // keeps (masked score = -inf) * scale = -inf
   a.wait_limit = 400000000LL + (long long)(g.range / 128) * 400000LL;
   if (g.cache.d <= 64) kv_prefill_kernel<64><<<(unsigned)ctas, THREADS, Cfg<64>::SMEM_BYTES, stream>>>(a);
