@@ -7,9 +7,9 @@
 //                    probabilities and writes these as f16 over the scores' own columns: the second product takes its
 //                    left operand from there.  The outputs stay in tensor memory too; they are read, scaled and
 //                    written back only when a row's maximum moves by more than 1.
-//   warp 8, 9        one thread each issues S = Q K^T and O += P V of its tile, half a tile of slots at a time: while the
-//                    softmax has one half, the tensor core multiplies the other's probabilities and puts the next
-//                    scores in their place.  (With whole tiles the softmax waited 2500 of 5500 cycles for the two.)
+//   warps 8-11       one thread each issues S = Q K^T (8, 9) or O += P V (10, 11) of a tile, half a tile of slots at a time:
+//                    while the softmax has one half, the tensor core multiplies the other's probabilities and puts the
+//                    next scores in their place.  (With whole tiles the softmax waited 2500 of 5500 cycles for the two.)
 //   warps 12-19      bring the codes: whole 16-byte pieces of a row from global memory into registers, one tile ahead, to
 //                    f16 (exact), and into the 128B-swizzled layout that both products read; the blocks' scales beside
 //                    them.  TMA cannot: the pages are scattered and the tensor core has no product of f16 with e4m3.
@@ -141,61 +141,58 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
 
   if (wg == 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    const int t = warp - 8;
+    const int t = warp & 1;
     if (t < ntile && lane == 0) {
-      const uint64_t dk = make_smem_desc(smem_base, 16, 1024, 2);             // K-major tiles (Q, K)
-      const uint64_t dv = make_smem_desc(smem_base, 16384, 1024, 2);          // MN-major tile (V)
-      const uint32_t hi_k = (uint32_t)(dk >> 32), hi_v = (uint32_t)(dv >> 32);
-      const uint32_t q_lo = (uint32_t)dk + (uint32_t)(t * C::TILE_BYTES >> 4);
-      const uint32_t k_lo = (uint32_t)dk + (uint32_t)(C::OFF_K >> 4), v_lo = (uint32_t)dv + (uint32_t)(C::OFF_V >> 4);
-      const uint32_t idesc_qk = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-      const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
       const uint32_t tm_s = tmem_base + C::TM_S + t * 128, tm_o = tmem_base + C::TM_O + t * 128;
-      const int ksteps = d / 16;
-      // S, half h of tile j: 64 slots
-      auto qk = [&](int j, int h) {
-        const uint32_t klo = k_lo + (uint32_t)((j % STAGES * C::TILE_BYTES + h * 8192) >> 4);
-        if (ksteps == DP / 16) {
+      if (warp < 10) {
+        // S = Q K^T, half h of tile j: 64 slots, over the probabilities that were multiplied last
+        const uint64_t dk = make_smem_desc(smem_base, 16, 1024, 2);           // K-major tiles (Q, K)
+        const uint32_t hi_k = (uint32_t)(dk >> 32);
+        const uint32_t q_lo = (uint32_t)dk + (uint32_t)(t * C::TILE_BYTES >> 4), k_lo = (uint32_t)dk + (uint32_t)(C::OFF_K >> 4);
+        const uint32_t idesc = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        const int ksteps = d / 16;
+        bool ok = T > 0 && mbar_wait(smem_u32(&bar_q[t]), 0, abortp, ga.wait_limit);
+        for (int j = 0; ok && j < T; ++j) {
+          if (!mbar_wait(smem_u32(&bar_k_full[j % STAGES]), (uint32_t)(j / STAGES) & 1u, abortp, ga.wait_limit)) break;
+          for (int h = 0; h < 2; ++h) {
+            if (j > 0 && !(ok = mbar_wait(smem_u32(&bar_pv_done[t][h]), (uint32_t)(j - 1) & 1u, abortp, ga.wait_limit))) break;
+            tc_fence_after();
+            const uint32_t klo = k_lo + (uint32_t)((j % STAGES * C::TILE_BYTES + h * 8192) >> 4);
+            if (ksteps == DP / 16) {
 #pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) {
-            const uint32_t off = (uint32_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
-            umma_lohi<2>(tm_s + h * 64, q_lo + off, hi_k, klo + off, hi_k, idesc_qk, ks > 0 ? 1u : 0u);
+              for (int ks = 0; ks < DP / 16; ++ks) {
+                const uint32_t off = (uint32_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
+                umma_lohi<2>(tm_s + h * 64, q_lo + off, hi_k, klo + off, hi_k, idesc, ks > 0 ? 1u : 0u);
+              }
+            } else {
+              for (int ks = 0; ks < ksteps; ++ks) {
+                const uint32_t off = (uint32_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
+                umma_lohi<2>(tm_s + h * 64, q_lo + off, hi_k, klo + off, hi_k, idesc, ks > 0 ? 1u : 0u);
+              }
+            }
+            umma_commit(smem_u32(&bar_s_full[t][h]));
           }
-        } else {
-          for (int ks = 0; ks < ksteps; ++ks) {
-            const uint32_t off = (uint32_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
-            umma_lohi<2>(tm_s + h * 64, q_lo + off, hi_k, klo + off, hi_k, idesc_qk, ks > 0 ? 1u : 0u);
-          }
+          if (ok) umma_commit(smem_u32(&bar_k_empty[j % STAGES]));            // one arrival per row tile
         }
-        umma_commit(smem_u32(&bar_s_full[t][h]));
-        if (h == 1) umma_commit(smem_u32(&bar_k_empty[j % STAGES]));          // one arrival per row tile
-      };
-      bool ok = T > 0 && mbar_wait(smem_u32(&bar_q[t]), 0, abortp, ga.wait_limit) &&
-                mbar_wait(smem_u32(&bar_k_full[0]), 0, abortp, ga.wait_limit);
-      if (ok) {
-        tc_fence_after();
-        qk(0, 0);
-        qk(0, 1);
-      }
-      for (int j = 0; ok && j < T; ++j) {
-        const int s = j % STAGES;
-        ok = mbar_wait(smem_u32(&bar_v_full[s]), (uint32_t)(j / STAGES) & 1u, abortp, ga.wait_limit);
-        const uint32_t vlo = v_lo + (uint32_t)(s * (C::TILE_BYTES >> 4));
-        for (int h = 0; ok && h < 2; ++h) {
-          // O += P V over the half's slots, 16 per product
-          if (!(ok = mbar_wait(smem_u32(&bar_p_full[t][h]), (uint32_t)j & 1u, abortp, ga.wait_limit))) break;
-          tc_fence_after();
+      } else {
+        // O += P V over the half's slots, 16 per product
+        const uint64_t dv = make_smem_desc(smem_base, 16384, 1024, 2);        // MN-major tile (V)
+        const uint32_t hi_v = (uint32_t)(dv >> 32), v_lo = (uint32_t)dv + (uint32_t)(C::OFF_V >> 4);
+        const uint32_t idesc = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        bool ok = true;
+        for (int j = 0; ok && j < T; ++j) {
+          const int s = j % STAGES;
+          if (!mbar_wait(smem_u32(&bar_v_full[s]), (uint32_t)(j / STAGES) & 1u, abortp, ga.wait_limit)) break;
+          const uint32_t vlo = v_lo + (uint32_t)(s * (C::TILE_BYTES >> 4));
+          for (int h = 0; h < 2; ++h) {
+            if (!(ok = mbar_wait(smem_u32(&bar_p_full[t][h]), (uint32_t)j & 1u, abortp, ga.wait_limit))) break;
+            tc_fence_after();
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma_ts(tm_o, tm_s + h * 64 + ks * 8, vlo + (uint32_t)((h * 4 + ks) * 2048 >> 4), hi_v, idesc_pv, (j > 0 || h > 0 || ks > 0) ? 1u : 0u);
-          umma_commit(smem_u32(&bar_pv_done[t][h]));
-          if (h == 1) umma_commit(smem_u32(&bar_v_empty[s]));
-          if (j + 1 >= T) continue;
-          // the next scores over the probabilities just multiplied
-          if (h == 0 && !(ok = mbar_wait(smem_u32(&bar_k_full[(j + 1) % STAGES]), (uint32_t)((j + 1) / STAGES) & 1u, abortp, ga.wait_limit))) break;
-          if (!(ok = mbar_wait(smem_u32(&bar_pv_done[t][h]), (uint32_t)j & 1u, abortp, ga.wait_limit))) break;
-          tc_fence_after();
-          qk(j + 1, h);
+            for (int ks = 0; ks < 4; ++ks)
+              umma_ts(tm_o, tm_s + h * 64 + ks * 8, vlo + (uint32_t)((h * 4 + ks) * 2048 >> 4), hi_v, idesc, (j > 0 || h > 0 || ks > 0) ? 1u : 0u);
+            umma_commit(smem_u32(&bar_pv_done[t][h]));
+          }
+          if (ok) umma_commit(smem_u32(&bar_v_empty[s]));
         }
       }
     }
