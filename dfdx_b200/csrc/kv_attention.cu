@@ -14,10 +14,10 @@
 //   kv_decode_kernel    few rows: bound by reading the codes.  A CTA has one (sequence, key head), up to 8 * NQ of its
 //                       rows (a row is a new token and one of the query heads that share the key head) and a range of
 //                       slots; each of its four warps walks 16 slots at a time on m16n8k16 f16 matrix instructions.
-//                       Codes go from global memory to registers directly: the order of the products' summation index
-//                       and of the output columns is free, and is chosen so that each lane reads whole 16-byte (d = 128)
-//                       pieces of a row, a warp whole 128-byte lines, with no shared memory and no barrier in the loop.
-//                       The next tile's keys load under this tile's softmax, the next values under its scores.
+//                       The order of the products' summation index and of the output columns is free, and is chosen so
+//                       that each lane reads whole 16-byte (d = 128) pieces of a row, a warp whole 128-byte lines, and
+//                       that no lane needs what another has read: codes go from global memory to registers, a tile
+//                       ahead, with no shared memory and no barrier in the loop.
 //                       Scores, maxima, sums and outputs are f32; codes are exact in f16, probabilities are rounded
 //                       to f16 for the second product only (2^-12 of each, of random sign).
 //   kv_combine_kernel   joins the ranges of a row, in order.
@@ -31,31 +31,32 @@ namespace {
 using namespace kv;
 
 constexpr int WARPS = 4;
-
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// N words from an address aligned to 16 bytes (N % 4 == 0), 8 bytes (N % 2 == 0) or 4.  Codes are read once per CTA.
-template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
-  if constexpr (N % 4 == 0) {
+// How SHARE neighbouring lanes share a row of codes, N words each: in pieces of SIZE bytes (16 for N % 4 == 0, 8 for
+// N % 2 == 0, else 4), piece i of all lanes side by side, so that every access covers whole 32-byte sectors.
+template <int N, int SHARE> struct Words {
+  static constexpr int SIZE = N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4, PIECES = N * 4 / SIZE;
+  // the code behind word w's first byte in lane `share`
+  static __device__ __forceinline__ constexpr int code(int w, int share) { return (w * 4 / SIZE * SHARE + share) * SIZE + w * 4 % SIZE; }
+  static __device__ __forceinline__ void load(const uint8_t* row, int share, uint32_t (&w)[N]) {
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + i);
-      w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+    for (int i = 0; i < PIECES; ++i) {
+      const uint8_t* p = row + (i * SHARE + share) * SIZE;
+      if constexpr (SIZE == 16) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+        w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+      } else if constexpr (SIZE == 8) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+        w[2 * i] = x.x; w[2 * i + 1] = x.y;
+      } else {
+        w[i] = __ldg(reinterpret_cast<const uint32_t*>(p));
+      }
     }
-  } else if constexpr (N % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      const uint2 x = __ldg(reinterpret_cast<const uint2*>(p) + i);
-      w[2 * i] = x.x; w[2 * i + 1] = x.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
   }
-}
+};
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {         // an 8 x 8 matrix of f16, two a lane
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -65,10 +66,12 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {         // an 8 x 8
 // NQ: eights of rows.  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T: the matrix instruction's 16-row
 // side then holds slots and head elements, which there are always enough of, and its 8-column side the few rows.
 template <int D, int NQ>
-__global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 4 : NQ == 2 ? 3 : 2) kv_decode_kernel(const __grid_constant__ AttArgs g) {
+__global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 3 : 2) kv_decode_kernel(const __grid_constant__ AttArgs g) {
   constexpr int KS = D / 16;                               // k-steps of S^T; also 16-element tiles of O^T
   constexpr int KW = D / 16;                               // words of a key row that a lane holds (D / 4 codes)
   constexpr int VW = D / 32;                               // words of a value row that a lane holds (D / 8 codes)
+  typedef Words<KW, 4> KeyWords;
+  typedef Words<VW, 8> ValueWords;
   constexpr int R = 8 * NQ;
   constexpr bool Q_REGS = NQ == 1;
   __shared__ __align__(16) float sh_o[WARPS][8][D + 4];
@@ -82,23 +85,45 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 4 : NQ == 2 ? 3 : 2) kv_
   if (!work_of<R>(g, blockIdx.x / (unsigned)g.splits, (int)(blockIdx.x % (unsigned)g.splits), w)) return;
   if (threadIdx.x == 0) sh_nan = 0;
 
-  // the queries as the second operand: lane (gr, c) has row gr's elements c D / 4 + 4 ks .. + 3 at step ks, the same order
-  // of summation in which it reads the keys
+  // the queries as the second operand: lane (gr, c) has four elements of row gr at each step, the same order of summation
+  // in which it reads the keys
   uint2 qf[Q_REGS ? KS : 1];
   auto query_of = [&](int r) -> const __half* {
     const int row = w.tile * R + r;
     return g.q + (long long)(w.q.first + row / g.group) * g.qt + (long long)(w.head * g.group + row % g.group) * g.qh;
   };
   if constexpr (Q_REGS) {
-    const __half* src = query_of(min(gr, w.rows - 1)) + c * (D / 4);
+    const __half* src = query_of(min(gr, w.rows - 1));
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const uint2*>(src + ks * 4);
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const uint2*>(src + KeyWords::code(ks, c));
   } else {
     for (int i = threadIdx.x; i < NQ * KS * 32; i += WARPS * 32) {
       const int l = i & 31, ks = (i >> 5) % KS, nt = (i >> 5) / KS;
-      sh_q[i] = *reinterpret_cast<const uint2*>(query_of(min(nt * 8 + (l >> 2), w.rows - 1)) + (l & 3) * (D / 4) + ks * 4);
+      sh_q[i] = *reinterpret_cast<const uint2*>(query_of(min(nt * 8 + (l >> 2), w.rows - 1)) + KeyWords::code(ks, l & 3));
     }
   }
+  // the pages and scales of a warp's next 32 tiles, one a lane; the first ones while the queries are on their way
+  const int* table = g.batch.table + (long long)w.s * g.batch.table_stride;
+  int id;
+  float ks_l, vs_l;
+  uint32_t bad_tiles;
+  auto pages_from = [&](int i0) {
+    const int mine = i0 + lane * WARPS;
+    bool bad = false;
+    id = 0;
+    ks_l = 0.f;
+    vs_l = 1.f;
+    if (mine < w.end) {
+      id = __ldg(table + ((mine << 4) >> g.cache.page_log2));
+      bad = id < 0 || id >= g.cache.pages;
+      if (bad) id = 0;                                     // its slots count for nothing; the caller learns of it
+      ks_l = __ldg(g.cache.k_scale + (long long)id * g.cache.heads + w.head) * g.scale_log2;
+      vs_l = __ldg(g.cache.v_scale + (long long)id * g.cache.heads + w.head);
+    }
+    bad_tiles = __ballot_sync(0xffffffffu, bad);
+    if (bad_tiles && lane == 0) flag_index(g.status);
+  };
+  pages_from(w.begin + warp);
   __syncthreads();
 
   float o[NQ][KS][4];
@@ -113,41 +138,21 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 4 : NQ == 2 ? 3 : 2) kv_
     l[t][0] = l[t][1] = 0.f;
   }
 
-  const int* table = g.batch.table + (long long)w.s * g.batch.table_stride;
-  const int in_page = g.cache.page - 1, shift = g.cache.page_log2;
+  const int in_page = g.cache.page - 1;
   for (int i0 = w.begin + warp; i0 < w.end; i0 += WARPS * 32) {
-    // the pages and scales of the warp's next 32 tiles, one a lane
-    const int mine = i0 + lane * WARPS;
-    int id = 0;
-    float ks_l = 0.f, vs_l = 1.f;
-    bool bad = false;
-    if (mine < w.end) {
-      id = table[(mine << 4) >> shift];
-      bad = id < 0 || id >= g.cache.pages;
-      if (bad) id = 0;                                     // its slots count for nothing; the caller learns of it
-      ks_l = g.cache.k_scale[(long long)id * g.cache.heads + w.head] * g.scale_log2;
-      vs_l = g.cache.v_scale[(long long)id * g.cache.heads + w.head];
-    }
-    const uint32_t bad_tiles = __ballot_sync(0xffffffffu, bad);
-    if (bad_tiles && lane == 0) flag_index(g.status);
+    if (i0 != w.begin + warp) pages_from(i0);
     const int n = min(32, (w.end - i0 + WARPS - 1) / WARPS);
-    uint32_t kw[2][KW], vw[4][VW];
-    auto base_of = [&](int i) -> long long {               // byte offset of tile i's first row
+    // Two tiles' codes in registers: the next ones load while these are worked on.
+    auto load = [&](int i, uint32_t (&kw)[2][KW], uint32_t (&vw)[4][VW]) {
       const int page = __shfl_sync(0xffffffffu, id, i);
-      return (((long long)page * g.cache.heads + w.head) * g.cache.page + (((i0 + i * WARPS) << 4) & in_page)) * D;
-    };
-    auto load_k = [&](long long at) {
+      const long long at = (((long long)page * g.cache.heads + w.head) * g.cache.page + (((i0 + i * WARPS) << 4) & in_page)) * D;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) load_words<KW>(g.cache.k + at + (h * 8 + gr) * D + c * (D / 4), kw[h]);
-    };
-    auto load_v = [&](long long at) {
+      for (int h = 0; h < 2; ++h) KeyWords::load(g.cache.k + at + (h * 8 + gr) * D, c, kw[h]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) load_words<VW>(g.cache.v + at + (2 * c + (t & 1) + (t >> 1) * 8) * D + gr * (D / 8), vw[t]);
+      for (int t = 0; t < 4; ++t) ValueWords::load(g.cache.v + at + (2 * c + (t & 1) + (t >> 1) * 8) * D, gr, vw[t]);
     };
-    long long at = base_of(0);
-    load_k(at);
-    load_v(at);
-    for (int i = 0; i < n; ++i) {
+    auto step = [&](int i, uint32_t (&kw)[2][KW], uint32_t (&vw)[4][VW], uint32_t (&next_kw)[2][KW], uint32_t (&next_vw)[4][VW]) {
+      if (i + 1 < n) load(i + 1, next_kw, next_vw);
       const int slot0 = (i0 + i * WARPS) << 4;
       const float sk = __shfl_sync(0xffffffffu, ks_l, i);
       const uint32_t sv = __float_as_uint(__shfl_sync(0xffffffffu, vs_l, i));
@@ -166,8 +171,6 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 4 : NQ == 2 ? 3 : 2) kv_
           mma16816(sc[t], a0, a1, a2, a3, b.x, b.y);
         }
       }
-      const long long next = i + 1 < n ? base_of(i + 1) : at;
-      if (i + 1 < n) load_k(next);
 
       // sc: slots gr (0, 1) and gr + 8 (2, 3), rows 2 c (0, 2) and 2 c + 1 (1, 3)
       const bool tile_bad = (bad_tiles >> i) & 1u;
@@ -241,8 +244,12 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 4 : NQ == 2 ? 3 : 2) kv_
 #pragma unroll
           for (int t = 0; t < NQ; ++t) mma16816(o[t][2 * x + b], a0, a1, a2, a3, pb[t][0], pb[t][1]);
         }
-      if (i + 1 < n) load_v(next);
-      at = next;
+    };
+    uint32_t ka[2][KW], va[4][VW], kb[2][KW], vb[4][VW];
+    load(0, ka, va);
+    for (int i = 0; i < n; i += 2) {
+      step(i, ka, va, kb, vb);
+      if (i + 1 < n) step(i + 1, kb, vb, ka, va);
     }
   }
 
@@ -257,10 +264,10 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 4 : NQ == 2 ? 3 : 2) kv_
       for (int x = 4; x < 32; x *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
       const int r = 2 * c + y;
       if (gr == 0) { sh_m[warp][r] = m[t][y]; sh_l[warp][r] = sum; }
-      // tiles' rows gr and gr + 8 are elements 2 j and 2 j + 1 of the lane's run of D / 8
+      // tiles' rows gr and gr + 8 are codes 2 j and 2 j + 1 of the lane's words
 #pragma unroll
       for (int j = 0; j < KS; j += 2)
-        *reinterpret_cast<float4*>(&sh_o[warp][r][gr * (D / 8) + 2 * j]) = make_float4(o[t][j][y], o[t][j][2 + y], o[t][j + 1][y], o[t][j + 1][2 + y]);
+        *reinterpret_cast<float4*>(&sh_o[warp][r][ValueWords::code(j / 2, gr)]) = make_float4(o[t][j][y], o[t][j][2 + y], o[t][j + 1][y], o[t][j + 1][2 + y]);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 8 * (D / 8); i += WARPS * 32) {
@@ -296,48 +303,78 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 4 : NQ == 2 ? 3 : 2) kv_
   }
 }
 
-// One CTA per row: the ranges' partial results, every (128 / (D / 4))-th to one of its parts, these in order.
-template <int D, int R>
-__global__ void __launch_bounds__(128) kv_combine_kernel(const AttArgs g) {
-  constexpr int COLS = D / 4, PARTS = 128 / COLS;          // 4, 5, 8 or 16 ranges at a time
-  __shared__ float sh_top[4];
-  __shared__ float4 sh_v[PARTS][COLS];
-  __shared__ float sh_sum[PARTS];
-  asm volatile("griddepcontrol.wait;" ::: "memory");       // the partial results are complete and visible
-  const unsigned unit = blockIdx.x / R;
-  const int r = (int)(blockIdx.x % R);
-  Work w;
-  if (!work_of<R>(g, unit, 0, w) || r >= w.rows || w.ranges == 1) return;
-  const long long cta0 = (long long)unit * g.splits;
-  float top = -INFINITY;
-  for (int x = threadIdx.x; x < w.ranges; x += 128) top = fmaxf(top, g.part_ml[(cta0 + x) * R + r].x);
-#pragma unroll
-  for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-  if ((threadIdx.x & 31) == 0) sh_top[threadIdx.x >> 5] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(sh_top[0], sh_top[1]), fmaxf(sh_top[2], sh_top[3]));
+// The ranges' partial results of a row, joined in order.  COLS lanes take a row's d elements, four each.  Up to FEW_RANGES
+// ranges: these lanes hold all of a row's at once, several rows a CTA.  More: a CTA has one row, and every PARTS-th range
+// goes to one of its groups of lanes.
+constexpr int FEW_RANGES = 8;
+template <int D, int R, bool FEW>
+__global__ void __launch_bounds__(128) kv_combine_kernel(const AttArgs g, long long rows_all) {
+  constexpr int COLS = D / 4, PARTS = 128 / COLS;          // 4, 5, 8 or 16 groups
   const int part = threadIdx.x / COLS, col = threadIdx.x % COLS;
-  float sum = 0.f;
+  const long long item = FEW ? (long long)blockIdx.x * PARTS + part : blockIdx.x;
+  const unsigned unit = (unsigned)(item / R);
+  const int r = (int)(item % R);
+  Work w;
+  const bool mine = part < PARTS && item < rows_all && work_of<R>(g, unit, 0, w) && r < w.rows && w.ranges > 1;
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // the partial results are complete and visible
+  const long long cta0 = (long long)unit * g.splits;
+  float top = -INFINITY, sum = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (part < PARTS) {
-#pragma unroll 4
-    for (int x = part; x < w.ranges; x += PARTS) {
-      const float2 ml = g.part_ml[(cta0 + x) * R + r];
-      const float4 o = *reinterpret_cast<const float4*>(g.part_o + ((cta0 + x) * R + r) * D + col * 4);
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-      sum = fmaf(ml.y, f, sum);
-      v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
-    }
-    sh_v[part][col] = v;
-    if (col == 0) sh_sum[part] = sum;
-  }
-  __syncthreads();
-  if (part) return;
+  if constexpr (FEW) {
+    if (!mine) return;
+    float2 ml[FEW_RANGES];
+    float4 o[FEW_RANGES];
 #pragma unroll
-  for (int x = 1; x < PARTS; ++x) {
-    const float4 o = sh_v[x][col];
-    sum += sh_sum[x];
-    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+    for (int x = 0; x < FEW_RANGES; ++x) {
+      ml[x] = make_float2(-INFINITY, 0.f);
+      if (x < w.ranges) {
+        ml[x] = g.part_ml[(cta0 + x) * R + r];
+        o[x] = *reinterpret_cast<const float4*>(g.part_o + ((cta0 + x) * R + r) * D + col * 4);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < FEW_RANGES; ++x) top = fmaxf(top, ml[x].x);
+#pragma unroll
+    for (int x = 0; x < FEW_RANGES; ++x) {
+      if (x >= w.ranges) continue;
+      const float f = ml[x].x == -INFINITY ? 0.f : ex2(ml[x].x - top);
+      sum = fmaf(ml[x].y, f, sum);
+      v.x = fmaf(o[x].x, f, v.x); v.y = fmaf(o[x].y, f, v.y); v.z = fmaf(o[x].z, f, v.z); v.w = fmaf(o[x].w, f, v.w);
+    }
+  } else {
+    __shared__ float sh_top[4];
+    __shared__ float4 sh_v[PARTS][COLS];
+    __shared__ float sh_sum[PARTS];
+    const bool any = __syncthreads_or(mine);               // the same in all threads of a row but those behind the groups
+    if (!any) return;
+    if (part < PARTS) {
+      for (int x = threadIdx.x; x < w.ranges; x += PARTS * COLS) top = fmaxf(top, g.part_ml[(cta0 + x) * R + r].x);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    if ((threadIdx.x & 31) == 0) sh_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(sh_top[0], sh_top[1]), fmaxf(sh_top[2], sh_top[3]));
+    if (part < PARTS) {
+#pragma unroll 8
+      for (int x = part; x < w.ranges; x += PARTS) {
+        const float2 ml = g.part_ml[(cta0 + x) * R + r];
+        const float4 o = *reinterpret_cast<const float4*>(g.part_o + ((cta0 + x) * R + r) * D + col * 4);
+        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+        v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
+      }
+      sh_v[part][col] = v;
+      if (col == 0) sh_sum[part] = sum;
+    }
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int x = 1; x < PARTS; ++x) {
+      const float4 o = sh_v[x][col];
+      sum += sh_sum[x];
+      v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+    }
   }
   const int row = w.tile * R + r, tok = w.q.first + row / g.group, qh = w.head * g.group + row % g.group;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -359,6 +396,7 @@ struct Plan {
 
 // Sequences with up to this many rows go to the kernel for few rows.
 constexpr int FEW_ROWS = 32;
+constexpr int ROUNDS = 4;
 
 // How the rows and slots of a call are cut.  Everything follows from what the host knows: the lengths stay on the device,
 // the page table's width bounds them.
@@ -366,7 +404,7 @@ Plan plan_of(const Cache& c, const Batch& b, int64_t q_heads, int64_t window, in
   Plan p;
   const int64_t group = q_heads / c.heads, rows = (int64_t)b.max_new * group;
   int64_t bound = (int64_t)b.max_pages << c.page_log2;
-  if (window && causal && bound > window + b.max_new) bound = window + b.max_new + 1;
+  if (window && causal && bound > window + b.max_new + 16) bound = window + b.max_new + 16;
   p.many = rows > FEW_ROWS;
   // sequences without new tokens aside, all have max_new of them when these add up to all tokens
   p.few = !p.many || (int64_t)b.seqs * b.max_new != b.tokens;
@@ -376,34 +414,40 @@ Plan plan_of(const Cache& c, const Batch& b, int64_t q_heads, int64_t window, in
   p.f_units = (int64_t)b.seqs * c.heads;
   p.f.rows_over = 0;
   p.f.rows_most = FEW_ROWS;
-  // One sequence is cut into as many ranges as make one round of CTAs.  Several are cut finer, four rounds if all were as
-  // long as the bound: shorter ones leave CTAs that return at once, and the ranges' equal length evens out the others.
-  // No range is shorter than 256 slots (64 KB at d = 128), below which a CTA's start and its partial result cost as
-  // much as its reading.
-  auto cut = [&](AttArgs& a, int64_t units, int64_t want, int64_t least, int64_t unit) {
-    int64_t parts = want / (units > 0 ? units : 1);
-    if (parts < 1) parts = 1;
-    int64_t range = (bound + parts - 1) / parts;
-    range = (range + unit - 1) / unit * unit;
+  // Tiles are cut into ranges of slots: into as many as make one round of CTAs, which is the quickest for one sequence and
+  // for short ones, where a CTA's start (about 4 us of latencies) costs more than its reading.  Where one round's ranges
+  // would be longer than 1024 slots and there are several sequences, into ROUNDS rounds if all were as long as the
+  // bound, no shorter than that: shorter sequences leave CTAs that return at once, and the ranges' equal length evens out
+  // the others.
+  auto cut = [&](AttArgs& a, int64_t units, int64_t round, int most_rounds, int64_t least, int64_t unit) {
+    int64_t range = 0;
+    for (int rounds = 1; rounds <= most_rounds; rounds += most_rounds > 1 ? most_rounds - 1 : 1) {
+      int64_t parts = rounds * round / (units > 0 ? units : 1);
+      if (parts < 1) parts = 1;
+      const int64_t r = ((bound + parts - 1) / parts + unit - 1) / unit * unit;
+      if (rounds == 1 || (range > 1024 && b.seqs > 1)) range = rounds == 1 || r > 1024 ? r : 1024;
+    }
     if (range < least) range = least;
     a.range = (int)(range > (1 << 30) ? (1 << 30) : range);
-    a.splits = (int)((bound + a.range - 1) / a.range) + (window ? 1 : 0);
+    a.splits = (int)((bound + a.range - 1) / a.range);
     if (a.splits < 1) a.splits = 1;
   };
-  cut(p.f, p.f_units, (int64_t)sms * (p.nq == 1 ? 4 : p.nq == 2 ? 3 : 2) * (b.seqs == 1 ? 1 : 4), 256, 64);
+  cut(p.f, p.f_units, (int64_t)sms * (p.nq == 1 ? 3 : 2), ROUNDS, 256, 64);
   // Many rows: tiles of 256, cut along the slots only while there are fewer of them than SMs.
   p.m.tiles = (int)((rows + TC_ROWS - 1) / TC_ROWS);
   p.m_units = (int64_t)b.seqs * c.heads * p.m.tiles;
   p.m.rows_over = FEW_ROWS;
   p.m.rows_most = 0x7fffffff;
-  cut(p.m, p.m_units, sms, 1024, 128);
+  cut(p.m, p.m_units, sms, 1, 1024, 128);
   return p;
 }
 
 template <int D, int R>
 int combine_one(const AttArgs& g, long long units, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * R));
+  const bool few = g.splits <= FEW_RANGES;
+  const int per_cta = few ? 128 / (D / 4) : 1;
+  cfg.gridDim = dim3((unsigned)((units * R + per_cta - 1) / per_cta));
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cudaLaunchAttribute early;                               // its launch overlaps the end of the kernel before it
@@ -411,7 +455,8 @@ int combine_one(const AttArgs& g, long long units, cudaStream_t stream) {
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  const int rc = note_cuda_error(cudaLaunchKernelEx(&cfg, kv_combine_kernel<D, R>, g), "cache attention join launch");
+  const int rc = note_cuda_error(few ? cudaLaunchKernelEx(&cfg, kv_combine_kernel<D, R, true>, g, units * R)
+                                     : cudaLaunchKernelEx(&cfg, kv_combine_kernel<D, R, false>, g, units * R), "cache attention join launch");
   count_launch(false);
   return rc;
 }
@@ -451,6 +496,8 @@ int launch_few_d(const AttArgs& g, int nq, long long ctas, cudaStream_t stream) 
 }
 
 }  // namespace
+
+int kv_attention_setup_device() { return kv::setup_attention_tc(); }
 
 size_t kv_cache_attention_workspace_bytes(const b200_kv_cache* cache, const b200_kv_batch* batch, int64_t q_heads, int64_t window, int causal) {
   Cache c;

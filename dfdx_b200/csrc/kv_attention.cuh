@@ -74,11 +74,13 @@ __device__ __forceinline__ bool work_of(const AttArgs& g, unsigned unit, int x, 
   const View first = view_of(g, w.q, w.tile * R), last = view_of(g, w.q, w.tile * R + w.rows - 1);
   w.lo_tile = first.lo; w.hi_tile = last.hi;
   w.lo_all = last.lo; w.hi_all = first.hi;
-  const int first_range = w.lo_tile / g.range;
-  w.ranges = w.hi_tile > w.lo_tile ? (w.hi_tile - 1) / g.range - first_range + 1 : 1;
+  // ranges are counted from the first slot that some row sees (its group of 16)
+  const int base = w.lo_tile & ~15;
+  w.ranges = w.hi_tile > w.lo_tile ? (w.hi_tile - 1 - base) / g.range + 1 : 1;
   if (x >= w.ranges) return false;
-  w.begin = max(w.lo_tile, (first_range + x) * g.range) >> 4;
-  w.end = w.hi_tile > w.lo_tile ? (int)min((long long)w.hi_tile, (first_range + x + 1ll) * g.range) + 15 >> 4 : w.begin;
+  const long long from = base + (long long)x * g.range, to = from + g.range;
+  w.begin = (int)(from >> 4);
+  w.end = w.hi_tile > w.lo_tile ? ((int)min((long long)w.hi_tile, to) + 15) >> 4 : w.begin;
   return true;
 }
 
@@ -104,6 +106,7 @@ static __device__ __noinline__ void nan_fixup(const AttArgs& g, const Work& w, i
 // kv_attention_tc.cu: the rows of sequences with many.  g.tiles counts tiles of TC_ROWS rows.
 constexpr int TC_ROWS = 256;
 int launch_attention_tc(const AttArgs& g, long long ctas, cudaStream_t stream);
+int setup_attention_tc();
 
 }  // namespace kv
 }  // namespace b200

@@ -488,14 +488,14 @@ int launch_attention_tc(const AttArgs& g, long long ctas, cudaStream_t stream) {
   return note_cuda_error(cudaGetLastError(), "cache attention launch (many rows)");
 }
 
-}  // namespace kv
-
-int kv_attention_setup_device() {
+int setup_attention_tc() {
   int rc = note_cuda_error(cudaFuncSetAttribute(kv_prefill_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<64>::SMEM_BYTES),
                            "cudaFuncSetAttribute(cache attention 64)");
   if (rc) return rc;
   return note_cuda_error(cudaFuncSetAttribute(kv_prefill_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<128>::SMEM_BYTES),
                          "cudaFuncSetAttribute(cache attention 128)");
 }
+
+}  // namespace kv
 
 }  // namespace b200
