@@ -297,21 +297,12 @@ int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq
     sd.ub = us[0]; sd.ut = us[1]; sd.uh = (int)us[2];
     sd.yb = ys[0]; sd.yt = ys[1]; sd.yh = (int)ys[2];
   }
-  // Groups that share a token: at most ten heads each, so that CTAs are short and end together, and more while the groups
-  // of all tokens would leave SMs without work.
   const int rows = (int)(q_heads + k_heads);
-  const int64_t want = (int64_t)ds->sm_count * (2048 / lpr);                 // groups that fill every SM
-  g.per_token = 1;
-  while (g.per_token < groups && g.per_token < rows && (rows > 10 * g.per_token || (int64_t)g.tokens * g.per_token < want)) g.per_token *= 2;
-  if (backward) {
-    // CTAs stay and loop there: as few groups a token as leave each CTA six rounds, so that the last one costs little.
-    const int64_t ctas = (int64_t)ds->sm_count * 4;
-    g.per_token = 1;
-    while (g.per_token < groups && g.per_token < rows && g.tokens * g.per_token < 6 * ctas * groups) g.per_token *= 2;
-  }
+  const int64_t resident = (int64_t)ds->sm_count * (backward ? 4 : 5);
+  g.per_token = groups_per_token(g.tokens, rows, groups, resident, !run ? 1 : run == 8 || backward || es == 4 ? 2 : 4);
   int64_t grid = rows ? (g.tokens + groups / g.per_token - 1) / (groups / g.per_token) : 0;
   // Backward: what is resident at once; each CTA's sums are two rows to add up at the end.
-  if (backward && grid > (int64_t)ds->sm_count * 4) grid = (int64_t)ds->sm_count * 4;
+  if (backward && grid > resident) grid = resident;
   if (backward && grid > MAX_PARTS) grid = MAX_PARTS;
   const bool sums = backward && g.t.normalize && (q_gain_grad || k_gain_grad);
   g.partial = sums ? (float*)workspace : nullptr;
