@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(THREADS, 4) qk_backward_kernel(const __grid_co
   constexpr int GROUPS = THREADS / LPR, U = VEC ? 2 : 1;
   __shared__ float2 table[GROUPS * LPR * S];
   __shared__ float sums[THREADS * 2 * S];
+  __shared__ __align__(16) float gains[2][LPR][2 * S];
   asm volatile("griddepcontrol.launch_dependents;");       // the sum of the partial rows may be brought in; it waits for this
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const Lane<T, S, INTER, VEC> ln(lane, g.d, g.t.pairs);
@@ -104,11 +105,22 @@ __global__ void __launch_bounds__(THREADS, 4) qk_backward_kernel(const __grid_co
   for (int w = 0; w < 2; ++w)
 #pragma unroll
     for (int e = 0; e < S / 2; ++e) acc[w].a[e] = acc[w].b[e] = f2{0.f, 0.f};
-  Raw<T, S, VEC> rx[U], rg[U];
+  // Two sets of rows: the next ones are on their way while these are worked on.
+  Raw<T, S, VEC> ax[U], ag[U], bx[U], bg[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    ln.clear(rx[u]);
-    ln.clear(rg[u]);
+    ln.clear(ax[u]);
+    ln.clear(ag[u]);
+    ln.clear(bx[u]);
+    ln.clear(bg[u]);
+  }
+  for (int i = threadIdx.x; i < 2 * LPR; i += THREADS) {   // the gains in f32, in the lanes' order
+    const Row<S> x = Lane<T, S, INTER, VEC>(i % LPR, g.d, g.t.pairs).gain(g.side[i / LPR].gain);
+#pragma unroll
+    for (int e = 0; e < S / 2; ++e) {
+      *reinterpret_cast<float2*>(&gains[i / LPR][i % LPR][2 * e]) = make_float2(x.a[e].x, x.a[e].y);
+      *reinterpret_cast<float2*>(&gains[i / LPR][i % LPR][S + 2 * e]) = make_float2(x.b[e].x, x.b[e].y);
+    }
   }
   for (int t0 = (int)blockIdx.x * per_cta; t0 < g.tokens; t0 += (int)gridDim.x * per_cta) {
     const int tok = t0 + mine;
@@ -124,7 +136,7 @@ __global__ void __launch_bounds__(THREADS, 4) qk_backward_kernel(const __grid_co
       const T* src = reinterpret_cast<const T*>(sd.x) + ib * sd.xb + is * sd.xt;
       const T* up = reinterpret_cast<const T*>(sd.up) + ib * sd.ub + is * sd.ut;
       T* dst = reinterpret_cast<T*>(sd.y) + ib * sd.yb + is * sd.yt;
-      auto load = [&](int r0) {
+      auto load = [&](int r0, Raw<T, S, VEC>(&rx)[U], Raw<T, S, VEC>(&rg)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int r = min(r0 + u * step + first, heads - 1);
@@ -132,12 +144,10 @@ __global__ void __launch_bounds__(THREADS, 4) qk_backward_kernel(const __grid_co
           ln.load(up + (long long)r * sd.uh, rg[u]);
         }
       };
-      load(0);
-      Row<S> gain;
-      if (g.t.normalize) gain = ln.gain(sd.gain);
+      load(0, ax, ag);
       if (!filled) {
         __syncthreads();                                   // the table's last readers are done
-        fill_table<THREADS>(g.t, table, per_cta, [&](int i) {    // once for all heads
+        fill_table<THREADS>(g.t, table, per_cta, [&](int i) {                 // once for all heads
           const int x = min(t0 + i, g.tokens - 1);
           return place_of(g.pos, g.axes, g.tokens, x, x % g.seq);
         });
@@ -147,7 +157,7 @@ __global__ void __launch_bounds__(THREADS, 4) qk_backward_kernel(const __grid_co
       Angle<S> angle = angle_from<S>(table + mine * pairs, ln.j0, on ? pairs : 0);
 #pragma unroll
       for (int e = 0; e < S / 2; ++e) angle.s[e] = neg2(angle.s[e]);         // the gradient turns back
-      for (int r0 = 0;;) {
+      auto work = [&](int r0, const Raw<T, S, VEC>(&rx)[U], const Raw<T, S, VEC>(&rg)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int r = r0 + u * step + first;
@@ -155,6 +165,13 @@ __global__ void __launch_bounds__(THREADS, 4) qk_backward_kernel(const __grid_co
           Row<S> h = turned<S, VEC>(ln.row(rg[u]), angle, ln.j0, pairs);
           if (g.t.normalize) {
             // both sums before the reciprocal root is known:  sum x^2  and  sum h gain x
+            Row<S> gain;
+#pragma unroll
+            for (int e = 0; e < S / 2; ++e) {
+              const float2 p = *reinterpret_cast<const float2*>(&gains[w][lane][2 * e]), q = *reinterpret_cast<const float2*>(&gains[w][lane][S + 2 * e]);
+              gain.a[e] = pack(p.x, p.y);
+              gain.b[e] = pack(q.x, q.y);
+            }
             const Row<S> x = ln.row(rx[u]), hx = times(h, x);
             float sq, hg;
             group_sum_pair<LPR>(dot(x, x), dot(hx, gain), sq, hg);
@@ -172,9 +189,14 @@ __global__ void __launch_bounds__(THREADS, 4) qk_backward_kernel(const __grid_co
           }
           if (live) ln.store(dst + (long long)r * sd.yh, h);
         }
-        r0 += U * step;
-        if (r0 >= heads) break;
-        load(r0);
+      };
+      const int stride = U * step;
+      for (int r0 = 0; r0 < heads; r0 += 2 * stride) {
+        if (r0 + stride < heads) load(r0 + stride, bx, bg);
+        work(r0, ax, ag);
+        if (r0 + stride >= heads) break;
+        if (r0 + 2 * stride < heads) load(r0 + 2 * stride, ax, ag);
+        work(r0 + stride, bx, bg);
       }
       first = (part - heads) & (step - 1);
     }
