@@ -38,8 +38,8 @@ struct QkArgs {
 constexpr int THREADS = 128;
 
 template <typename T, int S, int LPR, bool INTER, bool VEC>
-__global__ void __launch_bounds__(THREADS, S == 8 ? 5 : sizeof(T) == 2 && VEC ? 6 : 5) qk_forward_kernel(const __grid_constant__ QkArgs g) {
-  constexpr int GROUPS = THREADS / LPR, U = !VEC ? 1 : S * sizeof(T) == 8 ? 4 : 2;   // rows on their way per group
+__global__ void __launch_bounds__(THREADS, 4) qk_forward_kernel(const __grid_constant__ QkArgs g) {
+  constexpr int GROUPS = THREADS / LPR, U = VEC ? 2 : 1;   // rows of a set
   __shared__ float2 table[GROUPS * LPR * S];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const Lane<T, S, INTER, VEC> ln(lane, g.d, g.t.pairs);
@@ -48,9 +48,13 @@ __global__ void __launch_bounds__(THREADS, S == 8 ? 5 : sizeof(T) == 2 && VEC ? 
   const bool on = tok < g.tokens;
   const int tc = min(tok, g.tokens - 1), ib = tc / g.seq, is = tc % g.seq;   // a group without a token works on the last one
   const float inv_d = 1.f / (float)g.d;
-  Raw<T, S, VEC> raw[U];
+  // Two sets of rows: the next ones are on their way while these are worked on.
+  Raw<T, S, VEC> ra[U], rb[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) ln.clear(raw[u]);
+  for (int u = 0; u < U; ++u) {
+    ln.clear(ra[u]);
+    ln.clear(rb[u]);
+  }
   int first = part;
   bool filled = false;
   for (int w = 0; w < 2; ++w) {                            // queries, then keys; the next group begins where the last ended
@@ -59,11 +63,11 @@ __global__ void __launch_bounds__(THREADS, S == 8 ? 5 : sizeof(T) == 2 && VEC ? 
     if (heads == 0) continue;
     const T* src = reinterpret_cast<const T*>(sd.x) + ib * sd.xb + is * sd.xt;
     T* dst = reinterpret_cast<T*>(sd.y) + ib * sd.yb + is * sd.yt;
-    auto load = [&](int r0) {
+    auto load = [&](int r0, Raw<T, S, VEC>(&raw)[U]) {
 #pragma unroll
       for (int u = 0; u < U; ++u) ln.load(src + (long long)min(r0 + u * step + first, heads - 1) * sd.xh, raw[u]);
     };
-    load(0);
+    load(0, ra);
     const Row<S> gain = ln.gain(sd.gain);
     if (!filled) {                                         // under the first loads
       fill_table<THREADS>(g.t, table, per_cta, [&](int i) {    // once for all heads
@@ -74,16 +78,21 @@ __global__ void __launch_bounds__(THREADS, S == 8 ? 5 : sizeof(T) == 2 && VEC ? 
       filled = true;
     }
     const Coef<S> k = coef(angle_from<S>(table + mine * g.t.pairs, ln.j0, on ? g.t.pairs : 0), gain);
-    for (int r0 = 0;;) {                                   // the same trip count in every group
+    auto work = [&](int r0, const Raw<T, S, VEC>(&raw)[U]) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int r = r0 + u * step + first;
         const Row<S> y = transformed<S, LPR, VEC>(ln.row(raw[u]), k, g.t, ln.j0, inv_d);
         if (on && r < heads) ln.store(dst + (long long)r * sd.yh, y);
       }
-      r0 += U * step;
-      if (r0 >= heads) break;
-      load(r0);
+    };
+    const int stride = U * step;
+    for (int r0 = 0; r0 < heads; r0 += 2 * stride) {       // the same trip count in every group
+      if (r0 + stride < heads) load(r0 + stride, rb);
+      work(r0, ra);
+      if (r0 + stride >= heads) break;
+      if (r0 + 2 * stride < heads) load(r0 + 2 * stride, ra);
+      work(r0 + stride, rb);
     }
     first = (part - heads) & (step - 1);
   }
@@ -320,8 +329,8 @@ int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq
     sd.yb = ys[0]; sd.yt = ys[1]; sd.yh = (int)ys[2];
   }
   const int rows = (int)(q_heads + k_heads);
-  const int64_t resident = (int64_t)ds->sm_count * (backward ? 4 : 5);
-  g.per_token = groups_per_token(g.tokens, rows, groups, resident, !run ? 1 : run == 8 || backward || es == 4 ? 2 : 4);
+  const int64_t resident = (int64_t)ds->sm_count * 4;
+  g.per_token = groups_per_token(g.tokens, rows, groups, resident, run ? 2 : 1);
   int64_t grid = rows ? (g.tokens + groups / g.per_token - 1) / (groups / g.per_token) : 0;
   // Backward: what is resident at once; each CTA's sums are two rows to add up at the end.
   if (backward && grid > resident) grid = resident;
