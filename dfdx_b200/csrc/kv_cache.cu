@@ -1,7 +1,8 @@
 // Appending keys and values to the paged 8-bit cache (kv_common.cuh), the norm and rotation of the keys on the way, and
 // the new tokens' queries normed and rotated by the same launch; and reading blocks of the cache back.
 //
-//   kv_append_kernel  one CTA per (sequence, page that its new tokens touch, head, keys or values): it holds all new rows
+//   kv_append_kernel  one CTA per (sequence, page that its new tokens touch, head, keys or values; keys of several heads one
+//                     after another, which share the rows' sines): it holds all new rows
 //                     of the block in registers, takes their largest magnitude, settles the block's scale and writes
 //                     the codes, so that each input is read once and no other CTA ever touches the block.  A block
 //                     whose scale grows under earlier rows has these moved to the new scale, a power-of-two step.
@@ -37,22 +38,31 @@ struct AppendArgs {
   int* status;
 };
 
-// The sequence of a new token, by bisection over cu (the last s with cu[s] <= tok).
-__device__ __forceinline__ int owner_of(const int* cu, int n, int tok) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= tok) lo = mid;
-    else hi = mid - 1;
+// The last sequence s with key(cu[s], s) <= what, key rising with s, and its bounds: a warp looks at 32 at a time, so that up
+// to 31 sequences cost one read's latency (a thread's bisection costs one for every halving).
+template <typename Key>
+__device__ __forceinline__ Seq find_seq(const AppendArgs& g, long long what, Key key, int& s) {
+  const int lane = threadIdx.x & 31, n = g.batch.seqs;
+  int lo = 0, span = n;                                    // among [lo, lo + span)
+  while (span > 31) {
+    const int stride = (span + 31) / 32, at = lo + lane * stride;
+    const bool le = at < lo + span && key(__ldg(g.batch.cu + min(at, n)), at) <= what;
+    const int count = __popc(__ballot_sync(0xffffffffu, le));
+    const int from = lo + max(count - 1, 0) * stride;
+    span = min(stride, lo + span - from);
+    lo = from;
   }
-  return lo;
-}
-// A token's slot in its sequence; -1 for a token of no sequence.
-__device__ __forceinline__ int slot_of(const AppendArgs& g, int tok) {
-  if (tok >= g.batch.tokens) return -1;
-  const int s = g.batch.max_new == 1 && g.batch.tokens == g.batch.seqs ? tok : owner_of(g.batch.cu, g.batch.seqs, tok);
-  const Seq q = load_seq(g.batch, g.cache, s);
-  return q.ok && tok >= q.first && tok < q.first + q.m && q.m <= q.len ? q.len - q.m + (tok - q.first) : -1;
+  const int at = min(lo + lane, n);
+  const int cu = __ldg(g.batch.cu + at), len = __ldg(g.batch.lens + min(at, n - 1));
+  const bool le = lane < span && key(cu, at) <= what;
+  const int pick = max(__popc(__ballot_sync(0xffffffffu, le)) - 1, 0);
+  s = lo + pick;
+  Seq q;
+  q.first = __shfl_sync(0xffffffffu, cu, pick);
+  q.m = __shfl_sync(0xffffffffu, cu, pick + 1) - q.first;
+  q.len = __shfl_sync(0xffffffffu, len, pick);
+  q.ok = fits(g.batch, g.cache, q) && q.m <= q.len;
+  return q;
 }
 
 template <typename T, int LPR, bool INTER, bool VEC, int NT>
@@ -73,7 +83,22 @@ __device__ __forceinline__ void append_queries(const AppendArgs& g, unsigned cta
     ln.clear(raw[u]);
     ln.load(q + (long long)min(u * step + first, heads - 1) * g.qh, raw[u]);
   }
-  if (threadIdx.x < per_cta) slots[threadIdx.x] = slot_of(g, t0 + threadIdx.x);
+  // the tokens' slots in their sequences; -1 for a token of no sequence
+  if (g.batch.max_new == 1 && g.batch.tokens == g.batch.seqs) {
+    if (threadIdx.x < per_cta) {
+      Seq q;
+      q.ok = false;
+      if (t0 + (int)threadIdx.x < g.batch.tokens) q = load_seq(g.batch, g.cache, t0 + threadIdx.x);
+      slots[threadIdx.x] = q.ok && q.m == 1 && q.first == t0 + (int)threadIdx.x && q.len > 0 ? q.len - 1 : -1;
+    }
+  } else {
+    for (int i = threadIdx.x >> 5; i < per_cta; i += NT / 32) {
+      int s;
+      const int at = t0 + i;
+      const Seq q = find_seq(g, at, [](int cu, int) { return (long long)cu; }, s);
+      if ((threadIdx.x & 31) == 0) slots[i] = at < g.batch.tokens && q.ok && at >= q.first && at < q.first + q.m ? q.len - q.m + (at - q.first) : -1;
+    }
+  }
   const Row<4> gain = ln.gain(g.q_gain);
   __syncthreads();
   fill_table<NT>(g.t, table, per_cta, [&](int i) { return place_of(g.pos, g.axes, g.batch.tokens, min(t0 + i, g.batch.tokens - 1), slots[i]); });
@@ -129,6 +154,11 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC 
     append_queries<T, LPR, INTER, VEC, NT>(g, blockIdx.x - g.k_ctas - g.v_ctas, table);
     return;
   }
+  if (blockIdx.x == 0)                                     // sequences that no CTA would come to are reported all the same
+    for (int i = threadIdx.x; i < g.batch.seqs; i += NT) {
+      const Seq q = load_seq(g.batch, g.cache, i);
+      if (!q.ok || q.m > q.len) flag_index(g.status);
+    }
   constexpr int GROUPS = NT / LPR;
   constexpr bool AHEAD = VEC && ROWS * sizeof(T) <= 16;    // registers for the next head's rows beside this one's
   __shared__ float warp_top[2][NT / 32];
@@ -140,21 +170,17 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC 
   const int page = g.cache.page, shift = g.cache.page_log2;
   // unit -> (sequence, which of its touched pages)
   int s, nth;
+  Seq q;
   if (g.batch.max_new == 1) {
     s = unit;
     nth = 0;
+    q = load_seq(g.batch, g.cache, s);
+    q.ok = q.ok && q.m <= q.len;
   } else {
-    int lo = 0, hi = g.batch.seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((long long)(g.batch.cu[mid] >> shift) + 2 * mid <= unit) lo = mid;
-      else hi = mid - 1;
-    }
-    s = lo;
-    nth = unit - ((g.batch.cu[s] >> shift) + 2 * s);
+    q = find_seq(g, unit, [shift](int cu, int i) { return (long long)(cu >> shift) + 2ll * i; }, s);
+    nth = unit - ((q.first >> shift) + 2 * s);
   }
-  const Seq q = load_seq(g.batch, g.cache, s);
-  if (!q.ok || q.m > q.len) {
+  if (!q.ok) {
     if (threadIdx.x == 0) flag_index(g.status);
     return;
   }
@@ -162,11 +188,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC 
   const int start = q.len - q.m, col = (start >> shift) + nth;
   const int slot0 = max(start, col << shift), slot1 = min(q.len, (col + 1) << shift);
   if (slot0 >= slot1) return;                              // behind the sequence's last page
-  const int id = g.batch.table[(long long)s * g.batch.table_stride + col];
-  if (id < 0 || id >= g.cache.pages) {
-    if (threadIdx.x == 0) flag_index(g.status);
-    return;
-  }
+  const int id = __ldg(g.batch.table + (long long)s * g.batch.table_stride + col);
   const int rows = slot1 - slot0, row0 = slot0 & (page - 1), tok0 = q.first + (slot0 - start), pairs = g.t.pairs;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const Lane<T, 4, INTER, VEC> ln(lane, g.cache.d, pairs);
@@ -183,7 +205,11 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC 
   };
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) ln.clear(raw[i]);
-  load(head0);
+  load(head0);                                             // on their way while the page is looked up
+  if (id < 0 || id >= g.cache.pages) {
+    if (threadIdx.x == 0) flag_index(g.status);
+    return;
+  }
   Row<4> gain;
   if (change) {
     gain = ln.gain(g.k_gain);

@@ -30,14 +30,17 @@ struct Seq {
   bool ok;
 };
 
-// A sequence's bounds; what does not fit the buffers is refused here, before any address is formed from it.
+// Whether a sequence's bounds fit the buffers; checked before any address is formed from them.
+__device__ __forceinline__ bool fits(const Batch& b, const Cache& c, const Seq& q) {
+  return q.first >= 0 && q.m >= 0 && q.m <= b.max_new && q.first <= b.tokens - q.m && q.len >= 0 &&
+         q.len <= ((long long)b.max_pages << c.page_log2);
+}
 __device__ __forceinline__ Seq load_seq(const Batch& b, const Cache& c, int s) {
   Seq q;
   q.first = b.cu[s];
   q.m = b.cu[s + 1] - q.first;
   q.len = b.lens[s];
-  q.ok = q.first >= 0 && q.m >= 0 && q.m <= b.max_new && q.first <= b.tokens - q.m && q.len >= 0 &&
-         q.len <= ((long long)b.max_pages << c.page_log2);
+  q.ok = fits(b, c, q);
   return q;
 }
 __device__ __forceinline__ void flag_index(int* status) { atomicExch(status, (int)B200_ERR_INDEX); }
