@@ -150,15 +150,17 @@ __device__ __forceinline__ float top_of(const Lane<T, 4, INTER, VEC>& ln, const 
 template <typename T, int LPR, bool INTER, bool VEC, int NT, int ROWS>
 __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC ? 3 : 2) : 8) kv_append_kernel(const __grid_constant__ AppendArgs g) {
   extern __shared__ float2 table[];                        // cos and sin: new rows of the block (tokens of the CTA) x pairs
-  if (blockIdx.x >= g.k_ctas + g.v_ctas) {
-    append_queries<T, LPR, INTER, VEC, NT>(g, blockIdx.x - g.k_ctas - g.v_ctas, table);
-    return;
-  }
-  if (blockIdx.x == 0)                                     // sequences that no CTA would come to are reported all the same
+  if (blockIdx.x == gridDim.x - 1) {                       // reports every sequence that does not fit, visited below or not
     for (int i = threadIdx.x; i < g.batch.seqs; i += NT) {
       const Seq q = load_seq(g.batch, g.cache, i);
       if (!q.ok || q.m > q.len) flag_index(g.status);
     }
+    return;
+  }
+  if (blockIdx.x >= g.k_ctas + g.v_ctas) {
+    append_queries<T, LPR, INTER, VEC, NT>(g, blockIdx.x - g.k_ctas - g.v_ctas, table);
+    return;
+  }
   constexpr int GROUPS = NT / LPR;
   constexpr bool AHEAD = VEC && ROWS * sizeof(T) <= 16;    // registers for the next head's rows beside this one's
   __shared__ float warp_top[2][NT / 32];
@@ -180,11 +182,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC 
     q = find_seq(g, unit, [shift](int cu, int i) { return (long long)(cu >> shift) + 2ll * i; }, s);
     nth = unit - ((q.first >> shift) + 2 * s);
   }
-  if (!q.ok) {
-    if (threadIdx.x == 0) flag_index(g.status);
-    return;
-  }
-  if (q.m == 0 || nth < 0) return;
+  if (!q.ok || q.m == 0 || nth < 0) return;
   const int start = q.len - q.m, col = (start >> shift) + nth;
   const int slot0 = max(start, col << shift), slot1 = min(q.len, (col + 1) << shift);
   if (slot0 >= slot1) return;                              // behind the sequence's last page
@@ -363,10 +361,10 @@ int kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* 
   const bool one = g.batch.max_new == 1;
   g.per_token = groups_per_token(g.batch.tokens, g.q_heads, groups, (int64_t)ds->sm_count * (one ? 8 : 3), !vec ? 1 : es == 4 ? 2 : 4);
   const int64_t per_cta = groups / g.per_token, q_ctas = g.q_heads ? (g.batch.tokens + per_cta - 1) / per_cta : 0;
-  if (units > 0x7fffffff || k_ctas + v_ctas + q_ctas > 0x7fffffff) return B200_ERR_LIMIT;
+  if (units > 0x7fffffff || k_ctas + v_ctas + q_ctas >= 0x7fffffff) return B200_ERR_LIMIT;
   g.k_ctas = (unsigned)k_ctas;
   g.v_ctas = (unsigned)v_ctas;
-  const unsigned grid = (unsigned)(k_ctas + v_ctas + q_ctas);
+  const unsigned grid = (unsigned)(k_ctas + v_ctas + q_ctas + 1);
   return dtype == B200_F32 ? launch_type<float>(g, lpr, inter, vec, grid, stream) : launch_type<__half>(g, lpr, inter, vec, grid, stream);
 }
 
