@@ -325,6 +325,56 @@ def test_read_gives_codes_times_scales(cuda_dev):
     assert dev.device_status() == 0
 
 
+def test_append_with_positions_of_three_axes(cuda_dev):
+    """Positions given by the caller, and cu_tokens, seq_lens and a page table that are views."""
+    dev = cuda_dev
+    sv = Serving(dev, [20, 7], [13, 7], 16, 2, 64, 42)
+    sv.fill([7, 0])
+    g = sv.g
+    q, k, v = (torch.randn(20, h, 64, generator=g).half().cuda() for h in (4, 2, 2))
+    pos = torch.randint(-9, 5000, (3, 20), generator=g, dtype=torch.int32)
+    f = torch.rand(30, generator=g, dtype=torch.float64)
+    rotary = dfdx_b200.Rotary(f.cuda(), (12, 10, 8), True)
+    cu, lens, table, most = sv.args()
+    wide = torch.full((2, table.shape[1] + 3), -1, dtype=torch.int32, device="cuda")
+    wide[:, 2:2 + table.shape[1]] = table
+    y = dev.kv_cache_append(sv.cache, k, v, torch.cat([cu, cu])[:3], torch.cat([lens, lens])[2:], wide[:, 2:2 + table.shape[1]], most,
+                            q=q, rotary=rotary, positions=pos.cuda())
+    angle = ref.angles(pos, f, (12, 10, 8))
+    size = lambda x: x.abs().amax(-1, keepdim=True) * 1.4143
+    q64, k64 = q.cpu().double(), k.cpu().double()
+    want = ref.transform(q64, None, False, 0.0, angle, True)
+    within(y, want, out_tol(want, F16, 2.0 ** -18 * size(q64)), "q")
+    want = ref.transform(k64, None, False, 0.0, angle, True)
+    scale = sv.cache.k_scale.cpu().double()
+    for s, (a, b, n) in enumerate(((0, 13, 20), (13, 20, 7))):
+        got = sv.rows(s, n)[0][n - (b - a):]
+        blocks = torch.stack([scale[int(sv.table[s, i // 16])] for i in range(n - (b - a), n)])[..., None]
+        tol = torch.maximum(2.0 ** -4 * want[a:b].abs(), 2.0 ** -10 * blocks) * (1 + 2.0 ** -18) + 2.0 ** -18 * size(k64[a:b])
+        within(got, want[a:b], tol, f"codes {s}")
+    assert dev.device_status() == 0
+
+
+def test_append_reports_bounds_that_do_not_fit(cuda_dev):
+    dev = cuda_dev
+    sv = Serving(dev, [10, 10, 10], [2, 2, 2], 16, 1, 32, 43)
+    sv.fill([8, 8, 8])
+    cu, lens, table, most = sv.args()
+    x = torch.randn(6, 1, 32, generator=sv.g).half().cuda()
+    good = torch.full_like(x, 7.0)
+    for bad_cu, bad_lens in (([0, 2, 1, 6], None), ([0, 2, 9, 6], None), ([-1, 2, 4, 6], None), (None, [10, 1, 10]), (None, [10, 17, 10]), (None, [10, -3, 10])):
+        held = [t.view(torch.uint8).clone() for t in sv.cache[:2]]
+        c = torch.tensor(bad_cu, dtype=torch.int32).cuda() if bad_cu else cu
+        n = torch.tensor(bad_lens, dtype=torch.int32).cuda() if bad_lens else lens
+        dev.kv_cache_append(sv.cache, x, x, c, n, table, most, q=x, q_out=good)
+        assert dev.device_status() == _lib.ERR_INDEX
+        if bad_lens:                                                      # the other sequences' pages are written, this one's not
+            page = int(sv.table[1, 0])
+            assert all(torch.equal(a[page], b.view(torch.uint8)[page]) for a, b in zip(held, sv.cache[:2]))
+    dev.kv_cache_append(sv.cache, x, x, cu, lens, table, most)
+    assert dev.device_status() == 0
+
+
 def test_append_infinities_nan_zeros(cuda_dev):
     """An infinity is held as the block's largest code and does not set its scale, NaN stays NaN, zeros get the least scale."""
     dev = cuda_dev
@@ -376,6 +426,11 @@ ATT = [  # page, heads, q_heads, d, past, new, causal, window
     (16, 2, 12, 96, [37], [203], True, 50),
     (32, 3, 6, 32, [0, 64, 5], [129, 64, 40], True, 0),
     (128, 1, 8, 128, [9000], [1], True, 0),
+    (16, 2, 8, 64, [500, 0, 77, 1200], [1, 300, 9, 5], True, 0),         # few and many rows in one batch
+    (64, 1, 8, 128, [9000, 3], [40, 33], True, 0),                       # many rows over ranges that are joined
+    (32, 1, 16, 96, [6000], [60], True, 2500),
+    (128, 2, 32, 64, [3000, 5000], [3, 40], False, 0),
+    (64, 1, 40, 32, [300], [1], True, 0),                                # one token, more heads than a small tile's rows
 ]
 
 
@@ -589,6 +644,49 @@ def test_a_step_of_serving(cuda_dev):
         graph.replay()
         dev.synchronize()
         check_attention(dev, sv, q, out, lse, 0.125)
+    assert dev.device_status() == 0
+
+
+def test_calls_on_two_streams_and_in_two_graphs(cuda_dev):
+    """Calls that run at the same time, and graphs that are replayed in turn, each have their own partial results."""
+    dev = cuda_dev
+    cases = []
+    for seed, (page, heads, hq, d, past, new) in enumerate(((64, 2, 8, 128, [6000], [1]), (16, 2, 8, 64, [700, 4000], [40, 50]), (32, 1, 4, 96, [5000], [3]))):
+        sv = Serving(dev, [a + b for a, b in zip(past, new)], new, page, heads, d, 140 + seed)
+        sv.fill(sv.lens)
+        cases.append((sv, torch.randn(sum(new), hq, d, generator=sv.g).half().cuda(), sv.args()))
+    q, k = torch.randn(4, 200, 6, 64).half().cuda(), torch.randn(4, 200, 2, 64).half().cuda()
+    rotary = dfdx_b200.Rotary(dev.rotary_frequencies((32,)), (32,))
+
+    def run(i):
+        if i == 3:
+            return dev.qk_norm_rotary_backward(q, k, q, k, rotary)
+        sv, x, args = cases[i]
+        return dev.kv_cache_attention(sv.cache, x, *args, 0.1, want_lse=True)
+
+    want = [run(i) for i in range(4)]
+    dev.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = [[] for _ in range(4)]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(4):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
+    graphs, outs = [], []
+    for i in range(4):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(run(i))
+        graphs.append(gr)
+    for i in (0, 1, 2, 3, 3, 2, 1, 0, 2, 0, 3, 1):
+        graphs[i].replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(o, w))
     assert dev.device_status() == 0
 
 
