@@ -158,15 +158,6 @@ def load() -> C.CDLL:
     return lib
 
 
-def by_address(name: str):
-    """An entry point whose structs and stride arrays are passed as addresses, which spares the object around each."""
-    res, args = SIGNATURES[name]
-    fn = load()[name]                                   # a function object of its own: the typed one stays as it is
-    fn.restype = res
-    fn.argtypes = [a if a in (_sz, _vp, _i, _d) else _vp for a in args]
-    return fn
-
-
 def strides(seq):
     return (C.c_size_t * len(seq))(*[int(s) for s in seq])
 

@@ -7,12 +7,16 @@ Each .cu is compiled to an object in `dfdx_b200/lib/obj/` (in parallel), then li
 `dfdx_b200/lib/libdfdx_b200.so` with a statically linked CUDA runtime.  The driver API is not linked:
 the one driver entry point the library needs (tensor-map encoding) is resolved at run time, so the
 library loads on a machine without a GPU driver.
+
+`py_heads.cpp`, the host side of heads.py, becomes the Python module `dfdx_b200/lib/_heads.so` (g++, against torch's headers);
+it calls the library through addresses that it is given and is not linked to it.
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -21,6 +25,7 @@ CSRC = PKG / "csrc"
 LIBDIR = PKG / "lib"
 OBJDIR = LIBDIR / "obj"
 LIB = LIBDIR / "libdfdx_b200.so"
+MODULE = LIBDIR / "_heads.so"
 SOURCES = ["api.cu", "gemm_simt.cu", "gemm_tc.cu", "gemm_tc_pair.cu", "conv2d.cu", "attention.cu", "attention_bwd.cu", "rowwise.cu",
            "rotary.cu", "kv_cache.cu", "kv_attention.cu", "kv_attention_tc.cu"]
 NVCC_FLAGS = [
@@ -56,10 +61,29 @@ def _compile(src: str, force: bool) -> Path:
     return obj
 
 
+def _build_module(force: bool) -> None:
+    src = CSRC / "py_heads.cpp"
+    if not force and MODULE.exists() and MODULE.stat().st_mtime >= max(src.stat().st_mtime, (PKG.parent / "include" / "dfdx_b200.h").stat().st_mtime):
+        return
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    nvcc = Path(_nvcc())
+    cuda = nvcc.resolve().parent.parent / "include" if nvcc.is_absolute() else Path("/usr/local/cuda/include")
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda, Path(sysconfig.get_paths()["include"])]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in include), str(src), "-o", str(MODULE), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}",
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     OBJDIR.mkdir(parents=True, exist_ok=True)
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
+        module = ex.submit(_build_module, force)
         objs = list(ex.map(lambda s: _compile(s, force), SOURCES))
+        module.result()
     if force or not LIB.exists() or any(o.stat().st_mtime > LIB.stat().st_mtime for o in objs):
         cmd = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-cudart", "static",
                "-o", str(LIB), *map(str, objs)]
