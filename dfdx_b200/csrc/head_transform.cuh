@@ -383,14 +383,16 @@ inline int lanes_per_row(int64_t d, int slots) {
 }
 
 // How many of a CTA's groups of lanes share a token, a power of two: fewer compute the sines and addresses for more heads,
-// more leave the last round of CTAs less uneven and a small batch not idle.  The cost of a round is that of a group's
-// rows, taken `ahead` at a time, and of what it does once a token, measured at about four rows.
-inline int groups_per_token(int64_t tokens, int rows, int groups, int64_t resident, int ahead) {
+// more leave the last CTAs less uneven and a small batch not idle.  A CTA costs a group's rows, taken `ahead` at a time,
+// and what it does once a token, measured at about four rows.  CTAs that stay and loop (`looping`) all take the most
+// rounds that one of them has; others follow one another, and half a CTA's time goes by at the end.
+inline int groups_per_token(int64_t tokens, int rows, int groups, int64_t resident, int ahead, bool looping) {
   int best = 1;
   int64_t least = 0;
   for (int p = 1; p <= groups; p *= 2) {
-    const int64_t ctas = (tokens + groups / p - 1) / (groups / p), rounds = (ctas + resident - 1) / resident;
-    const int64_t cost = rounds * (4 + (rows + p * ahead - 1) / (p * ahead) * ahead);
+    const int64_t ctas = (tokens + groups / p - 1) / (groups / p);
+    const int64_t each = 4 + (rows + p * ahead - 1) / (p * ahead) * ahead;
+    const int64_t cost = (looping || ctas <= resident ? (ctas + resident - 1) / resident * resident : ctas + resident / 2) * each;
     if (p == 1 || cost < least) {
       best = p;
       least = cost;

@@ -359,7 +359,7 @@ int kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* 
   while (g.key_heads < g.cache.heads && units * ((g.cache.heads + 2 * g.key_heads - 1) / (2 * g.key_heads)) >= 2 * ds->sm_count) g.key_heads *= 2;
   const int64_t k_ctas = units * ((g.cache.heads + g.key_heads - 1) / g.key_heads), v_ctas = units * g.cache.heads;
   const bool one = g.batch.max_new == 1;
-  g.per_token = groups_per_token(g.batch.tokens, g.q_heads, groups, (int64_t)ds->sm_count * (one ? 8 : 3), !vec ? 1 : es == 4 ? 2 : 4);
+  g.per_token = groups_per_token(g.batch.tokens, g.q_heads, groups, (int64_t)ds->sm_count * (one ? 8 : 3), !vec ? 1 : es == 4 ? 2 : 4, false);
   const int64_t per_cta = groups / g.per_token, q_ctas = g.q_heads ? (g.batch.tokens + per_cta - 1) / per_cta : 0;
   if (units > 0x7fffffff || k_ctas + v_ctas + q_ctas >= 0x7fffffff) return B200_ERR_LIMIT;
   g.k_ctas = (unsigned)k_ctas;

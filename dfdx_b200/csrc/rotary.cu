@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(THREADS, 4) qk_forward_kernel(const __grid_con
 }
 
 template <typename T, int S, int LPR, bool INTER, bool VEC>
-__global__ void __launch_bounds__(THREADS, 4) qk_backward_kernel(const __grid_constant__ QkArgs g) {
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) qk_backward_kernel(const __grid_constant__ QkArgs g) {
   constexpr int GROUPS = THREADS / LPR, U = VEC ? 2 : 1;
   __shared__ float2 table[GROUPS * LPR * S];
   __shared__ float sums[THREADS * 2 * S];
@@ -329,8 +329,8 @@ int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq
     sd.yb = ys[0]; sd.yt = ys[1]; sd.yh = (int)ys[2];
   }
   const int rows = (int)(q_heads + k_heads);
-  const int64_t resident = (int64_t)ds->sm_count * 4;
-  g.per_token = groups_per_token(g.tokens, rows, groups, resident, run ? 2 : 1);
+  const int64_t resident = (int64_t)ds->sm_count * (backward && es == 4 ? 3 : 4);
+  g.per_token = groups_per_token(g.tokens, rows, groups, resident, run ? 2 : 1, backward);
   int64_t grid = rows ? (g.tokens + groups / g.per_token - 1) / (groups / g.per_token) : 0;
   // Backward: what is resident at once; each CTA's sums are two rows to add up at the end.
   if (backward && grid > resident) grid = resident;
