@@ -623,6 +623,8 @@ static int qk_norm_rotary_call(int dtype, const b200_head_op* op, size_t batch, 
   if (q_gain_grad || k_gain_grad) {
     if (!workspace || ((uintptr_t)workspace & 15)) return B200_ERR_NULL;
     if (workspace_bytes < qk_norm_rotary_backward_workspace_bytes((int64_t)d)) return B200_ERR_WORKSPACE;
+    // the two are written by different CTAs
+    if (q_gain_grad && k_gain_grad && q_gain_grad < k_gain_grad + d && k_gain_grad < q_gain_grad + d) return B200_ERR_STRIDE;
   }
   return qk_norm_rotary(dtype, op, (int64_t)batch, (int64_t)tokens, (int64_t)q_heads, (int64_t)k_heads, (int64_t)d, in, is, positions,
                         out, os, backward, q_gain_grad, k_gain_grad, accumulate, workspace, (cudaStream_t)stream);

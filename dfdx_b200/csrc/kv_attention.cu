@@ -404,9 +404,11 @@ Plan plan_of(const Cache& c, const Batch& b, int64_t q_heads, int64_t window, in
   Plan p;
   const int64_t group = q_heads / c.heads, rows = (int64_t)b.max_new * group;
   int64_t bound = (int64_t)b.max_pages << c.page_log2;
+  if (bound > MAX_SLOTS) bound = MAX_SLOTS;
   if (window && causal && bound > window + b.max_new + 16) bound = window + b.max_new + 16;
   p.many = rows > FEW_ROWS;
-  // sequences without new tokens aside, all have max_new of them when these add up to all tokens
+  // One launch does where every sequence may be as long as max_new: the kernel for many rows then takes the shorter ones
+  // of a padded batch too.
   p.few = !p.many || (int64_t)b.seqs * b.max_new != b.tokens;
   const int64_t few_rows = p.many ? FEW_ROWS : rows;
   p.nq = few_rows <= 8 ? 1 : few_rows <= 16 ? 2 : few_rows <= 24 ? 3 : 4;
@@ -436,7 +438,7 @@ Plan plan_of(const Cache& c, const Batch& b, int64_t q_heads, int64_t window, in
   // Many rows: tiles of 256, cut along the slots only while there are fewer of them than SMs.
   p.m.tiles = (int)((rows + TC_ROWS - 1) / TC_ROWS);
   p.m_units = (int64_t)b.seqs * c.heads * p.m.tiles;
-  p.m.rows_over = FEW_ROWS;
+  p.m.rows_over = p.few ? FEW_ROWS : 0;
   p.m.rows_most = 0x7fffffff;
   cut(p.m, p.m_units, sms, 1, 1024, 128);
   return p;

@@ -83,24 +83,30 @@ __device__ __forceinline__ void append_queries(const AppendArgs& g, unsigned cta
     ln.clear(raw[u]);
     ln.load(q + (long long)min(u * step + first, heads - 1) * g.qh, raw[u]);
   }
-  // the tokens' slots in their sequences; -1 for a token of no sequence
-  if (g.batch.max_new == 1 && g.batch.tokens == g.batch.seqs) {
-    if (threadIdx.x < per_cta) {
-      Seq q;
-      q.ok = false;
-      if (t0 + (int)threadIdx.x < g.batch.tokens) q = load_seq(g.batch, g.cache, t0 + threadIdx.x);
-      slots[threadIdx.x] = q.ok && q.m == 1 && q.first == t0 + (int)threadIdx.x && q.len > 0 ? q.len - 1 : -1;
+  // The tokens' slots in their sequences; -1 for a token of no sequence.  Where sequence i has token i alone, as in a batch
+  // without padding, one read finds them.
+  bool direct = g.batch.max_new == 1 && g.batch.tokens == g.batch.seqs;
+  if (direct) {
+    bool mine_is = true;
+    if (threadIdx.x < per_cta && t0 + (int)threadIdx.x < g.batch.tokens) {
+      const Seq q = load_seq(g.batch, g.cache, t0 + threadIdx.x);
+      mine_is = q.m == 1 && q.first == t0 + (int)threadIdx.x;
+      slots[threadIdx.x] = q.ok && q.len > 0 ? q.len - 1 : -1;
+    } else if (threadIdx.x < per_cta) {
+      slots[threadIdx.x] = -1;
     }
-  } else {
+    direct = __syncthreads_and(mine_is);
+  }
+  if (!direct) {
     for (int i = threadIdx.x >> 5; i < per_cta; i += NT / 32) {
       int s;
       const int at = t0 + i;
       const Seq q = find_seq(g, at, [](int cu, int) { return (long long)cu; }, s);
       if ((threadIdx.x & 31) == 0) slots[i] = at < g.batch.tokens && q.ok && at >= q.first && at < q.first + q.m ? q.len - q.m + (at - q.first) : -1;
     }
+    __syncthreads();
   }
   const Row<4> gain = ln.gain(g.q_gain);
-  __syncthreads();
   fill_table<NT>(g.t, table, per_cta, [&](int i) { return place_of(g.pos, g.axes, g.batch.tokens, min(t0 + i, g.batch.tokens - 1), slots[i]); });
   __syncthreads();
   const bool on = slots[mine] >= 0;                        // a token of no sequence is left alone

@@ -11,6 +11,7 @@
 namespace b200 {
 namespace kv {
 
+constexpr int MAX_SLOTS = 1 << 30; // of a sequence: slot arithmetic stays within 32 bits
 constexpr int MIN_EXP = -60;       // the smallest scale is 2^-60: what a block of zeros gets
 
 struct Cache {
@@ -33,7 +34,7 @@ struct Seq {
 // Whether a sequence's bounds fit the buffers; checked before any address is formed from them.
 __device__ __forceinline__ bool fits(const Batch& b, const Cache& c, const Seq& q) {
   return q.first >= 0 && q.m >= 0 && q.m <= b.max_new && q.first <= b.tokens - q.m && q.len >= 0 &&
-         q.len <= ((long long)b.max_pages << c.page_log2);
+         q.len <= min((long long)b.max_pages << c.page_log2, (long long)MAX_SLOTS);
 }
 __device__ __forceinline__ Seq load_seq(const Batch& b, const Cache& c, int s) {
   Seq q;

@@ -460,7 +460,7 @@ int b200_qk_norm_rotary_forward(int dtype, const b200_head_op* op, size_t batch,
                                 const size_t k_out_strides[4], void* stream);
 
 /* Its backward: grad_q and grad_k are written (each may be the upstream gradient itself); q_gain_grad and k_gain_grad (f32, d elements,
- * either may be NULL) are written, or added to when accumulate != 0.  The gains' sums over all rows have a fixed order:
+ * either may be NULL; B200_ERR_STRIDE where they overlap) are written, or added to when accumulate != 0.  The gains' sums over all rows have a fixed order:
  * the same bits in every run.  A broadcast (stride 0) q or k gets the gradient of every element of the view.
  * workspace: b200_qk_norm_rotary_backward_workspace_bytes(d) bytes, 16-byte aligned; not needed without gain gradients. */
 size_t b200_qk_norm_rotary_backward_workspace_bytes(size_t d);
@@ -493,8 +493,9 @@ typedef struct {
  * on the device and are read by the kernels: a captured graph replays with what they hold then.  Entries of the page
  * table behind a sequence's length are never read.  max_new: the most new tokens that a sequence has.  A sequence whose
  * numbers do not fit (cu_tokens outside [0, tokens] or falling, more than max_new tokens, a length outside
- * [0, max_pages * page_size]), and a page outside the cache, are skipped and reported as B200_ERR_INDEX by
- * b200_device_status.  Tokens of no sequence are left alone, in outputs too. */
+ * [0, max_pages * page_size] or above 2^30), and a page outside the cache, are skipped and reported as B200_ERR_INDEX by
+ * b200_device_status; where cu_tokens fall, sequences behind that place may be skipped too.  Tokens of no sequence are
+ * left alone, in outputs too. */
 typedef struct {
   size_t seqs, tokens, max_new;
   const int32_t* cu_tokens;
@@ -509,7 +510,8 @@ typedef struct {
  * NULL: the token's slot on every axis.  Codes are rounded to nearest, ties to even.  A block's scale is the smallest
  * power of two that brings its largest finite magnitude to at most 448 codes; it starts anew with the block's first
  * slot and never shrinks after; when it grows, the codes of the block's other slots move to it.  A page that several
- * sequences share must be full before they append.  f32 and f16. */
+ * sequences share must be full before they append: the pages that new tokens lie in are each one sequence's own.  f32
+ * and f16. */
 int b200_kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* batch, const b200_head_op* op, size_t q_heads,
                          const void* q, const size_t q_strides[3], const void* k, const size_t k_strides[3], const void* v,
                          const size_t v_strides[3], const int32_t* positions, void* q_out, const size_t q_out_strides[3],

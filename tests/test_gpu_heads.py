@@ -355,6 +355,27 @@ def test_append_with_positions_of_three_axes(cuda_dev):
     assert dev.device_status() == 0
 
 
+def test_append_padded_batches_of_single_tokens(cuda_dev):
+    """Sequences without a new token before those with one, tokens of no sequence behind: as many tokens as sequences."""
+    dev = cuda_dev
+    sv = Serving(dev, [5, 40, 17, 3, 64, 9], [0, 1, 1, 0, 1, 1], 16, 2, 64, 47)
+    sv.fill([5, 39, 16, 3, 63, 8])
+    q = torch.randn(6, 4, 64, generator=sv.g).half().cuda()
+    k, v = (torch.randn(6, 2, 64, generator=sv.g).half().cuda() for _ in range(2))
+    rotary = dfdx_b200.Rotary(dev.rotary_frequencies((32,)), (32,))
+    out = torch.full_like(q, 7.0)
+    dev.kv_cache_append(sv.cache, k, v, *sv.args(), q=q, rotary=rotary, q_out=out)
+    assert bool((out[4:] == 7.0).all())
+    pos = torch.tensor([[39, 16, 63, 8]], dtype=torch.int32).cuda()[:, None]
+    want, _ = dev.qk_norm_rotary_forward(q[None, :4], k[None, :4], rotary, pos, norm=False)
+    assert torch.equal(out[:4], want[0])
+    for s, tok in ((1, 0), (2, 1), (4, 2), (5, 3)):
+        got = sv.rows(s, sv.lens[s])[1][-1]
+        held = sv.cache.v_scale.cpu().double()[int(sv.table[s, (sv.lens[s] - 1) // 16])]
+        within(got, v[tok].cpu().double(), torch.maximum(2.0 ** -4 * v[tok].cpu().double().abs(), 2.0 ** -10 * held[:, None]), f"values {s}")
+    assert dev.device_status() == 0
+
+
 def test_append_reports_bounds_that_do_not_fit(cuda_dev):
     dev = cuda_dev
     sv = Serving(dev, [10, 10, 10], [2, 2, 2], 16, 1, 32, 43)
@@ -500,6 +521,37 @@ def test_attention_nan_in_slots_that_a_row_does_not_see(cuda_dev, new):
     nan = out[new - 2].isnan()
     assert bool(nan[:, 5].all()) and int(nan.sum()) == 2                  # the column whose value is NaN
     assert bool(out[new - 1].isnan().all()) and bool(lse[new - 1].isnan().all())
+
+
+@pytest.mark.parametrize("new", [(3, 43, 20), (0, 2, 48), (16, 17, 50)])
+def test_attention_of_a_padded_batch(cuda_dev, new):
+    """As many tokens as sequences of the longest length would have, though some are short: the rest belongs to none."""
+    dev = cuda_dev
+    sv = Serving(dev, [a + b for a, b in zip((70, 5, 200), new)], new, 16, 2, 64, 57)
+    sv.fill(sv.lens)
+    q = torch.randn(3 * max(new), 4, 64, generator=sv.g).half().cuda()
+    out = torch.full_like(q, 7.0)
+    _, lse = dev.kv_cache_attention(sv.cache, q, *sv.args(), 0.125, out=out, want_lse=True)
+    check_attention(dev, sv, q, out, lse, 0.125)
+    assert bool((out[sum(new):] == 7.0).all())
+    assert dev.device_status() == 0
+
+
+def test_lengths_above_the_limit_are_reported(cuda_dev):
+    dev = cuda_dev
+    cache = dev.kv_cache(1, 128, 1, 32)
+    x = torch.ones(1, 1, 32).half().cuda()
+    table = torch.zeros(1, (1 << 23) + 2, dtype=torch.int32, device="cuda")
+    cu, one, long = (torch.tensor(t, dtype=torch.int32).cuda() for t in ([0, 1], [1], [(1 << 30) + 1]))
+    dev.kv_cache_append(cache, x, x, cu, one, table, 1)
+    assert dev.device_status() == 0
+    out = torch.full_like(x, 7.0)
+    dev.kv_cache_append(cache, x + 1, x, cu, long, table, 1)
+    assert dev.device_status() == _lib.ERR_INDEX
+    dev.kv_cache_attention(cache, x, cu, long, table, 1, 1.0, window=16, out=out)
+    assert dev.device_status() == _lib.ERR_INDEX and bool((out == 7.0).all())
+    dev.kv_cache_attention(cache, x, cu, one, table, 1, 1.0, out=out)
+    assert dev.device_status() == 0 and bool((out == 1.0).all())
 
 
 def test_attention_strides_and_empty_rows(cuda_dev):

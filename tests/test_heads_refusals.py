@@ -68,6 +68,7 @@ def test_norm_rotary_backward(lib):
     assert backward(op(), nbytes=need - 1) == _lib.ERR_WORKSPACE
     assert backward(op(), ws=None) == _lib.ERR_NULL
     assert backward(op(norm=0)) == _lib.ERR_UNSUPPORTED                         # no norm, no gain's gradient
+    assert backward(op()) == _lib.ERR_STRIDE                                    # one buffer for both gains' gradients
 
 
 def append(lib, c=None, b=None, o=None, dtype=_lib.F16, q=P, q_heads=4, q_out=P, k=P, ks=None):
