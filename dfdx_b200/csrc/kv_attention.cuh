@@ -103,9 +103,10 @@ static __device__ __noinline__ void nan_fixup(const AttArgs& g, const Work& w, i
   }
 }
 
-// kv_attention_tc.cu: the rows of sequences with many.  g.tiles counts tiles of TC_ROWS rows.
+// kv_attention_tc.cu: the rows of sequences with many.  g.tiles counts tiles of TC_ROWS rows.  sort: the order of the CTAs
+// matters.
 constexpr int TC_ROWS = 256;
-int launch_attention_tc(const AttArgs& g, long long ctas, cudaStream_t stream);
+int launch_attention_tc(const AttArgs& g, long long ctas, bool sort, cudaStream_t stream);
 int setup_attention_tc();
 
 }  // namespace kv

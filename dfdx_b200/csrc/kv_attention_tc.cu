@@ -82,7 +82,9 @@ struct TcArgs2 {
   AttArgs a;
   uint32_t flip;                   // a negative alpha: the queries' signs are turned instead, so that every scale is positive
   long long wait_limit;
+  bool sorted;                     // CTAs take the row tiles of all sequences with the most slots first
 };
+constexpr int MOST_SORTED = 256;   // row tiles
 
 template <int DP>
 __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_constant__ TcArgs2 ga) {
@@ -93,17 +95,43 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
   __shared__ __align__(8) uint64_t bar_s_full[2][2], bar_p_full[2][2], bar_pv_done[2][2];   // per row tile and half of the slots
   __shared__ float4 scales[SCALE_SETS][8];                 // per 16 slots: key scale * alpha log2(e), log2 and reciprocal of the value scale
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_flag, sh_nan;
+  __shared__ int abort_flag, sh_nan, picked;
+  __shared__ __align__(16) int slots_of[MOST_SORTED];
 
   const uint32_t smem_base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
   volatile int* abortp = &abort_flag;
   asm volatile("griddepcontrol.launch_dependents;");
 
-  // the longest row tiles first: causal rows at the end of a sequence see the most slots
   unsigned unit = blockIdx.x / (unsigned)g.splits;
-  unit = unit - unit % (unsigned)g.tiles + ((unsigned)g.tiles - 1 - unit % (unsigned)g.tiles);
   const int x = (int)(blockIdx.x % (unsigned)g.splits);
+  if (ga.sorted) {
+    // CTA b has head b % heads of the row tile that is b / heads-th when all sequences' are put in the order of their
+    // slots: the last CTAs to start are then the shortest.  Ties go by index.
+    const int n = g.batch.seqs * g.tiles, i = threadIdx.x, want = (int)(unit / (unsigned)g.cache.heads);
+    if (i < MOST_SORTED) slots_of[i] = -2;                 // behind all others
+    if (i < n) {
+      const int s = i / g.tiles, row = i % g.tiles * TC_ROWS;
+      const Seq q = load_seq(g.batch, g.cache, s);
+      const int rows = q.ok ? q.m * g.group - row : 0;
+      slots_of[i] = rows > 0 ? max(view_of(g, q, row + min(rows, TC_ROWS) - 1).hi - view_of(g, q, row).lo, 0) : -1;
+    }
+    __syncthreads();
+    if (i < n) {
+      const int mine = slots_of[i];
+      int before = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; j += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(&slots_of[j]);
+        before += (v.x > mine - (j < i)) + (v.y > mine - (j + 1 < i)) + (v.z > mine - (j + 2 < i)) + (v.w > mine - (j + 3 < i));
+      }
+      if (before == want) picked = i;
+    }
+    __syncthreads();
+    unit = ((unsigned)(picked / g.tiles) * g.cache.heads + unit % (unsigned)g.cache.heads) * g.tiles + picked % g.tiles;
+  } else {                                                 // causal rows at the end of a sequence see the most slots
+    unit = unit - unit % (unsigned)g.tiles + ((unsigned)g.tiles - 1 - unit % (unsigned)g.tiles);
+  }
   Work w;
   if (!work_of<TC_ROWS>(g, unit, x, w)) return;
   const int ntile = w.rows > 128 ? 2 : 1;
@@ -475,12 +503,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
 
 namespace kv {
 
-int launch_attention_tc(const AttArgs& g, long long ctas, cudaStream_t stream) {
+int launch_attention_tc(const AttArgs& g, long long ctas, bool sort, cudaStream_t stream) {
   TcArgs2 a;
   a.a = g;
   a.flip = a.a.scale_log2 < 0.f ? 0x80008000u : 0u;
   a.a.scale_log2 = fabsf(a.a.scale_log2);
   if (a.a.scale_log2 == 0.f) a.a.scale_log2 = 1e-30f;       // keeps (masked score = -inf) * scale = -inf
+  a.sorted = sort && g.splits == 1 && (long long)g.batch.seqs * g.tiles <= MOST_SORTED;
   a.wait_limit = 400000000LL + (long long)(g.range / 128) * 400000LL;
   if (g.cache.d <= 64) kv_prefill_kernel<64><<<(unsigned)ctas, THREADS, Cfg<64>::SMEM_BYTES, stream>>>(a);
   else kv_prefill_kernel<128><<<(unsigned)ctas, THREADS, Cfg<128>::SMEM_BYTES, stream>>>(a);

@@ -451,6 +451,7 @@ ATT = [  # page, heads, q_heads, d, past, new, causal, window
     (64, 1, 8, 128, [9000, 3], [40, 33], True, 0),                       # many rows over ranges that are joined
     (32, 1, 16, 96, [6000], [60], True, 2500),
     (128, 2, 32, 64, [3000, 5000], [3, 40], False, 0),
+    (16, 8, 32, 32, [100, 5, 700, 0], [900, 3, 500, 0], True, 0),        # more row tiles than SMs, of uneven length
     (64, 1, 40, 32, [300], [1], True, 0),                                # one token, more heads than a small tile's rows
 ]
 
