@@ -164,11 +164,11 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 3 : 2) kv_decode_kernel(
         for (int e = 0; e < 4; ++e) sc[t][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const uint32_t a0 = values2(kw[0][ks]), a1 = values2(kw[1][ks]), a2 = values2(kw[0][ks] >> 16), a3 = values2(kw[1][ks] >> 16);
+        const uint2 lo = values4(kw[0][ks]), hi = values4(kw[1][ks]);
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
           const uint2 b = Q_REGS ? qf[Q_REGS ? ks : 0] : sh_q[(t * KS + ks) * 32 + lane];
-          mma16816(sc[t], a0, a1, a2, a3, b.x, b.y);
+          mma16816(sc[t], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
         }
       }
 
@@ -240,9 +240,9 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 3 : 2) kv_decode_kernel(
           // codes 4 x + 2 b and + 1 of the lane's run: (slot, slot + 1) pairs side by side
           const uint32_t sel = b == 0 ? 0x5140u : 0x7362u;
           const uint32_t x0 = __byte_perm(vw[0][x], vw[1][x], sel), x1 = __byte_perm(vw[2][x], vw[3][x], sel);
-          const uint32_t a0 = values2(x0), a1 = values2(x0 >> 16), a2 = values2(x1), a3 = values2(x1 >> 16);
+          const uint2 lo = values4(x0), hi = values4(x1);
 #pragma unroll
-          for (int t = 0; t < NQ; ++t) mma16816(o[t][2 * x + b], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+          for (int t = 0; t < NQ; ++t) mma16816(o[t][2 * x + b], lo.x, lo.y, hi.x, hi.y, pb[t][0], pb[t][1]);
         }
     };
     uint32_t ka[2][KW], va[4][VW], kb[2][KW], vb[4][VW];

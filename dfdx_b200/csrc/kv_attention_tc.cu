@@ -60,6 +60,11 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&v
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 // Two f32 in one register pair: the scores come out of tensor memory in neighbouring registers.
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   uint64_t r;
@@ -275,9 +280,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
         for (int p = 0; p < PC; ++p) {
           if ((c4 + 4 * p) * 16 >= d) continue;
           const uint4 q = from[i][p];
+          const uint2 a = values4(q.x), b = values4(q.y), e = values4(q.z), f = values4(q.w);
           const uint32_t row = tile + (uint32_t)p * 16384 + r * 128;
-          st_shared_v4_u32(row + ((((uint32_t)c4 * 2) ^ (r & 7u)) << 4), values2(q.x), values2(q.x >> 16), values2(q.y), values2(q.y >> 16));
-          st_shared_v4_u32(row + ((((uint32_t)c4 * 2 + 1) ^ (r & 7u)) << 4), values2(q.z), values2(q.z >> 16), values2(q.w), values2(q.w >> 16));
+          st_shared_v4_u32(row + ((((uint32_t)c4 * 2) ^ (r & 7u)) << 4), a.x, a.y, b.x, b.y);
+          st_shared_v4_u32(row + ((((uint32_t)c4 * 2 + 1) ^ (r & 7u)) << 4), e.x, e.y, f.x, f.y);
         }
       }
     };
@@ -389,10 +395,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
         for (int b = 0; b < 4; ++b) {
           float e0 = __uint_as_float(xr[b * 16]), e1 = __uint_as_float(xr[b * 16 + 1]);
 #pragma unroll
-          for (int q = 2; q < 16; q += 2) {
-            e0 = fmaxf(e0, __uint_as_float(xr[b * 16 + q]));
-            e1 = fmaxf(e1, __uint_as_float(xr[b * 16 + q + 1]));
+          for (int q = 2; q < 14; q += 4) {
+            e0 = max3(e0, __uint_as_float(xr[b * 16 + q]), __uint_as_float(xr[b * 16 + q + 1]));
+            e1 = max3(e1, __uint_as_float(xr[b * 16 + q + 2]), __uint_as_float(xr[b * 16 + q + 3]));
           }
+          e0 = max3(e0, __uint_as_float(xr[b * 16 + 14]), __uint_as_float(xr[b * 16 + 15]));
           const float2 s2 = *reinterpret_cast<const float2*>(&sc[b]);
           top = fmaxf(top, fmaf(fmaxf(e0, e1), s2.x, s2.y));   // the scales are positive: see flip
         }

@@ -260,7 +260,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC 
         const int r = i / words;
         if (r >= row0 && r < row0 + rows) continue;
         uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
-        const float2 f = halves(values2(*w)), h = halves(values2(*w >> 16));
+        const uint2 x4 = values4(*w);
+        const float2 f = halves(x4.x), h = halves(x4.y);
         const float v[4] = {f.x, f.y, h.x, h.y};
         *w = codes4(v, ratio);
       }
@@ -286,7 +287,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const Cache c, const int* 
 #pragma unroll 4
   for (int i = threadIdx.x; i < chunks; i += 256) {
     const uint2 x = ok ? codes[i] : make_uint2(0, 0);
-    const float2 a = halves(values2(x.x)), b = halves(values2(x.x >> 16)), e = halves(values2(x.y)), f = halves(values2(x.y >> 16));
+    const uint2 lo = values4(x.x), hi = values4(x.y);
+    const float2 a = halves(lo.x), b = halves(lo.y), e = halves(hi.x), f = halves(hi.y);
     if constexpr (sizeof(T) == 2) {
       reinterpret_cast<uint4*>(out)[i] = make_uint4(half2_of(a.x * scale, a.y * scale), half2_of(b.x * scale, b.y * scale),
                                                     half2_of(e.x * scale, e.y * scale), half2_of(f.x * scale, f.y * scale));

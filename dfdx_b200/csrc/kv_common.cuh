@@ -66,9 +66,10 @@ __device__ __forceinline__ uint32_t codes2(float x, float y) {
 __device__ __forceinline__ uint32_t codes4(const float (&x)[4], float inv) {
   return codes2(x[0] * inv, x[1] * inv) | codes2(x[2] * inv, x[3] * inv) << 16;
 }
-__device__ __forceinline__ uint32_t values2(uint32_t codes) {      // the low two codes as two f16
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)codes));
+__device__ __forceinline__ uint2 values4(uint32_t codes) {         // four codes as f16, exact
+  uint2 r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+      : "=r"(r.x), "=r"(r.y) : "r"(codes));
   return r;
 }
 
