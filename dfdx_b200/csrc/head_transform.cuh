@@ -7,11 +7,10 @@
 // for every rotated pair i, whose two elements are (i, i + pairs) or, interleaved, (2 i, 2 i + 1); the elements behind
 // 2 * pairs pass through.  The pairs are dealt to the position axes in consecutive sections.
 //
-// A row of d elements belongs to a group of LPR lanes, S = 4 pairs ("slots") and so eight elements a lane: both elements of
-// a pair sit in one lane, and the row's sum of squares is the only exchange.  Slot j's elements are those of pair j;
-// slots j >= pairs hold the pass-through elements 2 j, 2 j + 1 with cos = 1, sin = 0.  (Eight slots a lane for f16, with
-// 16-byte accesses and half the exchanges, took the registers of half the warps: 161 us against 116 for the backward of
-// 2 x 8192 tokens, 36 heads of 128.)
+// A row of d elements belongs to a group of LPR lanes with S pairs ("slots"), 2 S elements, a lane: both elements of a pair
+// sit in one lane, and the row's sum of squares is the only exchange.  Slot j's elements are those of pair j; slots
+// j >= pairs hold the pass-through elements 2 j, 2 j + 1 with cos = 1, sin = 0.  S is 8 in the forward of f16 rows that
+// 16-byte accesses fit, else 4.
 //
 // The angle is reduced in turns in f64: position * (frequency / 2 pi) minus its nearest whole number loses
 // 2^-53 * |turns|, nothing that f32 sees for any 32-bit position; the remainder's sine and cosine are f32.

@@ -13,14 +13,19 @@
 //
 //   kv_decode_kernel    few rows: bound by reading the codes.  A CTA has one (sequence, key head), up to 8 * NQ of its
 //                       rows (a row is a new token and one of the query heads that share the key head) and a range of
-//                       slots; each of its four warps walks 16 slots at a time on m16n8k16 f16 matrix instructions.
+//                       slots; its four warps take every fourth 16 slots each, on m16n8k16 f16 matrix instructions (the
+//                       fifth-generation ones take 128 rows at least, which a token's shared heads do not fill).
 //                       The order of the products' summation index and of the output columns is free, and is chosen so
 //                       that each lane reads whole 16-byte (d = 128) pieces of a row, a warp whole 128-byte lines, and
 //                       that no lane needs what another has read: codes go from global memory to registers, a tile
-//                       ahead, with no shared memory and no barrier in the loop.
+//                       ahead, with no shared memory and no barrier in the loop.  (A ring in shared memory filled by
+//                       asynchronous copies took 150 us where this takes 117.)
 //                       Scores, maxima, sums and outputs are f32; codes are exact in f16, probabilities are rounded
 //                       to f16 for the second product only (2^-12 of each, of random sign).
-//   kv_combine_kernel   joins the ranges of a row, in order.
+//                       48 sequences of 200 to 12000 slots, one token, 32 query and 8 key heads of 128: 117 us with the
+//                       joining, 5.2 TB/s, 0.79 of a plain copy; one of 131000: 53 us, 5.0 TB/s.
+//   kv_combine_kernel   joins the ranges of a row, in order; its launch overlaps the end of the kernel before.
+// The kernel for many rows is in kv_attention_tc.cu.
 // A range is a fixed number of slots, not a share of the sequence, so that ragged lengths give CTAs of equal work.
 #include "kv_attention.cuh"
 
@@ -305,7 +310,8 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 3 : 2) kv_decode_kernel(
 
 // The ranges' partial results of a row, joined in order.  COLS lanes take a row's d elements, four each.  Up to FEW_RANGES
 // ranges: these lanes hold all of a row's at once, several rows a CTA.  More: a CTA has one row, and every PARTS-th range
-// goes to one of its groups of lanes.
+// goes to one of its groups of lanes.  (With the first form up to 2 ranges only: 6.5 us against 6.1 for one sequence of 900
+// slots, 119.5 against 117 for 48 of up to 12000.)
 constexpr int FEW_RANGES = 8;
 template <int D, int R, bool FEW>
 __global__ void __launch_bounds__(128) kv_combine_kernel(const AttArgs g, long long rows_all) {
@@ -394,9 +400,12 @@ struct Plan {
   size_t m_rows() const { return many && m.splits > 1 ? (size_t)m_ctas() * TC_ROWS : 0; }
 };
 
-// Sequences with up to this many rows go to the kernel for few rows.
+// Sequences with up to this many rows go to the kernel for few rows.  In us, this kernel against the one for many, 32 query
+// and 8 key heads: 24 sequences of 50 to 6000 slots, 20 rows of 128: 81, 93; 32 rows of 96: 83, 95; one sequence of 30000,
+// 32 rows of 96: 31, 41; 64 short ones, 32 rows of 128: 61, 65.  At 32 rows of 128 the registers are used up and the two
+// meet: 112, 95 for the 24 sequences, 40, 40 for the long one.
 constexpr int FEW_ROWS = 32;
-constexpr int ROUNDS = 4;
+constexpr int ROUNDS = 4;          // 48 sequences of 200 to 12000 slots: 138 us with 3, 120 with 4, 121 with 6, 127 with 8
 
 // How the rows and slots of a call are cut.  Everything follows from what the host knows: the lengths stay on the device,
 // the page table's width bounds them.

@@ -1,15 +1,22 @@
 // Norm of every query and key head with the position rotation in the same pass, forward and backward
-// (head_transform.cuh has the formulas).  Both are bound by HBM: forward reads and writes each element once, backward
-// reads x and the upstream gradient once and writes the gradient once; the norm's statistics are recomputed from the
-// row that the backward holds anyway, so nothing is saved between the two.
+// (head_transform.cuh has the formulas).  The least that has to move is each element once in and once out forward, x and
+// the upstream gradient in and the gradient out backward; the norm's statistics are recomputed from the row that the
+// backward holds anyway, so nothing is saved between the two.
 //
 //   qk_forward_kernel   a group of LPR lanes owns a token and walks its heads (queries, then keys) `per_token` groups
-//                       apart: the angles' sines are computed once per token and group and serve all its heads.
-//   qk_backward_kernel  the same walk.  With h' = R^T g the gradient before the rotation,
+//                       apart.  The angles' sines go through f64 and are worth about 60 instructions a pair: they are put
+//                       into a table in shared memory once for all heads, under the first rows' loads.  Two sets of rows
+//                       in registers, one on its way while the other is worked on.
+//                       Bound by HBM: 16384 tokens, 40 heads of 128, f16: 64 us, 5.3 TB/s, 0.81 of a plain copy.
+//   qk_backward_kernel  the same walk by CTAs that stay and loop.  With h' = R^T g the gradient before the rotation,
 //                         dgain += h' * xhat,   dx = r (h' gain - xhat mean(h' gain xhat)),   xhat = x r.
 //                       The gains' sums stay in f32 registers over all rows of a lane, are added up per CTA in a fixed
 //                       order and leave as one row of partial sums per CTA.
-//   gain_sum_kernel     adds the CTAs' rows in a fixed order: no atomics, the same bits in every run.
+//                       Bound by what 16 warps an SM (12 in f32) can have on their way and by issue (0.54 of the cycles
+//                       issue): 16384 tokens, 36 heads of 128, f16: 107 us, 4.2 TB/s; 4950 tokens, 24 heads of 96, f32:
+//                       37 us, 3.7 TB/s.  More warps do not fit: x, g and the sums of both gains take 119 registers.
+//   gain_sum_kernel     adds the CTAs' rows in a fixed order: no atomics, the same bits in every run.  Its launch overlaps
+//                       the end of the backward.
 #include "head_transform.cuh"
 
 namespace b200 {
@@ -23,8 +30,8 @@ struct Side {                      // queries or keys
   void* y;                         // output; gradient (backward)
   const void* gain;
   int heads;
-  int xh, uh, yh;                  // element strides of the head, batch and token axes
-  long long xb, xt, ub, ut, yb, yt;
+  int xh, uh, yh;                  // element strides: head axis,
+  long long xb, xt, ub, ut, yb, yt;  // batch and token axes
 };
 struct QkArgs {
   Transform t;
@@ -306,8 +313,10 @@ int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq
   g.seq = (int)seq; g.d = (int)d;
   g.pos = positions;
   const bool inter = op->interleaved != 0;
-  // Elements that a lane moves at a time.  Eight of f16 (16 bytes) halve the forward's instructions; the backward, with
-  // twice the rows in registers, would lose half its warps to them (186 us against 130 for 2 x 8192 tokens of 36 heads).
+  // Elements that a lane moves at a time.  Eight of f16 (16 bytes) halve the forward's loads, stores and exchanges (66 us
+  // against 70 for 16384 tokens, 40 heads of 128); the backward, with two inputs and the gains' sums in registers, would
+  // lose a quarter of its warps to them (119 us against 109 for 16384 tokens, 36 heads of 128, 41 against 33 for 8192, 32 of
+  // 64).
   int run = 0;
   for (int n = es == 2 && !backward ? 8 : 4; n >= 4 && !run; n /= 2) {
     bool ok = d % (2 * n) == 0 && g.t.pairs % n == 0;
