@@ -4,10 +4,10 @@
 // backward holds anyway, so nothing is saved between the two.
 //
 //   qk_forward_kernel   a group of LPR lanes owns a token and walks its heads (queries, then keys) `per_token` groups
-//                       apart.  The angles' sines go through f64 and are worth about 60 instructions a pair: they are put
-//                       into a table in shared memory once for all heads, under the first rows' loads.  Two sets of rows
-//                       in registers, one on its way while the other is worked on.
-//                       Bound by HBM: 16384 tokens, 40 heads of 128, f16: 64 us, 5.3 TB/s, 0.81 of a plain copy.
+//                       apart.  The angles go through f64 and are the costliest part: their sines are put into a table in
+//                       shared memory once for all heads, under the first rows' loads.  Two sets of rows in registers,
+//                       one on its way while the other is worked on.
+//                       Bound by HBM: 16384 tokens, 40 heads of 128, f16: 63 us, 5.3 TB/s, 0.81 of a plain copy.
 //   qk_backward_kernel  the same walk by CTAs that stay and loop.  With h' = R^T g the gradient before the rotation,
 //                         dgain += h' * xhat,   dx = r (h' gain - xhat mean(h' gain xhat)),   xhat = x r.
 //                       The gains' sums stay in f32 registers over all rows of a lane, are added up per CTA in a fixed
@@ -313,8 +313,8 @@ int qk_norm_rotary(int dtype, const b200_head_op* op, int64_t batch, int64_t seq
   g.seq = (int)seq; g.d = (int)d;
   g.pos = positions;
   const bool inter = op->interleaved != 0;
-  // Elements that a lane moves at a time.  Eight of f16 (16 bytes) halve the forward's loads, stores and exchanges (66 us
-  // against 70 for 16384 tokens, 40 heads of 128); the backward, with two inputs and the gains' sums in registers, would
+  // Elements that a lane moves at a time.  Eight of f16 (16 bytes) halve the forward's loads, stores and exchanges (63 us
+  // against 85 for 16384 tokens, 40 heads of 128); the backward, with two inputs and the gains' sums in registers, would
   // lose a quarter of its warps to them (119 us against 109 for 16384 tokens, 36 heads of 128, 41 against 33 for 8192, 32 of
   // 64).
   int run = 0;
