@@ -9,7 +9,7 @@
 //                     for sequences that do not fit.  A page's scale starts anew with its first row.
 //                     Bound by instruction issue (two thirds of the cycles issue) and by the latencies of a block's CTA
 //                     (bounds, page, rows, the largest of all rows, codes), which three CTAs an SM overlap.  9 prompts of 130
-//                     to 1900 tokens, 10117 in all, 32 query and 8 key heads of 128, pages of 64, f16: 61 us, 3.8 TB/s; one
+//                     to 1900 tokens, 10117 in all, 32 query and 8 key heads of 128, pages of 64, f16: 61 us, 3.7 TB/s; one
 //                     token of 64 sequences: 4.4 us, mostly the launch.
 //   kv_read_kernel    codes times scale, 8 codes a thread and step; bound by HBM: 512 pages of 64 slots, 8 heads of 128, to f16:
 //                     38 us, 5.3 TB/s.
