@@ -87,7 +87,12 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 3 : 2) kv_decode_kernel(
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, c = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;");       // the joining kernel may be brought in; it waits for this one
   Work w;
-  if (!work_of<R>(g, blockIdx.x / (unsigned)g.splits, (int)(blockIdx.x % (unsigned)g.splits), w)) return;
+  // All sequences' first ranges, then the second ones, and so on: what runs last are the ends of the longest.  (17.2 us
+  // against 17.6 sequence by sequence for 24 sequences' drafts of 2 to 5 tokens, 22.3 against 23.3 for 16 of 4.)
+  const unsigned units = gridDim.x / (unsigned)g.splits, unit = blockIdx.x % units;
+  const int x_range = (int)(blockIdx.x / units);
+  if (!work_of<R>(g, unit, x_range, w)) return;
+  const long long cta = (long long)unit * g.splits + x_range;        // its place among the partial results
   if (threadIdx.x == 0) sh_nan = 0;
 
   // the queries as the second operand: lane (gr, c) has four elements of row gr at each step, the same order of summation
@@ -299,10 +304,10 @@ __global__ void __launch_bounds__(WARPS * 32, NQ == 1 ? 3 : 2) kv_decode_kernel(
         *reinterpret_cast<uint4*>(g.out + tok * g.ot + qh * g.oh + j) = pk;
         if (g.lse && j == 0) g.lse[(long long)tok * g.q_heads + qh] = sum == 0.f ? -INFINITY : (top - LIFT + log2f(sum)) * 0.6931471805599453f;
       } else {
-        float* dst = g.part_o + ((long long)blockIdx.x * R + t * 8 + r) * D + j;
+        float* dst = g.part_o + (cta * R + t * 8 + r) * D + j;
         *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        if (j == 0) g.part_ml[(long long)blockIdx.x * R + t * 8 + r] = make_float2(top, sum);
+        if (j == 0) g.part_ml[cta * R + t * 8 + r] = make_float2(top, sum);
       }
     }
   }
