@@ -1,16 +1,16 @@
 // Appending keys and values to the paged 8-bit cache (kv_common.cuh), the norm and rotation of the keys on the way, and
 // the new tokens' queries normed and rotated by the same launch; and reading blocks of the cache back.
 //
-//   kv_append_kernel  one CTA per (sequence, page that its new tokens touch, head, keys or values; keys of several heads one
-//                     after another, which share the rows' sines): it holds all new rows of the block in registers, takes
-//                     their largest magnitude, settles the block's scale and writes the codes, so that each input is read
-//                     once and no other CTA ever touches the block.  A block whose scale grows under earlier rows has
-//                     these moved to the new scale, a power-of-two step.  Further CTAs take the queries, one more looks
-//                     for sequences that do not fit.  A page's scale starts anew with its first row.
+//   kv_append_kernel  one CTA per (sequence, page that its new tokens touch, some heads, keys or values), a head's block
+//                     after another: it holds all new rows of the block in registers, takes their largest magnitude,
+//                     settles the block's scale and writes the codes, so that each input is read once and no other CTA
+//                     ever touches the block.  A block whose scale grows under earlier rows has these moved to the new
+//                     scale, a power-of-two step.  Further CTAs take the queries, one more looks for sequences that do
+//                     not fit.  A page's scale starts anew with its first row.
 //                     Bound by instruction issue (two thirds of the cycles issue) and by the latencies of a block's CTA
 //                     (bounds, page, rows, the largest of all rows, codes), which three CTAs an SM overlap.  9 prompts of 130
-//                     to 1900 tokens, 10117 in all, 32 query and 8 key heads of 128, pages of 64, f16: 61 us, 3.7 TB/s; one
-//                     token of 64 sequences: 4.4 us, mostly the launch.
+//                     to 1900 tokens, 10117 in all, 32 query and 8 key heads of 128, pages of 64, f16: 58 us, 3.9 TB/s; one
+//                     token of 64 sequences: 4.1 us, mostly the launch.
 //   kv_read_kernel    codes times scale, 8 codes a thread and step; bound by HBM: 512 pages of 64 slots, 8 heads of 128, to f16:
 //                     38 us, 5.3 TB/s.
 // Which (sequence, page) a CTA has follows from cu_tokens alone: a sequence that ends at token e can touch at most
@@ -30,8 +30,8 @@ struct AppendArgs {
   Transform t;
   Cache cache;
   Batch batch;
-  int key_heads;                   // heads that a key CTA takes one after another
-  unsigned k_ctas, v_ctas;         // candidates (sequence, page) * head groups; candidates * heads; the CTAs behind take queries
+  int heads_each;                  // heads that a CTA of keys or values takes one after another
+  unsigned k_ctas, v_ctas;         // candidates (sequence, page) * groups of heads; the CTAs behind take queries
   int q_heads, per_token;
   int axes;
   const int* pos;                  // axes x tokens, or nullptr: the token's slot on every axis
@@ -176,10 +176,10 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (ROWS * sizeof(T) <= 8 && VEC 
   constexpr bool AHEAD = VEC && ROWS * sizeof(T) <= 16;    // registers for the next head's rows beside this one's
   __shared__ float warp_top[2][NT / 32];
   const bool values = blockIdx.x >= g.k_ctas;
-  const int per_unit = values ? g.cache.heads : (g.cache.heads + g.key_heads - 1) / g.key_heads;
+  const int per_unit = (g.cache.heads + g.heads_each - 1) / g.heads_each;
   const unsigned at = blockIdx.x - (values ? g.k_ctas : 0);
-  const int unit = (int)(at / (unsigned)per_unit), head0 = (int)(at % (unsigned)per_unit) * (values ? 1 : g.key_heads);
-  const int head1 = min(head0 + (values ? 1 : g.key_heads), g.cache.heads);
+  const int unit = (int)(at / (unsigned)per_unit), head0 = (int)(at % (unsigned)per_unit) * g.heads_each;
+  const int head1 = min(head0 + g.heads_each, g.cache.heads);
   const int page = g.cache.page, shift = g.cache.page_log2;
   // unit -> (sequence, which of its touched pages)
   int s, nth;
@@ -368,11 +368,14 @@ int kv_cache_append(int dtype, const b200_kv_cache* cache, const b200_kv_batch* 
   const int lpr = vec && g.cache.d <= 64 ? 8 : 16, groups = (g.batch.max_new == 1 ? NT_ONE : NT_MANY) / lpr;
   // a sequence's m new tokens touch at most (m - 1) / page + 2 pages, one token only one
   const int64_t units = g.batch.max_new == 1 ? g.batch.seqs : (int64_t)(g.batch.tokens >> g.cache.page_log2) + 2 * (int64_t)g.batch.seqs;
-  // A key CTA computes its rows' sines once for several heads, as long as two CTAs an SM remain (61 us against 72 with one
-  // head a CTA, for the 9 prompts).
-  g.key_heads = 1;
-  while (g.key_heads < g.cache.heads && units * ((g.cache.heads + 2 * g.key_heads - 1) / (2 * g.key_heads)) >= 2 * ds->sm_count) g.key_heads *= 2;
-  const int64_t k_ctas = units * ((g.cache.heads + g.key_heads - 1) / g.key_heads), v_ctas = units * g.cache.heads;
+  // A CTA takes several heads: its look-ups and the rows' sines serve them all, and the next head's rows load under this one's
+  // work.  As long as the keys alone leave a CTA for every SM, beside which the queries' run: 58 us for the 9 prompts, with
+  // two for every SM 61, half a one 58; 4.1, 4.5 and 5.0 for one token of 64 sequences; 57, 60 and 73 for 3 prompts of 500
+  // to 2000 tokens with 32 key heads.  Without queries two for every SM: 29 us, with one 36, three 31 for the 9 prompts.
+  const int64_t least = g.q_heads ? ds->sm_count : 2 * (int64_t)ds->sm_count;
+  g.heads_each = 1;
+  while (g.heads_each < g.cache.heads && units * ((g.cache.heads + 2 * g.heads_each - 1) / (2 * g.heads_each)) >= least) g.heads_each *= 2;
+  const int64_t k_ctas = units * ((g.cache.heads + g.heads_each - 1) / g.heads_each), v_ctas = k_ctas;
   const bool one = g.batch.max_new == 1;
   g.per_token = groups_per_token(g.batch.tokens, g.q_heads, groups, (int64_t)ds->sm_count * (one ? 8 : 3), !vec ? 1 : es == 4 ? 2 : 4, false);
   const int64_t per_cta = groups / g.per_token, q_ctas = g.q_heads ? (g.batch.tokens + per_cta - 1) / per_cta : 0;

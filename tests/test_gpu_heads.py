@@ -249,10 +249,13 @@ APPEND = [  # dtype, page, heads, q_heads, d, past, new, pairs, interleaved, nor
     (F16, 128, 4, 4, 64, [0, 100, 127, 3], [300, 28, 2, 129], 32, False, False),
     (F16, 16, 3, 3, 128, [7, 0, 15, 16, 17], [0, 0, 40, 16, 3], 0, False, False),
     (F32, 64, 2, 4, 128, [10], [200], 30, False, True),                  # pairs no multiple of 4
+    (F16, 16, 5, 10, 64, [7 * i % 50 for i in range(100)], [1] * 100, 32, False, True),            # several heads a CTA, the
+    (F16, 16, 7, 7, 96, [5 * i % 33 for i in range(60)], [1 + 11 * i % 37 for i in range(60)], 48, False, True),  # last fewer
+    (F32, 32, 3, 3, 64, [3 * i % 40 for i in range(70)], [1 + 13 * i % 50 for i in range(70)], 16, True, False),
 ]
 
 
-@pytest.mark.parametrize("case", APPEND, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c))
+@pytest.mark.parametrize("case", APPEND, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c)[:80])
 def test_append(cuda_dev, case):
     dtype, page, heads, hq, d, past, new, pairs, inter, norm = case
     dev = cuda_dev
