@@ -95,6 +95,9 @@ struct TcArgs2 {
   bool sorted;                     // CTAs take the row tiles of all sequences with the most slots first
 };
 constexpr int MOST_SORTED = 256;   // row tiles
+// The least factor of a block's scores, also where alpha is 0 or alpha * scale vanishes in f32: a masked score is -infinity
+// before it is scaled, and 0 would make NaN of it.  Scores are below 65504 * 448 * 128 < 2^32: this one moves no exponent.
+constexpr float MIN_FACTOR = 1.1754944e-38f;               // 2^-126
 
 template <int DP>
 __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_constant__ TcArgs2 ga) {
@@ -294,12 +297,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prefill_kernel(const __grid_con
     };
     // Scales of the group that lane i < 2 answers for (of rows row0 + 64 i), for the tile whose pages are `id`.
     auto scale_of = [&](const int (&id)[2]) -> float4 {
-      float4 sc = make_float4(g.scale_log2, -INFINITY, 1.f, 0.f);             // no such slots: their scores count for nothing
+      float4 sc = make_float4(1.f, -INFINITY, 1.f, 0.f);   // no such slots: their scores count for nothing
       const int p = lane == 0 ? id[0] : id[1];
       if ((cw & 1) == 0 && lane < 2 && p >= 0) {
         const long long blk = (long long)p * g.cache.heads + w.head;
         const uint32_t sv = __float_as_uint(__ldg(g.cache.v_scale + blk));
-        sc = make_float4(__ldg(g.cache.k_scale + blk) * g.scale_log2, (float)((int)(sv >> 23) - 127), __uint_as_float((254u << 23) - sv), 0.f);
+        sc = make_float4(fmaxf(__ldg(g.cache.k_scale + blk) * g.scale_log2, MIN_FACTOR), (float)((int)(sv >> 23) - 127),
+                         __uint_as_float((254u << 23) - sv), 0.f);
       }
       return sc;
     };
@@ -520,7 +524,6 @@ int launch_attention_tc(const AttArgs& g, long long ctas, bool sort, cudaStream_
   a.a = g;
   a.flip = a.a.scale_log2 < 0.f ? 0x80008000u : 0u;
   a.a.scale_log2 = fabsf(a.a.scale_log2);
-  if (a.a.scale_log2 == 0.f) a.a.scale_log2 = 1e-30f;       // keeps (masked score = -inf) * scale = -inf
   a.sorted = sort && g.splits == 1 && (long long)g.batch.seqs * g.tiles <= MOST_SORTED;
   a.wait_limit = 400000000LL + (long long)(g.range / 128) * 400000LL;
   if (g.cache.d <= 64) kv_prefill_kernel<64><<<(unsigned)ctas, THREADS, Cfg<64>::SMEM_BYTES, stream>>>(a);

@@ -1,0 +1,41 @@
+"""Limits of the per-head norm and rotation, the 8-bit cache and the attention over it: factors of zero, positions at the
+ends of 32 bits, strides that no address depends on, many sequences, the forms of the append that single tokens take.
+
+Definitions: tests/heads_reference.py; tolerances as in tests/test_gpu_heads.py unless a test derives its own.
+"""
+import pytest
+import torch
+
+import heads_reference as ref
+from test_gpu_heads import Serving, check_attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("window", [0, 21])
+@pytest.mark.parametrize("new", [3, 45])
+def test_attention_with_a_factor_of_zero(cuda_dev, new, window):
+    """alpha = 0, or so small that its product with a block's scale is 0 in f32, takes the mean of the visible values: with
+    blocks of zero keys (the least scale, 2^-60) on both sides of the causal edge and of the window's, and a block of keys
+    of about 2^100.  In sequences of few and of many rows, alone and in one batch."""
+    dev = cuda_dev
+    for lens, news in (([100 + new], [new]), ([20 + new, 64, 70], [new, 1, min(new, 64)])):
+        sv = Serving(dev, lens, lens, 16, 1, 64, 73)
+        n = sum(lens)
+        k, v = (torch.randn(n, 1, 64, generator=sv.g) for _ in range(2))
+        at = 0
+        for m in lens:
+            slot = torch.arange(m)
+            k[at:at + m][slot // 16 % 3 == 0] = 0.0
+            k[at:at + m][slot >= m - new] = 0.0                           # the edge of all rows lies among zero keys
+            k[at:at + m][slot // 16 == 1] *= 2.0 ** 100
+            at += m
+        dev.kv_cache_append(sv.cache, k.cuda(), v.cuda(), *sv.args())
+        assert float(sv.cache.k_scale[int(sv.table[0, 0]), 0]) == ref.MIN_SCALE
+        sv.new = news
+        q = torch.randn(sum(news), 2, 64, generator=sv.g).half().cuda()
+        for alpha in (0.0, -0.0, 1e-40, 2.0 ** -100, -2.0 ** -100, 2.0 ** -126):
+            out, lse = dev.kv_cache_attention(sv.cache, q, *sv.args(), alpha, window=window, want_lse=True)
+            assert bool(out.isfinite().all()) and bool(lse.isfinite().all()), alpha
+            check_attention(dev, sv, q, out, lse, alpha, True, window)
+    assert dev.device_status() == 0
