@@ -44,7 +44,8 @@ __device__ __forceinline__ Seq load_seq(const Batch& b, const Cache& c, int s) {
   q.ok = fits(b, c, q);
   return q;
 }
-__device__ __forceinline__ void flag_index(int* status) { atomicExch(status, (int)B200_ERR_INDEX); }
+// A wait that ran out (it exchanges the word) says more, and stays.
+__device__ __forceinline__ void flag_index(int* status) { atomicCAS(status, 0, (int)B200_ERR_INDEX); }
 
 // The exponent of the smallest power of two s with absmax <= 448 s; 448 = 1.75 * 2^8.
 __device__ __forceinline__ int scale_exp(float absmax) {

@@ -107,8 +107,8 @@ const char* b200_strerror(int status);
 /* Text of the last CUDA error seen by this thread inside the library ("" if none). */
 const char* b200_last_cuda_error(void);
 /* Reads (and clears) the device-side status word of the current device after synchronising
- * `stream`: 0, B200_ERR_DEVICE_TIMEOUT if any kernel gave up on a bounded wait, or B200_ERR_INDEX if one met an index
- * outside its buffers; the latest of several. */
+ * `stream`: 0, B200_ERR_DEVICE_TIMEOUT if any kernel gave up on a bounded wait, otherwise B200_ERR_INDEX if one met an
+ * index outside its buffers. */
 int b200_device_status(void* stream);
 /* Process-wide override of kernel-family selection (testing / profiling). */
 int b200_set_path(int path);

@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import heads_reference as ref
-from test_gpu_heads import Serving, check_attention
+from dfdx_b200 import _lib
+from test_gpu_heads import F32, Serving, check_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -38,4 +39,25 @@ def test_attention_with_a_factor_of_zero(cuda_dev, new, window):
             out, lse = dev.kv_cache_attention(sv.cache, q, *sv.args(), alpha, window=window, want_lse=True)
             assert bool(out.isfinite().all()) and bool(lse.isfinite().all()), alpha
             check_attention(dev, sv, q, out, lse, alpha, True, window)
+    assert dev.device_status() == 0
+
+
+def test_a_wait_that_ran_out_is_reported_before_a_bad_index(cuda_dev):
+    """Both happened: the kernel that gave up on a wait left an output that does not hold, whichever came first."""
+    dev = cuda_dev
+    cache = dev.kv_cache(1, 16, 1, 32)
+    for t in cache:
+        t.zero_() if t.dtype is F32 else t.view(torch.uint8).zero_()
+    bad = torch.tensor([5], dtype=torch.int32).cuda()
+
+    def wait():
+        assert dev.lib.b200_selftest_bounded_wait(200000, None, dev._stream()) == 0
+
+    for calls in ((wait, lambda: dev.kv_cache_read(cache, bad)), (lambda: dev.kv_cache_read(cache, bad), wait)):
+        assert dev.device_status() == 0
+        for call in calls:
+            call()
+        assert dev.device_status() == _lib.ERR_DEVICE_TIMEOUT
+    dev.kv_cache_read(cache, bad)
+    assert dev.device_status() == _lib.ERR_INDEX                          # and by itself a bad index is reported as before
     assert dev.device_status() == 0
