@@ -583,15 +583,24 @@ int b200_attention_backward(int dtype, size_t batch, size_t heads, size_t s1, si
 }
 
 // ---- queries and keys before attention -------------------------------------------------------------
+// The stride of an axis as the kernels take it: no address depends on that of an axis of one element, which may be anything.
+static int take_stride(size_t s, size_t n, bool written, int64_t* to) {
+  *to = 0;
+  if (n <= 1) return B200_OK;
+  if (written && s == 0) return B200_ERR_STRIDE;
+  if (s > ((size_t)1 << 40)) return B200_ERR_LIMIT;
+  *to = (int64_t)s;
+  return B200_OK;
+}
+
 // The pointer and the strides of one (batch, token, head, element) view of an operand that is needed.
-static int check_heads_view(const void* p, const size_t s[4], size_t batch, size_t tokens, size_t heads, bool written) {
+static int check_heads_view(const void* p, const size_t s[4], int64_t to[3], size_t batch, size_t tokens, size_t heads, bool written) {
   if (!p || !s) return B200_ERR_NULL;
   if (s[3] != 1) return B200_ERR_UNSUPPORTED;
   const size_t n[3] = {batch, tokens, heads};
-  for (int i = 0; i < 3; ++i) {
-    if (written && n[i] > 1 && s[i] == 0) return B200_ERR_STRIDE;
-    if (s[i] > ((size_t)1 << 40)) return B200_ERR_LIMIT;
-  }
+  int rc;
+  for (int i = 0; i < 3; ++i)
+    if ((rc = take_stride(s[i], n[i], written, &to[i]))) return rc;
   return B200_OK;
 }
 
@@ -612,13 +621,11 @@ static int qk_norm_rotary_call(int dtype, const b200_head_op* op, size_t batch, 
   const bool empty = batch * tokens == 0;
   for (int i = 0; i < (backward ? 4 : 2); ++i) {
     if (empty || heads[i & 1] == 0) continue;
-    if ((rc = check_heads_view(in[i], in_s[i], batch, tokens, heads[i & 1], false))) return rc;
-    for (int a = 0; a < 3; ++a) is[i][a] = (int64_t)in_s[i][a];
+    if ((rc = check_heads_view(in[i], in_s[i], is[i], batch, tokens, heads[i & 1], false))) return rc;
   }
   for (int i = 0; i < 2; ++i) {
     if (empty || heads[i] == 0) continue;
-    if ((rc = check_heads_view(out[i], out_s[i], batch, tokens, heads[i], true))) return rc;
-    for (int a = 0; a < 3; ++a) os[i][a] = (int64_t)out_s[i][a];
+    if ((rc = check_heads_view(out[i], out_s[i], os[i], batch, tokens, heads[i], true))) return rc;
   }
   if (q_gain_grad || k_gain_grad) {
     if (!workspace || ((uintptr_t)workspace & 15)) return B200_ERR_NULL;
@@ -665,11 +672,9 @@ static int check_token_view(const size_t s[3], int64_t to[2], size_t tokens, siz
   if (!s) return B200_ERR_NULL;
   if (s[2] != 1) return B200_ERR_UNSUPPORTED;
   const size_t n[2] = {tokens, heads};
-  for (int i = 0; i < 2; ++i) {
-    if (written && n[i] > 1 && s[i] == 0) return B200_ERR_STRIDE;
-    if (s[i] > ((size_t)1 << 40)) return B200_ERR_LIMIT;
-    to[i] = (int64_t)s[i];
-  }
+  int rc;
+  for (int i = 0; i < 2; ++i)
+    if ((rc = take_stride(s[i], n[i], written, &to[i]))) return rc;
   return B200_OK;
 }
 

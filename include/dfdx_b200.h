@@ -451,7 +451,8 @@ typedef struct {
 
 /* The transform above on all query and key heads in one pass.  q: (batch, tokens, q_heads, d) view, k: (batch, tokens,
  * k_heads, d) view, likewise the outputs, which may be the inputs themselves; strides [batch, token, head, element], the
- * last one 1, output strides non-zero over extents > 1 (B200_ERR_STRIDE).  positions: int32, axes x batch x tokens
+ * last one 1, output strides non-zero over extents > 1 (B200_ERR_STRIDE); the stride of an axis of one element, here
+ * and in the calls below, may be anything.  positions: int32, axes x batch x tokens
  * contiguous, `axes` being the last axis with rotated pairs; NULL: the index in the sequence, on every axis.
  * f32 and f16 (f32 arithmetic, one rounding); even d <= 256, otherwise B200_ERR_UNSUPPORTED.  q_heads or k_heads may be 0. */
 int b200_qk_norm_rotary_forward(int dtype, const b200_head_op* op, size_t batch, size_t tokens, size_t q_heads, size_t k_heads,

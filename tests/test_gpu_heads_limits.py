@@ -6,9 +6,10 @@ Definitions: tests/heads_reference.py; tolerances as in tests/test_gpu_heads.py 
 import pytest
 import torch
 
+import dfdx_b200
 import heads_reference as ref
 from dfdx_b200 import _lib
-from test_gpu_heads import F32, Serving, check_attention
+from test_gpu_heads import F32, Serving, check_attention, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -60,4 +61,51 @@ def test_a_wait_that_ran_out_is_reported_before_a_bad_index(cuda_dev):
         assert dev.device_status() == _lib.ERR_DEVICE_TIMEOUT
     dev.kv_cache_read(cache, bad)
     assert dev.device_status() == _lib.ERR_INDEX                          # and by itself a bad index is reported as before
+    assert dev.device_status() == 0
+
+
+def test_strides_of_axes_of_one_element(cuda_dev):
+    """No address depends on the stride of an axis of extent 1: one token, one head or one batch entry may have any."""
+    dev = cuda_dev
+    g = gen(93)
+    rotary = dfdx_b200.Rotary(dev.rotary_frequencies((32,)), (32,))
+
+    def odd(t, axis, stride):
+        """t with another stride on an axis of extent 1."""
+        assert t.shape[axis] == 1
+        s = list(t.stride())
+        s[axis] = stride
+        return t.as_strided(t.shape, s)
+
+    sv = Serving(dev, [50], [1], 16, 1, 64, 94)
+    sv.fill([50])
+    for hq, axis in ((4, 0), (1, 0), (1, 1)):
+        t = 1 if axis == 0 else 5
+        sv.new = [t]
+        q = torch.randn(t, hq, 64, generator=g).half().cuda()
+        want, wlse = dev.kv_cache_attention(sv.cache, q, *sv.args(), 0.125, want_lse=True)
+        for stride in (0, 515, (1 << 31) + 1, 1 << 41):
+            out = torch.zeros_like(q)
+            _, lse = dev.kv_cache_attention(sv.cache, odd(q, axis, stride), *sv.args(), 0.125, out=odd(out, axis, stride), want_lse=True)
+            assert torch.equal(out, want) and torch.equal(lse, wlse)
+            a, b = dev.kv_cache(4, 16, 1, 64), dev.kv_cache(4, 16, 1, 64)
+            k, v = (torch.randn(t, 1, 64, generator=g).half().cuda() for _ in range(2))
+            cu, lens, table, most = torch.tensor([0, t], dtype=torch.int32).cuda(), torch.tensor([t], dtype=torch.int32).cuda(), sv.table[:, :1].cuda() * 0, t
+            wq = dev.kv_cache_append(a, k, v, cu, lens, table, most, q=q, rotary=rotary)
+            gq = torch.zeros_like(q)
+            dev.kv_cache_append(b, odd(k, axis, stride), odd(v, axis, stride), cu, lens, table, most, q=odd(q, axis, stride), rotary=rotary,
+                                q_out=odd(gq, axis, stride))
+            assert torch.equal(gq, wq)
+            for x, y in zip(a[:2], b[:2]):
+                assert torch.equal(x[0, :, :t].view(torch.uint8), y[0, :, :t].view(torch.uint8))
+            assert torch.equal(a.k_scale[0], b.k_scale[0]) and torch.equal(a.v_scale[0], b.v_scale[0])
+            x4, k4 = q[None], k[None]
+            wy = dev.qk_norm_rotary_forward(x4, k4, rotary)
+            wd = dev.qk_norm_rotary_backward(x4, k4, x4, k4, rotary)
+            for ax in (0, axis + 1):
+                o = [torch.zeros_like(x) for x in (x4, k4, x4, k4)]
+                xs, ks = odd(x4, ax, stride), odd(k4, ax, stride)
+                dev.qk_norm_rotary_forward(xs, ks, rotary, out=(odd(o[0], ax, stride), odd(o[1], ax, stride)))
+                d = dev.qk_norm_rotary_backward(xs, ks, xs, ks, rotary, out=(odd(o[2], ax, stride), odd(o[3], ax, stride)))
+                assert all(torch.equal(x, y) for x, y in zip((*o[:2], *d), (*wy, *wd)))
     assert dev.device_status() == 0
