@@ -12,8 +12,10 @@
 // j >= pairs hold the pass-through elements 2 j, 2 j + 1 with cos = 1, sin = 0.  S is 8 in the forward of f16 rows that
 // 16-byte accesses fit, else 4.
 //
-// The angle is reduced in turns in f64: position * (frequency / 2 pi) minus its nearest whole number loses
-// 2^-53 * |turns|, nothing that f32 sees for any 32-bit position; the remainder's sine and cosine are f32.
+// The angle is reduced in turns: position * (frequency / 2 pi) minus its nearest whole number, the quotient in two f64
+// parts and the product fused with the subtraction.  (With the quotient and the product rounded to f64 the remainder is off
+// by up to 2^-52 * |turns|: 5e-7 radians at position 2^31 and frequency 1, and more with the frequency.)  What is left is
+// below 2^-50 turns at any 32-bit position and frequencies up to 2^20.  The remainder's sine and cosine are f32.
 // Statistics and products are f32; the one rounding to f16 is the store's.
 #pragma once
 #include "common.cuh"
@@ -211,11 +213,18 @@ template <int S> struct Angle {
   f2 c[S / 2], s[S / 2];
 };
 struct Place { int p0, p1, p2; };
-// cos and sin of pair j at a place, from the pair's turns per position.
-__device__ __forceinline__ double turns_of(const Transform& t, int j) { return __ldg(t.freq + j) * 0.15915494309189535; }
-__device__ __forceinline__ float2 cos_sin(const Transform& t, int j, double per_pos, const Place& p) {
-  double x = (double)(j < t.end0 ? p.p0 : j < t.end1 ? p.p1 : p.p2) * per_pos;
-  x -= rint(x);
+// cos and sin of pair j at a place, from the pair's turns per position (a sum of two).
+struct Turns { double hi, lo; };
+__device__ __forceinline__ Turns turns_of(const Transform& t, int j) {
+  constexpr double INV = 0.15915494309189535, INV_REST = -9.839338337591243e-18;   // 1 / 2 pi
+  const double f = __ldg(t.freq + j), hi = f * INV;
+  return {hi, fma(f, INV_REST, fma(f, INV, -hi))};
+}
+__device__ __forceinline__ float2 cos_sin(const Transform& t, int j, const Turns& per_pos, const Place& p) {
+  const double n = (double)(j < t.end0 ? p.p0 : j < t.end1 ? p.p1 : p.p2);
+  constexpr double WHOLE = 6755399441055744.0;             // 1.5 * 2^52: what is added to it is rounded to a whole number
+  const double turns = fma(n, per_pos.hi, WHOLE) - WHOLE;
+  const double x = fma(n, per_pos.lo, fma(n, per_pos.hi, -turns));
   float2 r;
   sincospif(2.f * (float)x, &r.y, &r.x);
   return r;
@@ -228,7 +237,7 @@ __device__ __forceinline__ void fill_table(const Transform& t, float2* table, in
   const int j0 = threadIdx.x % lead, i0 = threadIdx.x / lead, stride = NT / lead;
   if (i0 >= stride) return;
   for (int j = j0; j < t.pairs; j += lead) {
-    const double per_pos = turns_of(t, j);
+    const Turns per_pos = turns_of(t, j);
     for (int i = i0; i < n; i += stride) table[i * t.pairs + j] = cos_sin(t, j, per_pos, place_at(i));
   }
 }

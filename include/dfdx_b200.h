@@ -437,7 +437,8 @@ int b200_softmax_backward(int dtype, size_t rows, size_t cols, const void* y, si
  * interleaved != 0; the elements behind the rotated ones pass through.  The first axis_pairs[0] pairs turn with position
  * axis 0, the next axis_pairs[1] with axis 1, the others with axis 2 (e.g. time, height, width); a text model uses one axis.
  *   frequencies : device pointer, radians per position of each pair in f64 (NULL without rotated pairs).  The angle is
- *                 reduced in f64, so any 32-bit position is as exact as position 0.
+ *                 reduced in f64 with a second part for what f64 rounds off, so any 32-bit position is as exact as
+ *                 position 0 (frequencies up to 2^20).
  *   q_gain, k_gain : d elements of the call's dtype each, or NULL for 1; only with normalize. */
 typedef struct {
   const double* frequencies;

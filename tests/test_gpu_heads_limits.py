@@ -3,13 +3,15 @@ ends of 32 bits, strides that no address depends on, many sequences, the forms o
 
 Definitions: tests/heads_reference.py; tolerances as in tests/test_gpu_heads.py unless a test derives its own.
 """
+from fractions import Fraction
+
 import pytest
 import torch
 
 import dfdx_b200
 import heads_reference as ref
 from dfdx_b200 import _lib
-from test_gpu_heads import F32, Serving, check_attention, gen
+from test_gpu_heads import F32, U, Serving, check_attention, gen, within
 
 pytestmark = pytest.mark.gpu
 
@@ -108,4 +110,46 @@ def test_strides_of_axes_of_one_element(cuda_dev):
                 dev.qk_norm_rotary_forward(xs, ks, rotary, out=(odd(o[0], ax, stride), odd(o[1], ax, stride)))
                 d = dev.qk_norm_rotary_backward(xs, ks, xs, ks, rotary, out=(odd(o[2], ax, stride), odd(o[3], ax, stride)))
                 assert all(torch.equal(x, y) for x, y in zip((*o[:2], *d), (*wy, *wd)))
+    assert dev.device_status() == 0
+
+
+TWO_PI = Fraction("6.28318530717958647692528676655900576839433879875021164194988918461563281257241799726")
+
+
+def exact_angles(positions, frequencies):
+    """position * frequency less its whole turns, (positions, pairs), from exact products and 80 digits of 2 pi."""
+    def angle(p, f):
+        turns = Fraction(p) * Fraction(f) / TWO_PI
+        return float((turns - round(turns)) * TWO_PI)
+    return torch.tensor([[angle(p, f) for f in frequencies] for p in positions], dtype=torch.float64)
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotation_at_the_ends_of_32_bits(cuda_dev, inter):
+    """Positions up to +-2^31 at frequencies of 2^-12 to 2^10 radians are as exact as position 0.
+
+    Tolerance: the remainder in turns, at most 1/2, is rounded to f32 (2^-25: pi u of angle, u = 2^-24), sine and cosine
+    are within an ulp (at most 2 u), the first product is rounded (u) and the sum (u of |a| + |b| at most): 8 u (|a| + |b|)
+    covers their 3.15 + 2 + 1 + 1."""
+    dev = cuda_dev
+    g = gen(91)
+    pos = [0, 1, -1, 1 << 20, (1 << 27) + 1, (1 << 30) - 1, -(1 << 30) - 7, (1 << 31) - 1, -(1 << 31), 2147480001, -2000000011]
+    f = torch.exp2(22 * torch.rand(16, generator=g, dtype=torch.float64) - 12)
+    f[0], f[1] = 1.0, 1024.0
+    want_angle = exact_angles(pos, f.tolist())
+    n = len(pos)
+    q, k = (torch.randn(n, h, 32, generator=g) for h in (3, 2))
+    rotary = dfdx_b200.Rotary(f.cuda(), (16,), inter)
+    p = torch.tensor(pos, dtype=torch.int64).to(torch.int32).cuda()
+    yq, yk = dev.qk_norm_rotary_forward(q.cuda()[None], k.cuda()[None], rotary, p[None, None], norm=False)
+    dq, dk, _, _ = dev.qk_norm_rotary_backward(q.cuda()[None], k.cuda()[None], q.cuda()[None], k.cuda()[None], rotary, p[None, None], norm=False)
+    cache = dev.kv_cache(1, 16, 2, 32)
+    cu, lens, table = (torch.tensor(t, dtype=torch.int32).cuda() for t in ([0, n], [n], [[0]]))
+    aq = dev.kv_cache_append(cache, k.cuda(), k.cuda(), cu, lens, table, n, q=q.cuda(), rotary=rotary, positions=p[None])
+    for x, sign, got in ((q, 1, yq[0]), (k, 1, yk[0]), (q, -1, dq[0]), (k, -1, dk[0]), (q, 1, aq)):
+        want = ref.transform(x.double(), None, False, 0.0, sign * want_angle, inter)
+        size = x.double().abs()
+        size = size[..., 0::2] + size[..., 1::2] if inter else size[..., :16] + size[..., 16:]
+        size = size.repeat_interleave(2, -1) if inter else torch.cat((size, size), -1)
+        within(got, want, 8 * U * size, "rotated")
     assert dev.device_status() == 0
