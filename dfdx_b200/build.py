@@ -8,8 +8,9 @@ Each .cu is compiled to an object in `dfdx_b200/lib/obj/` (in parallel), then li
 the one driver entry point the library needs (tensor-map encoding) is resolved at run time, so the
 library loads on a machine without a GPU driver.
 
-`py_heads.cpp`, the host side of heads.py, becomes the Python module `dfdx_b200/lib/_heads.so` (g++, against torch's headers);
-it calls the library through addresses that it is given and is not linked to it.  Where it cannot be built (no C++ headers of
+`py_heads.cpp`, the host side of heads.py, becomes a Python module in `dfdx_b200/lib/` (g++, against torch's headers), named
+after the torch and Python whose binary interface it has, so that no other ones load it; it calls the library through addresses
+that it is given and is not linked to it.  Where it cannot be built (no C++ headers of
 Python or torch) the library is made all the same, with a warning; the calls of heads.py then raise.
 """
 from __future__ import annotations
@@ -27,7 +28,6 @@ CSRC = PKG / "csrc"
 LIBDIR = PKG / "lib"
 OBJDIR = LIBDIR / "obj"
 LIB = LIBDIR / "libdfdx_b200.so"
-MODULE = LIBDIR / "_heads.so"
 SOURCES = ["api.cu", "gemm_simt.cu", "gemm_tc.cu", "gemm_tc_pair.cu", "conv2d.cu", "attention.cu", "attention_bwd.cu", "rowwise.cu",
            "rotary.cu", "kv_cache.cu", "kv_attention.cu", "kv_attention_tc.cu"]
 NVCC_FLAGS = [
@@ -63,18 +63,24 @@ def _compile(src: str, force: bool) -> Path:
     return obj
 
 
-def _build_module(force: bool) -> None:
-    src = CSRC / "py_heads.cpp"
-    if not force and MODULE.exists() and MODULE.stat().st_mtime >= max(src.stat().st_mtime, (PKG.parent / "include" / "dfdx_b200.h").stat().st_mtime):
-        return
-    MODULE.unlink(missing_ok=True)              # none rather than that of an earlier source
+def module_path() -> Path:
+    """The compiled host side of heads.py for the running Python and its torch."""
     import torch
+    return LIBDIR / f"_heads.torch-{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}"
+
+
+def _build_module(force: bool) -> None:
+    import torch
+    src, module = CSRC / "py_heads.cpp", module_path()
+    if not force and module.exists() and module.stat().st_mtime >= max(src.stat().st_mtime, (PKG.parent / "include" / "dfdx_b200.h").stat().st_mtime):
+        return
+    module.unlink(missing_ok=True)              # none rather than that of an earlier source
     root = Path(torch.__file__).resolve().parent
     nvcc = Path(_nvcc())
     cuda = nvcc.resolve().parent.parent / "include" if nvcc.is_absolute() else Path("/usr/local/cuda/include")
     include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda, Path(sysconfig.get_paths()["include"])]
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-isystem{p}" for p in include), str(src), "-o", str(MODULE), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}",
+           *(f"-isystem{p}" for p in include), str(src), "-o", str(module), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}",
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
@@ -95,7 +101,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     try:
         module.result()
     except (RuntimeError, ImportError, OSError) as e:
-        warnings.warn(f"{MODULE.name}, the host side of heads.py, was not built: {e}", RuntimeWarning)
+        warnings.warn(f"py_heads.cpp, the host side of heads.py, was not built: {e}", RuntimeWarning)
     if verbose:
         print(f"built {LIB}")
     return LIB

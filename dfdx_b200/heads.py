@@ -43,10 +43,12 @@ _module = None
 
 
 def _host():
-    """The compiled host side (csrc/py_heads.cpp), bound to the library's entry points.  Raises if it is missing."""
+    """The compiled host side (csrc/py_heads.cpp), bound to the library's entry points.  Raises if it is missing, also where
+    there is one for another torch or Python."""
     global _module
     if _module is None:
-        path = _lib.LIB_PATH.parent / "_heads.so"
+        from .build import module_path
+        path = module_path()
         if not path.exists():
             raise RuntimeError(f"{path} is missing: build it with `python -m dfdx_b200.build`")
         loader = importlib.machinery.ExtensionFileLoader("_heads", str(path))

@@ -2,9 +2,9 @@
 import subprocess
 
 import pytest
-import torch  # noqa: F401  (imported before subprocess.run is replaced)
+import torch
 
-from dfdx_b200 import build
+from dfdx_b200 import build, heads
 
 
 @pytest.fixture
@@ -27,8 +27,7 @@ def tools(tmp_path, monkeypatch):
     t = Tools()
     monkeypatch.setattr(build, "LIBDIR", tmp_path)
     monkeypatch.setattr(build, "OBJDIR", tmp_path / "obj")
-    for name in ("LIB", "MODULE"):
-        monkeypatch.setattr(build, name, tmp_path / getattr(build, name).name)
+    monkeypatch.setattr(build, "LIB", tmp_path / build.LIB.name)
     monkeypatch.setattr(build.subprocess, "run", t.run)
     return t
 
@@ -36,10 +35,10 @@ def tools(tmp_path, monkeypatch):
 @pytest.mark.parametrize("why", ["fatal error: Python.h: No such file or directory", FileNotFoundError("g++")])
 def test_the_library_is_made_without_the_python_module(tools, why):
     tools.failing["g++"] = why
-    build.MODULE.write_text("of an earlier source")
+    build.module_path().write_text("of an earlier source")
     with pytest.warns(RuntimeWarning, match="was not built"):
         assert build.build(force=True) == build.LIB
-    assert build.LIB.exists() and not build.MODULE.exists()
+    assert build.LIB.exists() and not build.module_path().exists()
 
 
 def test_a_failing_library_is_an_error(tools):
@@ -51,7 +50,25 @@ def test_a_failing_library_is_an_error(tools):
 
 def test_both_are_made_and_then_kept(tools):
     build.build()
-    assert build.LIB.exists() and build.MODULE.exists()
+    assert build.LIB.exists() and build.module_path().exists()
     n = len(tools.commands)
     build.build()
     assert len(tools.commands) == n
+
+
+def test_a_module_of_another_torch_is_neither_kept_nor_loaded(tools, monkeypatch):
+    build.build()
+    before, n = build.module_path(), len(tools.commands)
+    monkeypatch.setattr(heads, "_module", None)
+    monkeypatch.setattr(torch, "__version__", "99.0.1")
+    assert build.module_path() != before
+    with pytest.raises(RuntimeError, match="is missing"):
+        heads._host()
+    build.build()
+    assert [c[0] for c in tools.commands[n:]] == ["g++"] and build.module_path().exists() and before.exists()
+
+
+def test_the_module_is_named_after_the_python(monkeypatch):
+    before = build.module_path()
+    monkeypatch.setattr(build.sysconfig, "get_config_var", lambda name: ".cpython-399.so")
+    assert build.module_path() != before and build.module_path().name.endswith(".cpython-399.so")
