@@ -11,7 +11,8 @@ import torch
 import dfdx_b200
 import heads_reference as ref
 from dfdx_b200 import _lib
-from test_gpu_heads import F32, U, Serving, check_attention, gen, within
+from test_gpu_heads import F16, F32, U, Serving, check_attention, gen, within
+from test_gpu_heads import test_append as check_append
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +154,75 @@ def test_rotation_at_the_ends_of_32_bits(cuda_dev, inter):
         size = size.repeat_interleave(2, -1) if inter else torch.cat((size, size), -1)
         within(got, want, 8 * U * size, "rotated")
     assert dev.device_status() == 0
+
+
+@pytest.mark.parametrize("seqs", [40, 991, 993, 2500])
+@pytest.mark.parametrize("most", [1, 3])
+def test_append_of_many_sequences(cuda_dev, seqs, most):
+    """More sequences than one look of a warp, or two, narrows down to one; runs of sequences without new tokens, tokens of
+    no sequence in front and behind."""
+    dev = cuda_dev
+    g = gen(95 + seqs)
+    new = torch.randint(0, most + 1, (seqs,), generator=g)
+    new[seqs // 3:seqs // 3 + 35] = 0
+    new[:2] = 0
+    new[-3:-1] = 0
+    past = torch.randint(0, 40, (seqs,), generator=g)
+    lead, tail, page = 5, 9, 16
+    t = lead + int(new.sum()) + tail
+    lens = past + new
+    table = torch.randperm(4 * seqs + 7, generator=g)[:4 * seqs].view(seqs, 4)
+    cache = dev.kv_cache(4 * seqs + 7, page, 2, 32)
+    cu = lead + torch.cat([torch.zeros(1, dtype=torch.int64), new.cumsum(0)])
+    on = lambda x: x.to(torch.int32).cuda()
+    for x in cache[:2]:
+        x.view(torch.uint8).fill_(0x7F)
+    # the earlier slots, through appends of at most 20 sequences
+    for s0 in range(0, seqs, 20):
+        p = past[s0:s0 + 20]
+        c = torch.cat([torch.zeros(1, dtype=torch.int64), p.cumsum(0)])
+        if int(c[-1]):
+            old = torch.zeros(int(c[-1]), 2, 32).half().cuda()
+            dev.kv_cache_append(cache, old, old, on(c), on(p), on(table[s0:s0 + 20]), int(p.max()))
+    held = [x.view(torch.uint8).cpu() for x in cache[:2]]
+    q, k, v = (torch.randn(t, h, 32, generator=g).half().cuda() for h in (3, 2, 2))
+    rotary = dfdx_b200.Rotary(dev.rotary_frequencies((16,)), (16,))
+    out = torch.full_like(q, 7.0)
+    dev.kv_cache_append(cache, k, v, on(cu), on(lens), on(table), most, q=q, rotary=rotary, q_out=out)
+    assert dev.device_status() == 0
+    owner = torch.arange(seqs).repeat_interleave(new)
+    slot = torch.cat([torch.arange(int(p), int(p + m)) for p, m in zip(past, new)])
+    mine = slice(lead, t - tail)
+    wq, wk = dev.qk_norm_rotary_forward(q[None, mine], k[None, mine], rotary, on(slot)[None, None], norm=False)
+    assert torch.equal(out[mine], wq[0]) and bool((out[:lead] == 7.0).all()) and bool((out[t - tail:] == 7.0).all())
+    ids, row = table[owner, slot // page], slot % page
+    for c, want in enumerate((wk[0], v[mine])):
+        want = want.cpu().double()
+        scale = cache[2 + c].cpu().double()[ids][..., None]
+        got = cache[c].cpu()[ids, :, row].double() * scale
+        # half a code; the keys' want is itself rounded to f16
+        within(got, want, torch.maximum(2.0 ** -4 * want.abs(), 2.0 ** -10 * scale) * (1 + 2.0 ** -6) + 2.0 ** -10 * want.abs(), f"codes {c}")
+        same = torch.ones(held[c].shape[0], page, dtype=torch.bool)
+        same[ids, row] = False
+        same[ids[row > 0]] = False                                        # blocks whose scale may have grown under zeros
+        fresh = same[:, :, None].expand(-1, -1, 2).transpose(1, 2)
+        assert torch.equal(cache[c].view(torch.uint8).cpu()[fresh], held[c][fresh])
+
+
+APPEND = [  # dtype, page, heads, q_heads, d, past, new, pairs, interleaved, norm: forms that the cases of test_gpu_heads.py leave out
+    (F32, 64, 2, 4, 128, [63, 64, 0, 5], [1, 1, 1, 1], 64, False, True),              # single tokens: f32,
+    (F32, 16, 3, 6, 64, [15, 16, 0, 33, 7], [1, 1, 1, 1, 0], 32, True, True),         # adjacent pairs, an empty sequence,
+    (F16, 32, 2, 6, 96, [31, 0, 40], [1, 1, 1], 48, True, False),
+    (F32, 128, 1, 5, 96, [127, 3, 200], [1, 1, 1], 30, False, True),                  # pairs no multiple of 4: element access,
+    (F16, 16, 5, 5, 32, [9, 0, 15], [1, 1, 1], 7, True, True),
+    (F32, 16, 7, 7, 64, [5 * i % 50 for i in range(90)], [1] * 90, 16, True, False),  # several heads a CTA
+    (F32, 128, 2, 2, 128, [0, 100, 127], [300, 28, 2], 64, True, True),               # f32 with the largest pages
+    (F32, 128, 1, 3, 64, [60, 0], [140, 257], 32, False, True),
+    (F32, 128, 2, 2, 96, [1, 130], [129, 90], 25, False, True),
+    (F16, 128, 3, 3, 128, [5], [300], 13, True, True),
+]
+
+
+@pytest.mark.parametrize("case", APPEND, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c)[:80])
+def test_append_forms(cuda_dev, case):
+    check_append(cuda_dev, case)
