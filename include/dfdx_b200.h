@@ -496,7 +496,7 @@ typedef struct {
  * table behind a sequence's length are never read.  max_new: the most new tokens that a sequence has.  A sequence whose
  * numbers do not fit (cu_tokens outside [0, tokens] or falling, more than max_new tokens, a length outside
  * [0, max_pages * page_size] or above 2^30), and a page outside the cache, are skipped and reported as B200_ERR_INDEX by
- * b200_device_status; where cu_tokens fall, sequences behind that place may be skipped too.  Tokens of no sequence are
+ * b200_device_status; where cu_tokens fall, tokens of other sequences may be skipped too.  Tokens of no sequence are
  * left alone, in outputs too. */
 typedef struct {
   size_t seqs, tokens, max_new;

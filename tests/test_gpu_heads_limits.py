@@ -209,6 +209,43 @@ def test_append_of_many_sequences(cuda_dev, seqs, most):
         assert torch.equal(cache[c].view(torch.uint8).cpu()[fresh], held[c][fresh])
 
 
+def test_append_leaves_what_does_not_fit_untouched(cuda_dev):
+    """Bounds that do not fit: the sequences' tokens, pages and the rows around the buffers stay as they were."""
+    dev = cuda_dev
+    sv = Serving(dev, [10, 10, 10], [2, 2, 2], 16, 1, 32, 96)
+    sv.fill([8, 8, 8])
+    cu, lens, table, most = sv.args()
+    x = torch.randn(10, 1, 32, generator=sv.g).half().cuda()[2:8]
+    owned = {int(p) for p in sv.table.flatten()}
+    spare = [i for i in range(sv.cache.k.shape[0]) if i not in owned]
+    assert spare
+    for bad_cu, bad_lens, skipped in (([0, 2, 1, 6], None, (1, 2)), ([0, 2, 9, 6], None, (1, 2)), ([-1, 2, 4, 6], None, (0,)), ([0, 2, 4, 7], None, (2,)),
+                                      ([0, 2, 4, 1 << 30], None, (2,)), (None, [10, 1, 10], (1,)), (None, [10, 17, 10], (1,)), (None, [10, -3, 10], (1,))):
+        held = [t.view(torch.uint8).clone() for t in sv.cache]
+        buf = torch.full((12, 1, 32), 7.0, dtype=F16, device="cuda")
+        c = torch.tensor(bad_cu, dtype=torch.int32).cuda() if bad_cu else cu
+        n = torch.tensor(bad_lens, dtype=torch.int32).cuda() if bad_lens else lens
+        dev.kv_cache_append(sv.cache, x, x, c, n, table, most, q=x, q_out=buf[3:9])
+        assert dev.device_status() == _lib.ERR_INDEX
+        assert bool((buf[:3] == 7.0).all()) and bool((buf[9:] == 7.0).all())
+        out = buf[3:9]
+        falling = bad_cu is not None and sorted(bad_cu) != bad_cu          # then other sequences' tokens may be skipped too
+        for s in range(3):
+            rows = slice(2 * s, 2 * s + 2)
+            done = (out[rows] == x[rows]).all(-1)
+            left = (out[rows] == 7.0).all(-1)
+            assert bool((done | left).all())
+            assert falling or bool((left if s in skipped else done).all()), (bad_cu, bad_lens, s)
+            if s in skipped:
+                for was, now in zip(held, sv.cache):
+                    p = int(sv.table[s, 0])
+                    assert torch.equal(was[p], now.view(torch.uint8)[p]), (bad_cu, bad_lens, s)
+        for was, now in zip(held, sv.cache):
+            assert torch.equal(was[spare], now.view(torch.uint8)[spare])
+    dev.kv_cache_append(sv.cache, x, x, cu, lens, table, most)
+    assert dev.device_status() == 0
+
+
 APPEND = [  # dtype, page, heads, q_heads, d, past, new, pairs, interleaved, norm: forms that the cases of test_gpu_heads.py leave out
     (F32, 64, 2, 4, 128, [63, 64, 0, 5], [1, 1, 1, 1], 64, False, True),              # single tokens: f32,
     (F32, 16, 3, 6, 64, [15, 16, 0, 33, 7], [1, 1, 1, 1, 0], 32, True, True),         # adjacent pairs, an empty sequence,
