@@ -3,6 +3,7 @@ ends of 32 bits, strides that no address depends on, many sequences, the forms o
 
 Definitions: tests/heads_reference.py; tolerances as in tests/test_gpu_heads.py unless a test derives its own.
 """
+import math
 from fractions import Fraction
 
 import pytest
@@ -43,6 +44,38 @@ def test_attention_with_a_factor_of_zero(cuda_dev, new, window):
             out, lse = dev.kv_cache_attention(sv.cache, q, *sv.args(), alpha, window=window, want_lse=True)
             assert bool(out.isfinite().all()) and bool(lse.isfinite().all()), alpha
             check_attention(dev, sv, q, out, lse, alpha, True, window)
+    assert dev.device_status() == 0
+
+
+@pytest.mark.parametrize("new", [3, 45])
+def test_log_sum_exp_beside_values_of_another_size(cuda_dev, new):
+    """Value scales 2^116 apart, the most that is promised: a block of zeros (2^-60) whose slots weigh 2^-20 to 2^100 times as
+    much as those of blocks of values up to 448 * 2^56.  (The outputs are no matter here: values of 2^65 and scores that differ by up to 2^60 leave f16.)"""
+    dev = cuda_dev
+    n = 32 + new
+    sv = Serving(dev, [n], [n], 16, 1, 64, 97)
+    k, v = (torch.randn(n, 1, 64, generator=sv.g) for _ in range(2))
+    v = v.clamp(-1, 1) * 448 * 2.0 ** 56
+    v[16:, 0, 0] = 448 * 2.0 ** 56
+    v[:16] = 0.0
+    k[:, 0, 0] = 0.0
+    k[:16, 0, 0] = 1.0
+    dev.kv_cache_append(sv.cache, k.cuda(), v.cuda(), *sv.args())
+    scales = sv.cache.v_scale.cpu()[sv.table[0].long(), 0]
+    assert float(scales[0]) == ref.MIN_SCALE and bool((scales[1:] == 2.0 ** 56).all())
+    sv.new = [new]
+    heads = (-20, 0, 10, 50, 100)
+    q = torch.randn(new, len(heads), 64, generator=sv.g)
+    q[..., 0] = torch.tensor(heads, dtype=torch.float32)
+    q = q.half().cuda()
+    alpha = math.log(2.0)
+    _, lse = dev.kv_cache_attention(sv.cache, q, *sv.args(), alpha, want_lse=True)
+    kk, vv = sv.rows(0, n)
+    vis = torch.arange(n)[None] <= torch.arange(n - new, n)[:, None]
+    _, want, _ = ref.attention(q.cpu().double(), kk, vv, alpha, vis)
+    # a score of 64 products in f32: off by 64 u of the sum of their magnitudes, 100 + 64 * 5 * 5 at most
+    assert float(q[..., 1:].abs().max()) < 5 and float(k.abs().max()) < 5
+    within(lse, want, 2 * 64 * U * alpha * (100 + 64 * 25) + 2.0 ** -19 + 4 * U * want.abs(), "lse")
     assert dev.device_status() == 0
 
 
