@@ -189,6 +189,22 @@ def test_rotation_at_the_ends_of_32_bits(cuda_dev, inter):
     assert dev.device_status() == 0
 
 
+def test_sines_and_cosines(cuda_dev):
+    """A pair (1, 0) turns into its cosine and sine themselves.  They are CUDA's of the angle's f32 part, within an ulp (2^-24
+    below 1), plus the rest's share, rounded once (half an ulp): 1.5 u."""
+    dev = cuda_dev
+    g = gen(92)
+    f = torch.exp2(-12 * torch.rand(16, generator=g, dtype=torch.float64))
+    pos = torch.randint(-(1 << 31), 1 << 31, (400,), generator=g)
+    pos = torch.where(torch.arange(400) % 2 == 0, pos, pos % 9000)
+    angle = exact_angles(pos.tolist(), f.tolist())
+    want = torch.cat((angle.cos(), angle.sin()), -1)[:, None]
+    x = torch.cat((torch.ones(400, 1, 16), torch.zeros(400, 1, 16)), -1)
+    p = pos.to(torch.int32).cuda()
+    y, _ = dev.qk_norm_rotary_forward(x.cuda()[None], x[:, :0].cuda()[None], dfdx_b200.Rotary(f.cuda(), (16,)), p[None, None], norm=False)
+    within(y[0], want, 1.5 * U, "cosine and sine")
+
+
 @pytest.mark.parametrize("seqs", [40, 991, 993, 2500])
 @pytest.mark.parametrize("most", [1, 3])
 def test_append_of_many_sequences(cuda_dev, seqs, most):
