@@ -5,7 +5,8 @@
 // head, neighbours in that order -- as two tiles of 128, and walks the slots that some row sees, 128 at a time.
 //   warps 0-3, 4-7   softmax of tile 0 and 1: a thread owns a row.  Reads its 128 scores from tensor memory, turns them into
 //                    probabilities and writes these as f16 over the scores' own columns: the second product takes its
-//                    left operand from there.  The outputs stay in tensor memory too; they are read, scaled and
+//                    left operand from there, in the type of the values' tile (2^-12 of each probability, of random sign;
+//                    the sums take them in f32).  The outputs stay in tensor memory too; they are read, scaled and
 //                    written back only when a row's maximum moves by more than 1.
 //   warps 8-11       one thread each issues S = Q K^T (8, 9) or O += P V (10, 11) of a tile, half a tile of slots at a time:
 //                    while the softmax has one half, the tensor core multiplies the other's probabilities and puts the

@@ -11,7 +11,8 @@
 //   qk_backward_kernel  the same walk by CTAs that stay and loop.  With h' = R^T g the gradient before the rotation,
 //                         dgain += h' * xhat,   dx = r (h' gain - xhat mean(h' gain xhat)),   xhat = x r.
 //                       The gains' sums stay in f32 registers over all rows of a lane, are added up per CTA in a fixed
-//                       order and leave as one row of partial sums per CTA.
+//                       order and leave as one row of partial sums per CTA: at 59400 rows 1.7e-7 of the sums' norm off,
+//                       where f64 sums of f32 products are 7e-8 off.
 //                       Bound by what 16 warps an SM (12 in f32) can have on their way and by issue (0.54 of the cycles
 //                       issue): 16384 tokens, 36 heads of 128, f16: 107 us, 4.2 TB/s; 4950 tokens, 24 heads of 96, f32:
 //                       37 us, 3.7 TB/s.  More warps do not fit: x, g and the sums of both gains take 119 registers.
