@@ -1,7 +1,7 @@
 // The host side of heads.py: checks a call's tensors, allocates its results and workspace from torch, lays its structs out
 // and calls the C ABI.  A decoding step's kernels take a few microseconds each, and the same work in Python (attribute
-// lookups, tuples, ctypes objects) took 13 to 18 microseconds a call; here a call takes 5 to 6.5 of host time, two torch
-// allocations (1.8 each) and the launch included, the backward with five allocations and two launches 11.
+// lookups, tuples, ctypes objects) took 13 to 18 microseconds a call; here a call takes 5 to 6.5 of host time, its
+// results' allocation and the launch included, the backward with five allocations and two launches 11.
 //
 // The entry points come as addresses from the ctypes binding (bind), so that this module and _lib.py use one library.
 // No C++ exception leaves a function: whatever is thrown becomes a Python one.
