@@ -527,7 +527,8 @@ int b200_kv_cache_read(int dtype, const b200_kv_cache* cache, size_t n, const in
  * the last `window` ones if window != 0; or all seq_lens[s] slots (causal == 0, no window).  q, out: (tokens, q_heads,
  * d) views, strides [token, head, element] with the last 1 and the others multiples of 8, 16-byte aligned; q_heads a
  * multiple of the cache's heads, query head h reads key head h / (q_heads / heads).  lse: NULL or tokens x q_heads floats,
- * log(sum exp(alpha * s)).  A token that sees no slot gets zeros and -infinity.  f16 / AMP f16 only; f32 softmax and sums,
+ * log(sum exp(alpha * s)).  A token that sees no slot, or none whose score is above -infinity, gets zeros
+ * and -infinity.  f16 / AMP f16 only; f32 softmax and sums,
  * probabilities rounded to f16 for the product with the values.  These carry their block's value scale: an output is off by
  * up to 2^-38 of the largest value in a visible block for each slot, and slots whose value scale is more than 2^116 below
  * another visible block's may drop out of the sums and of lse (f32 values above 2^64 beside zeros; no f16 values).
